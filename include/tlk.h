@@ -830,6 +830,63 @@ int tlk_reid_part_head(const void *feat_dev, int feat_pix_stride, int dtype, int
                        const int32_t *counts_dev, const int32_t *slot_base_dev, int rows, int max_dets, float vis_threshold,
                        float *emb_dev, unsigned char *vis_dev, unsigned char *nonfinite_flag_dev, void *hip_stream);
 
+/* ------------------------------------------------------------------------------------------
+ * The gated attention unit's operators: attention whose score carries a bias learned per bucket of the distance between key and query,
+ * gated, with its gradients; and the joint of two blocks (norm, gate, scaled residual, next norm), with its gradients.  They stand for
+ * the RTMCC head's unit of the pose networks behind tracklab/wrappers/pose_estimator/rtmlib_api.py:15-33 (ScaleNorm, relu^2 attention,
+ * gate, residual scale; there an eager composition) and carry what such a unit needs for longer sequences, caches and fine-tuning.
+ *
+ * tlk_gau_attention_fwd:  S[i,j] = scale * q[i] . k[j] + table[bucket_of[clip(j - (i + start_b), -D, D) + D]][h]
+ *                         W = relu(S)^2 (TLK_GAU_RELU2) or softmax over j (TLK_GAU_SOFTMAX);  o = W v;  out = gate * o (out = o without a gate)
+ *   over the keys j < lens[b] (all len_k without lens; lens is clipped to 0..len_k) and, when causal, j <= i + start_b; start_b = q_start_dev[b],
+ *   or q_start.  A row that sees no key gives zeros.  Keys at or behind lens[b] are not read.  Head h reads key / value head h / (heads / kv_heads).
+ *   q (batch, len_q, heads, dim_k), k (batch, len_k, kv_heads, dim_k), v (.., dim_v), gate (batch, len_q, heads, dim_v): strides in elements for
+ *   batch, row and head, the last dimension contiguous; every stride a multiple of 16 bytes, every pointer 16-byte aligned; dim_k <= 128 and dim_v
+ *   multiples of 16 bytes of elements.  table (num_buckets, heads) of `dtype` or (table_f32) float32, bucket_of (2 * max_distance + 1) int32 (values are clipped to
+ *   0..num_buckets - 1); num_buckets 0: no bias.  max_distance <= 2048.  out, o_raw, dq.. are contiguous (batch, len, heads, dim).
+ *   o_raw (nullable): o before the gate, lse (nullable, softmax): log2 sum_j 2^(S log2 e) per (batch, len_q, heads), +inf for a row without keys: what
+ *   the backward call takes.  Products run on the matrix cores in `dtype` and are summed in float32; weights are rounded to `dtype` for the second product
+ *   (float16: with a power of two per row, so weights beyond its range survive), o and out once.
+ * tlk_gau_attention_bwd:  dout, o_raw (needed with a gate or softmax), lse (softmax) -> dq, dk, dv, dgate (with a gate), dtable (with a table); weights
+ *   are formed again from q and k.  With shared key heads the gradients of the sharing heads are summed in float32.  No atomics: equal bits on every run.
+ * Workspace: device memory of at least tlk_gau_attention_workspace(args, backward) bytes (-1..: an error code), not shared by calls that may overlap. */
+enum { TLK_GAU_RELU2 = 0, TLK_GAU_SOFTMAX = 1 };
+typedef struct {
+    int32_t dtype, kind, causal, table_f32;
+    int32_t batch, len_q, len_k, heads, kv_heads, dim_k, dim_v;
+    int32_t num_buckets, max_distance, q_start;
+    float scale;
+    int64_t q_stride[3], k_stride[3], v_stride[3], gate_stride[3];
+    const void *q, *k, *v, *gate, *table;
+    const int32_t *bucket_of, *lens, *q_start_dev;
+} tlk_gau_args;
+long long tlk_gau_attention_workspace(const tlk_gau_args *args, int backward);
+int tlk_gau_attention_fwd(const tlk_gau_args *args, void *out_dev, void *o_raw_dev, float *lse_dev, void *workspace_dev, long long workspace_bytes,
+                          void *hip_stream);
+int tlk_gau_attention_bwd(const tlk_gau_args *args, const void *dout_dev, const void *o_raw_dev, const float *lse_dev, void *dq_dev, void *dk_dev,
+                          void *dv_dev, void *dgate_dev, void *dtable_dev, void *workspace_dev, long long workspace_bytes, void *hip_stream);
+
+/* tlk_norm_gate_residual_fwd:  y = res_scale * x + gate * N1(h),  z = N2(y) (z only with next_norm), over rows of `dim` values (<= 8192), one HBM pass.
+ *   N: TLK_NORM_SCALE v * weight[0] / max(|v| / sqrt(dim), eps), TLK_NORM_RMS v * weight / sqrt(mean v^2 + eps), TLK_NORM_LAYER (with weight, bias nullable),
+ *   TLK_NORM_NONE.  x, res_scale (dim), gate are nullable; gate row r / gate_rows belongs to row r (1: a gate for every row, rows: one vector).  Rows of
+ *   h, x and gate may be strided; y, z and the gradients are contiguous.  All tensors of `dtype`; arithmetic in float32, y enters N2 unrounded.
+ * tlk_norm_gate_residual_bwd: dy, dz (nullable: zero) -> gradients; statistics are formed again.  dh always, dx with x, dgate with a gate, a parameter's
+ *   gradient with the parameter.  Column sums in float32 in a fixed order (no atomics). */
+enum { TLK_NORM_NONE = 0, TLK_NORM_SCALE = 1, TLK_NORM_RMS = 2, TLK_NORM_LAYER = 3 };
+typedef struct {
+    int32_t dtype, norm, next_norm, dim;
+    int64_t rows, gate_rows, h_stride, x_stride, gate_stride;
+    float eps, next_eps;
+    const void *h, *x, *gate, *res_scale, *weight, *bias, *next_weight, *next_bias;
+} tlk_norm_args;
+typedef struct {
+    void *dh, *dx, *dgate, *dres_scale, *dweight, *dbias, *dnext_weight, *dnext_bias;
+} tlk_norm_grads;
+int tlk_norm_gate_residual_fwd(const tlk_norm_args *args, void *y_dev, void *z_dev, void *hip_stream);
+long long tlk_norm_gate_residual_workspace(const tlk_norm_args *args);
+int tlk_norm_gate_residual_bwd(const tlk_norm_args *args, const void *dy_dev, const void *dz_dev, const tlk_norm_grads *grads, void *workspace_dev,
+                               long long workspace_bytes, void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

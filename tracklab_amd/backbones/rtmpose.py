@@ -22,6 +22,9 @@ from .common import ConvBiasAct, epilogue_, finalize, param_key, random_init_, s
 USE_TLK_DWCONV = _os.environ.get("TLK_DWCONV", "1") != "0"
 # the 7 x 7 keypoint-map convolution on the 8 x 6 map as one dense GEMM (RTMPoseNet._final_maps); TLK_POSE_FINAL_GEMM=0 = the convolution
 USE_FINAL_GEMM = _os.environ.get("TLK_POSE_FINAL_GEMM", "1") != "0"
+# the gated attention unit on libtlk's operators (tlk_gau_attention_fwd, tlk_norm_gate_residual_fwd) instead of ~15 eager launches; off by default: the
+# weights stay unrounded in between, so float16 results differ from the eager composition in the last places.  A unit with a position bias always takes it.
+USE_TLK_GAU = _os.environ.get("TLK_GAU", "0") != "0"
 # CSPLayer: the two halves of the concatenation written in place by the convolutions that produce them (libtlk routes); 0 = torch.cat
 USE_SLICE_CONCAT = _os.environ.get("TLK_SLICE_CONCAT", "1") != "0"
 
@@ -133,9 +136,10 @@ class ScaleNorm(nn.Module):
 
 
 class GAU(nn.Module):
-    """RTMCCBlock (self-attention variant): gated attention unit with relu^2 kernel."""
+    """RTMCCBlock (self-attention variant): gated attention unit with relu^2 kernel.  rel_buckets > 0: with a position bias learned per bucket of the
+    distance between two tokens (``attention.relative_buckets``: logarithmic up to max_distance; trainable through the operators' gradients)."""
 
-    def __init__(self, dim=256, s=128, expansion=2):
+    def __init__(self, dim=256, s=128, expansion=2, rel_buckets=0, max_distance=16):
         super().__init__()
         self.e, self.s = dim * expansion, s
         self.ln = ScaleNorm(dim)
@@ -145,18 +149,39 @@ class GAU(nn.Module):
         self.o = nn.Linear(self.e, dim, bias=False)
         self.res_scale = nn.Parameter(torch.ones(dim))
         self.sqrt_s = math.sqrt(s)
+        self.max_distance = max_distance
+        if rel_buckets:
+            from ..attention import relative_buckets
+            self.rel_bias = nn.Parameter(torch.zeros(rel_buckets, 1))
+            self.register_buffer("buckets", relative_buckets(rel_buckets, max_distance, device="cpu"), persistent=False)
+        else:
+            self.rel_bias = self.buckets = None
 
     def forward(self, x):
-        h = F.silu(self.uv(self.ln(x)))
+        own = x.is_cuda and (USE_TLK_GAU or self.rel_bias is not None)
+        if own:
+            from .. import attention
+            n = attention.norm_gate_residual(x, norm="scale", weight=self.ln.g, eps=self.ln.eps)
+        else:
+            n = self.ln(x)
+        h = F.silu(self.uv(n))
         u, v, base = torch.split(h, [self.e, self.e, self.s], dim=-1)
         base = base.unsqueeze(2) * self.gamma[None, None] + self.beta
         q, k = base[:, :, 0], base[:, :, 1]
-        kernel = torch.square(F.relu(torch.bmm(q, k.transpose(1, 2)) / self.sqrt_s))
+        if own:
+            o = attention.gated_attention(q, k, v, u, kind="relu2", scale=1.0 / self.sqrt_s, bias=self.rel_bias, buckets=self.buckets)
+            return attention.norm_gate_residual(self.o(o), x, res_scale=self.res_scale)
+        score = torch.bmm(q, k.transpose(1, 2)) / self.sqrt_s
+        if self.rel_bias is not None:
+            t = torch.arange(x.shape[1], device=x.device)
+            away = (t[None, :] - t[:, None]).clamp(-self.max_distance, self.max_distance) + self.max_distance
+            score = score + self.rel_bias[self.buckets[away].long(), 0]
+        kernel = torch.square(F.relu(score))
         return x * self.res_scale + self.o(u * torch.bmm(kernel, v))
 
 
 class RTMPoseNet(nn.Module):
-    def __init__(self, widen=0.75, deepen=0.67, keypoints=17, input_hw=(256, 192), simcc_split=2.0):
+    def __init__(self, widen=0.75, deepen=0.67, keypoints=17, input_hw=(256, 192), simcc_split=2.0, rel_buckets=0):
         super().__init__()
         c = [int(v * widen) for v in (64, 128, 256, 512, 1024)]
         n = [max(round(v * deepen), 1) for v in (3, 6, 6, 3)]
@@ -174,7 +199,7 @@ class RTMPoseNet(nn.Module):
         fh, fw = input_hw[0] // 32, input_hw[1] // 32
         self.final_layer = nn.Conv2d(c[4], keypoints, 7, 1, 3)
         self.mlp = nn.Sequential(ScaleNorm(fh * fw), nn.Linear(fh * fw, 256, bias=False))
-        self.gau = GAU(256, 128, 2)
+        self.gau = GAU(256, 128, 2, rel_buckets)
         self.cls_x = nn.Linear(256, int(input_hw[1] * simcc_split), bias=False)
         self.cls_y = nn.Linear(256, int(input_hw[0] * simcc_split), bias=False)
 
@@ -209,9 +234,10 @@ class RTMPoseNet(nn.Module):
         return self.cls_x(t).float().contiguous(), self.cls_y(t).float().contiguous()
 
 
-def rtmpose(size="m", device="cuda", dtype=torch.float16, channels_last=True, seed=0):
+def rtmpose(size="m", device="cuda", dtype=torch.float16, channels_last=True, seed=0, rel_buckets=0):
+    """rel_buckets > 0: the head's attention unit learns a position bias over the keypoint tokens (GAU)"""
     widen, deepen = {"t": (0.375, 0.167), "s": (0.5, 0.33), "m": (0.75, 0.67), "l": (1.0, 1.0)}[size]
-    net = random_init_(RTMPoseNet(widen, deepen), seed)
+    net = random_init_(RTMPoseNet(widen, deepen, rel_buckets=rel_buckets), seed)
     with torch.no_grad():                      # random_init_ zeroes every 1-D parameter (biases); the norm gains are 1-D too
         for m in net.modules():
             if isinstance(m, ScaleNorm):

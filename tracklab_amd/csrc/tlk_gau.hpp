@@ -1,0 +1,890 @@
+// tlk_gau.hpp -- device side of the gated attention unit's core (tlk_gau_attention_fwd / _bwd), one template for float16, bfloat16 and float32.
+//
+//   S_ij = scale * q_i . k_j + bias[clip(j - (i + start), -D, D)]      (bias: the learned table, expanded over distances)
+//   W    = relu(S)^2  or  softmax_j(S);   O = W v;   out = gate * O
+//
+// Tiles are 16 x 16 MFMA tiles with 32 products each (16-bit: one v_mfma_f32_16x16x32; float32: eight v_mfma_f32_16x16x4 over the same eight values
+// a lane holds).  Every product is formed TRANSPOSED so that the row statistics live in one lane: S^T = K Q^T puts a query in a lane's column, four
+// consecutive keys in its registers, and those registers -- converted -- are already the B operand of O^T = V^T W^T: which 32 keys a lane's eight
+// operand slots name is free as long as both operands agree, so the weights never pass through shared memory.  V^T comes from the row-major V tile
+// by the transposing LDS read (ds_read_b64_tr_b16).  The backward kernels use the same scheme: dQ with a query, dK / dV with a key in the column.
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include "tlk_common.hpp"
+
+namespace tlk {
+namespace gau {
+
+enum { RELU2 = 0, SOFTMAX = 1 };
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f8 __attribute__((ext_vector_type(8)));
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float NEG = -3.0e38f;                 // running maximum before the first key: finite, below every score
+
+struct Args {
+    const void *q, *k, *v, *gate;
+    const void *table;                          // (num_buckets, heads)
+    const int *bucket_of, *lens, *q_start;
+    long long qs[3], ks[3], vs[3], gs[3];       // batch, row, head strides in elements
+    int B, Lq, Lk, H, Hk, dk, dv, nb, D, q0, causal, table_f32;
+    float scale;
+    // forward
+    void *out, *o;
+    float *lse;                                 // (B, Lq, H): log2 of the row's sum of 2^(S log2 e), +inf for a row without keys
+    float *part, *ml;                           // split keys: (split, B, Lq, H, dv) sums and (split, B, Lq, H, 2) maximum and sum
+    int nsplit, split_keys, nchunk, nrow, fold;
+    // backward
+    const void *dO;                             // (B, Lq, H, dv) contiguous: the gradient behind the gate
+    const float *delta;                         // (B, Lq, H): sum_d dO o (softmax)
+    void *dq, *dk_, *dv_;
+    float *dq_part, *dk_part;                   // (chunk, B, L, heads, dk) when dv is walked in several chunks
+    float *db_part;                             // (heads, B * chunk * nrow * waves, 2 D + 1)
+};
+
+template <class T> struct Ty;
+template <> struct Ty<_Float16> {
+    using V4 = h4;
+    using V8 = h8;
+    static constexpr bool scaled = true;        // relu^2 weights and score gradients pass float16's range: held with a running power of two
+    static __device__ __forceinline__ f4 mma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Ty<__bf16> {
+    using V4 = b4;
+    using V8 = b8;
+    static constexpr bool scaled = false;
+    static __device__ __forceinline__ f4 mma(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Ty<float> {
+    using V4 = f4;
+    using V8 = f8;
+    static constexpr bool scaled = false;
+    static __device__ __forceinline__ f4 mma(f8 a, f8 b, f4 c)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+template <class T> __device__ __forceinline__ typename Ty<T>::V8 zero8()
+{
+    typename Ty<T>::V8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (T)0.f;
+    return r;
+}
+
+// eight consecutive values of a row
+template <class T> __device__ __forceinline__ typename Ty<T>::V8 ld8(const T *p) { return *reinterpret_cast<const typename Ty<T>::V8 *>(p); }
+
+// values (row0 + 4 g + 0..3, col0 + l) of a row-major LDS tile, g = lane / 16, l = lane % 16: four rows of one column
+template <class T> __device__ __forceinline__ typename Ty<T>::V4 ld_col4(const T *tile, int ld, int g, int l)
+{
+    if constexpr (sizeof(T) == 2) {
+        const T *p = tile + (g * 4 + (l >> 2)) * ld + (l & 3) * 4;
+        s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(p));
+        return __builtin_bit_cast(typename Ty<T>::V4, r);
+    } else {
+        typename Ty<T>::V4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = tile[(g * 4 + i) * ld + l];
+        return r;
+    }
+}
+template <class T> __device__ __forceinline__ typename Ty<T>::V8 ld_col8(const T *tile, int ld, int g, int l)      // rows 4 g + 0..3 and 16 + 4 g + 0..3
+{
+    return __builtin_shufflevector(ld_col4(tile, ld, g, l), ld_col4(tile + 16 * ld, ld, g, l), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <class T> __device__ __forceinline__ typename Ty<T>::V8 pack8(f4 a, f4 b)
+{
+    typename Ty<T>::V8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[i] = (T)a[i];
+        r[4 + i] = (T)b[i];
+    }
+    return r;
+}
+
+// a (ROWS x COLS) tile on its way from HBM to LDS through registers: 16 bytes a lane; rows from `rend` and columns from `cend` read as zero
+template <class T, int ROWS, int COLS, int NTH> struct Stage {
+    static constexpr int VN = 16 / sizeof(T), CV = COLS / VN, TOT = ROWS * CV, N = (TOT + NTH - 1) / NTH;
+    u4 r[N];
+    __device__ __forceinline__ void load(const T *base, long long rs, int row0, int rend, int cend)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int idx = i * NTH + (int)threadIdx.x, row = idx / CV, c = (idx - row * CV) * VN;
+            r[i] = u4{0, 0, 0, 0};
+            if (idx < TOT && row0 + row < rend && c < cend) r[i] = *reinterpret_cast<const u4 *>(base + (long long)(row0 + row) * rs + c);
+        }
+    }
+    __device__ __forceinline__ void store(T *lds, int ld) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int idx = i * NTH + (int)threadIdx.x, row = idx / CV, c = (idx - row * CV) * VN;
+            if (idx < TOT) *reinterpret_cast<u4 *>(lds + row * ld + c) = r[i];
+        }
+    }
+};
+
+// the learned table over distances -D .. D of head h, into LDS; softmax works in powers of two, so its bias carries log2 e (finite values stay finite)
+template <class T, int KIND> __device__ __forceinline__ void expand_bias(const Args &p, int h, float *dst, int nth)
+{
+    for (int t = threadIdx.x; t < 2 * p.D + 1; t += nth) {
+        int b = p.bucket_of[t];
+        b = b < 0 ? 0 : (b >= p.nb ? p.nb - 1 : b);
+        const long long at = (long long)b * p.H + h;
+        float x = p.table_f32 ? reinterpret_cast<const float *>(p.table)[at] : (float)reinterpret_cast<const T *>(p.table)[at];
+        if (KIND == SOFTMAX) {
+            const float y = x * LOG2E;
+            x = (__builtin_isinf(y) && !__builtin_isinf(x)) ? (x < 0.f ? -1.0e38f : 1.0e38f) : y;
+        }
+        dst[t] = x;
+    }
+}
+
+__device__ __forceinline__ int key_end(const Args &p, int b) { const int n = p.lens ? p.lens[b] : p.Lk; return n < 0 ? 0 : (n > p.Lk ? p.Lk : n); }
+__device__ __forceinline__ int row_start(const Args &p, int b)
+{
+    const int lim = 1 << 29, s = p.q_start ? p.q_start[b] : p.q0;
+    return s < -lim ? -lim : (s > lim ? lim : s);
+}
+
+__device__ __forceinline__ float over_groups_max(float x) { x = fmaxf(x, __shfl_xor(x, 16)); return fmaxf(x, __shfl_xor(x, 32)); }
+__device__ __forceinline__ float over_groups_sum(float x) { x += __shfl_xor(x, 16); return x + __shfl_xor(x, 32); }
+__device__ __forceinline__ int wave_min_i(int x)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o));
+    return x;
+}
+__device__ __forceinline__ int wave_max_i(int x)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o));
+    return x;
+}
+__device__ __forceinline__ float relu_(float x) { return x < 0.f ? 0.f : x; }          // (NaN stays NaN)
+
+// running power of two of a column's float16 operands: values times 2^-e stay below 2^7; `t` = largest magnitude of this tile's column.
+// Returns the factor for what has been summed so far (1 where nothing changes).
+__device__ __forceinline__ float raise_exponent(int &e, float t)
+{
+    if (!(ldexpf(t, -e) > 128.f)) return 1.f;
+    int n;
+    (void)frexpf(t, &n);                          // t in [2^(n-1), 2^n)
+    if (!(t < 1.3e36f)) n = 120;
+    const float f = ldexpf(1.f, e - n < -150 ? -150 : e - n);
+    e = n;
+    return f;
+}
+constexpr int E_NONE = -120;                      // exponent before the first non-zero value
+
+// bias of key j at query position pos: LDS gather near the diagonal, the two end values beyond it
+__device__ __forceinline__ float bias_at(const float *tab, int D, int j, int pos)
+{
+    int d = j - pos;
+    d = d < -D ? -D : (d > D ? D : d);
+    return tab[d + D];
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------ forward
+// WM x WN waves; a wave owns MT x 16 rows and NT x 16 columns of the output.  Rows of a block are (head of the group, query) pairs when p.fold
+// (few queries: the heads that share keys and values are answered in one pass over them).
+template <class T, int KIND, int DK, int MT, int NT, int WM, int WN, int KT>
+__global__ void __launch_bounds__(64 * WM * WN) fwd_kernel(const Args p)
+{
+    using V8 = typename Ty<T>::V8;
+    constexpr int NTH = 64 * WM * WN, BM = WM * MT * 16, DVB = WN * NT * 16, PAD = 16 / sizeof(T), LDK = DK + PAD, LDV = DVB + 2 * PAD, NS = KT / 16;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T *Ks = reinterpret_cast<T *>(smem), *Vs = Ks + KT * LDK;
+    float *tab = reinterpret_cast<float *>(Vs + KT * LDV);
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / WN, wn = w - wm * WN, g = lane >> 4, l = lane & 15;
+    const int G = p.H / p.Hk, GB = p.fold ? G : 1, HB = p.H / GB, rows = p.Lq * GB, TW = 2 * p.D + 1;
+    int id = blockIdx.x;
+    const int rt = id % p.nrow; id /= p.nrow;
+    const int ch = id % p.nchunk; id /= p.nchunk;
+    const int sp = id % p.nsplit; id /= p.nsplit;
+    const int hb = id % HB, b = id / HB;
+    const int hk = p.fold ? hb : hb / G, h0 = p.fold ? hb * G : hb;
+    const int kend_all = key_end(p, b), q0 = row_start(p, b);
+    const int c0 = ch * DVB, cend = p.dv - c0;
+    if (p.table)
+        for (int i = 0; i < GB; ++i) expand_bias<T, KIND>(p, h0 + i, tab + i * TW, NTH);
+
+    const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0];
+    const T *K = reinterpret_cast<const T *>(p.k) + b * p.ks[0] + hk * p.ks[2];
+    const T *V = reinterpret_cast<const T *>(p.v) + b * p.vs[0] + hk * p.vs[2] + c0;
+    int qi[MT], qh[MT], pos[MT];
+    bool ok[MT];
+    V8 qf[MT][DK / 32];
+    int pmin = 0x7fffffff, pmax = -0x7fffffff;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int r = rt * BM + (wm * MT + mt) * 16 + l;
+        ok[mt] = r < rows;
+        const int rr = ok[mt] ? r : 0, hi = rr / p.Lq;
+        qi[mt] = rr - hi * p.Lq;
+        qh[mt] = hi;
+        pos[mt] = qi[mt] + q0;
+        if (ok[mt]) { pmin = min(pmin, pos[mt]); pmax = max(pmax, pos[mt]); }
+        const T *src = Q + (long long)qi[mt] * p.qs[1] + (h0 + hi) * p.qs[2] + g * 8;
+#pragma unroll
+        for (int ks = 0; ks < DK / 32; ++ks) qf[mt][ks] = (ok[mt] && ks * 32 + g * 8 < p.dk) ? ld8(src + ks * 32) : zero8<T>();
+    }
+    pmin = __builtin_amdgcn_readfirstlane(wave_min_i(pmin));
+    pmax = __builtin_amdgcn_readfirstlane(wave_max_i(pmax));
+    // keys of this block: its split, below the length, and not beyond its last row's position
+    int kb = sp * p.split_keys, ke = min(kend_all, p.nsplit > 1 ? kb + p.split_keys : kend_all);
+    if (p.causal) {
+        const int r0 = rt * BM, r1 = min(rows, r0 + BM) - 1;
+        const int last = (r0 / p.Lq == r1 / p.Lq) ? r1 % p.Lq : p.Lq - 1;
+        ke = min(ke, last + q0 + 1);
+    }
+    f4 acc[NT][MT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[n][mt] = f4{0, 0, 0, 0};
+    float m[MT], lsum[MT];
+    int ex[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) { m[mt] = NEG; lsum[mt] = 0.f; ex[mt] = E_NONE; }
+    const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
+
+    Stage<T, KT, DK, NTH> stk;
+    Stage<T, KT, DVB, NTH> stv;
+    if (kb < ke) { stk.load(K, p.ks[1], kb, ke, p.dk); stv.load(V, p.vs[1], kb, ke, cend); }
+    for (int j0 = kb; j0 < ke; j0 += KT) {
+        __syncthreads();
+        stk.store(Ks, LDK);
+        stv.store(Vs, LDV);
+        __syncthreads();
+        if (j0 + KT < ke) { stk.load(K, p.ks[1], j0 + KT, ke, p.dk); stv.load(V, p.vs[1], j0 + KT, ke, cend); }
+        if (pmin > pmax || (p.causal && j0 > pmax)) continue;      // no row of this wave, or none that sees this tile (uniform over the wave)
+        f4 s[MT][NS];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) s[mt][n] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < DK / 32; ++ks) {
+                const V8 a = ld8(Ks + (n * 16 + l) * LDK + ks * 32 + g * 8);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, qf[mt][ks], s[mt][n]);
+            }
+        }
+        // scores: scale, bias, mask
+        const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin);
+        const int where = !p.table ? 0 : (j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const float *tb = tab + qh[mt] * TW;
+            const float far = where == 1 ? tb[TW - 1] : (where == 2 ? tb[0] : 0.f);
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int j = j0 + n * 16 + g * 4 + r;
+                    float x = s[mt][n][r] * sc + (where == 3 ? bias_at(tb, p.D, j, pos[mt]) : far);
+                    if (!full && (j >= ke || (p.causal && j > pos[mt]))) x = KIND == SOFTMAX ? -INFINITY : 0.f;
+                    s[mt][n][r] = KIND == SOFTMAX ? x : relu_(x);
+                }
+        }
+        // weights
+        float fac[MT];
+        bool any = false;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            fac[mt] = 1.f;
+            if (KIND == SOFTMAX || Ty<T>::scaled) {
+                float t = s[mt][0][0];
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) t = fmaxf(t, s[mt][n][r]);
+                t = over_groups_max(t);
+                if (KIND == SOFTMAX) {
+                    const float mn = fmaxf(m[mt], t);
+                    fac[mt] = exp2f(m[mt] - mn);
+                    m[mt] = mn;
+                    lsum[mt] *= fac[mt];
+                } else {
+                    const float f = raise_exponent(ex[mt], t);
+                    fac[mt] = f * f;
+                }
+                any |= fac[mt] != 1.f;
+            }
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = s[mt][n][r];
+                    if (KIND == SOFTMAX) {
+                        x = exp2f(x - m[mt]);
+                        lsum[mt] += x;
+                    } else {
+                        if (Ty<T>::scaled) x = ldexpf(x, -ex[mt]);
+                        x = x * x;
+                    }
+                    s[mt][n][r] = x;
+                }
+        }
+        if ((KIND == SOFTMAX || Ty<T>::scaled) && __any(any)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) acc[n][mt] *= fac[mt];
+        }
+#pragma unroll
+        for (int kk = 0; kk < NS / 2; ++kk) {
+            V8 pb[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) pb[mt] = pack8<T>(s[mt][2 * kk], s[mt][2 * kk + 1]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const V8 a = ld_col8<T>(Vs + kk * 32 * LDV + (wn * NT + n) * 16, LDV, g, l);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) acc[n][mt] = Ty<T>::mma(a, pb[mt], acc[n][mt]);
+            }
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        if (KIND == SOFTMAX) lsum[mt] = over_groups_sum(lsum[mt]);
+        if (!ok[mt]) continue;
+        const long long row = ((long long)b * p.Lq + qi[mt]) * p.H + h0 + qh[mt];
+        float fin = 1.f;
+        if (KIND == SOFTMAX) fin = p.nsplit > 1 ? 1.f : (lsum[mt] == 0.f ? 0.f : 1.f / lsum[mt]);
+        else if (Ty<T>::scaled) fin = ex[mt] == E_NONE ? 0.f : ldexpf(1.f, ex[mt]);      // applied twice: the square may pass float32 where the product does not
+        constexpr bool TWICE = KIND == RELU2 && Ty<T>::scaled;
+        const int cw = c0 + wn * NT * 16;
+        if (p.nsplit > 1) {
+            const long long at = (long long)sp * p.B * p.Lq * p.H + row;
+            if (KIND == SOFTMAX && c0 == 0 && wn == 0 && g == 0) { p.ml[2 * at] = m[mt]; p.ml[2 * at + 1] = lsum[mt]; }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int c = cw + n * 16 + g * 4;
+                f4 x = acc[n][mt] * fin;
+                if (TWICE) x *= fin;
+                if (c < p.dv) *reinterpret_cast<f4 *>(p.part + at * p.dv + c) = x;
+            }
+            continue;
+        }
+        if (p.lse && c0 == 0 && wn == 0 && g == 0) p.lse[row] = lsum[mt] == 0.f ? INFINITY : m[mt] + log2f(lsum[mt]);
+        const T *gp = p.gate ? reinterpret_cast<const T *>(p.gate) + b * p.gs[0] + (long long)qi[mt] * p.gs[1] + (h0 + qh[mt]) * p.gs[2] : nullptr;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int c = cw + n * 16 + g * 4;
+            if (c >= p.dv) continue;
+            f4 x = acc[n][mt] * fin;
+            if (TWICE) x *= fin;
+            typename Ty<T>::V4 y;
+            if (p.o) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
+                *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.o) + row * p.dv + c) = y;
+            }
+            if (gp) {
+                const typename Ty<T>::V4 u = *reinterpret_cast<const typename Ty<T>::V4 *>(gp + c);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] *= (float)u[r];
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
+            *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.out) + row * p.dv + c) = y;
+        }
+    }
+}
+
+// joins the key splits of few-row calls: one lane per four output values
+template <class T, int KIND> __global__ void __launch_bounds__(256) join_kernel(const Args p)
+{
+    const int cv = p.dv / 4;
+    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x, nrow = (long long)p.B * p.Lq * p.H;
+    if (idx >= nrow * cv) return;
+    const long long row = idx / cv;
+    const int c = (int)(idx - row * cv) * 4;
+    f4 x = {0, 0, 0, 0};
+    if (KIND == SOFTMAX) {
+        float m = NEG, s = 0.f;
+        for (int i = 0; i < p.nsplit; ++i) m = fmaxf(m, p.ml[2 * (i * nrow + row)]);
+        for (int i = 0; i < p.nsplit; ++i) {
+            const float f = exp2f(p.ml[2 * (i * nrow + row)] - m);
+            s += f * p.ml[2 * (i * nrow + row) + 1];
+            x += *reinterpret_cast<const f4 *>(p.part + (i * nrow + row) * p.dv + c) * f;
+        }
+        x *= s == 0.f ? 0.f : 1.f / s;
+        if (p.lse && c == 0) p.lse[row] = s == 0.f ? INFINITY : m + log2f(s);
+    } else {
+        for (int i = 0; i < p.nsplit; ++i) x += *reinterpret_cast<const f4 *>(p.part + (i * nrow + row) * p.dv + c);
+    }
+    const int h = (int)(row % p.H);
+    const long long bi = row / p.H;
+    typename Ty<T>::V4 y;
+    if (p.o) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
+        *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.o) + row * p.dv + c) = y;
+    }
+    if (p.gate) {
+        const typename Ty<T>::V4 u = *reinterpret_cast<const typename Ty<T>::V4 *>(reinterpret_cast<const T *>(p.gate) + (bi / p.Lq) * p.gs[0] + (bi % p.Lq) * p.gs[1] + h * p.gs[2] + c);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] *= (float)u[r];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
+    *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.out) + row * p.dv + c) = y;
+}
+
+// ----------------------------------------------------------------------------------------------------------------------------------- backward
+// behind the gate: dO = dout * gate, dgate = dout * O, delta = sum_d dO * O.  One wave per row.
+template <class T> struct GateArgs {
+    const T *dout, *gate, *o;
+    long long gs[3];
+    T *dO, *dgate;
+    float *delta;
+    long long rows;
+    int Lq, H, dv;
+};
+template <class T> __global__ void __launch_bounds__(256) gate_bwd_kernel(const GateArgs<T> p)
+{
+    using V4 = typename Ty<T>::V4;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= p.rows) return;
+    const long long bi = row / p.H;
+    const T *gp = p.gate ? p.gate + (bi / p.Lq) * p.gs[0] + (bi % p.Lq) * p.gs[1] + (row % p.H) * p.gs[2] : nullptr;
+    float d = 0.f;
+    for (int c = lane * 4; c < p.dv; c += 256) {
+        const V4 du = *reinterpret_cast<const V4 *>(p.dout + row * p.dv + c), o = *reinterpret_cast<const V4 *>(p.o + row * p.dv + c);
+        V4 a, b;
+        if (gp) {
+            const V4 u = *reinterpret_cast<const V4 *>(gp + c);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                a[r] = (T)((float)du[r] * (float)u[r]);
+                b[r] = (T)((float)du[r] * (float)o[r]);
+                d += (float)a[r] * (float)o[r];
+            }
+            *reinterpret_cast<V4 *>(p.dO + row * p.dv + c) = a;
+            *reinterpret_cast<V4 *>(p.dgate + row * p.dv + c) = b;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d += (float)du[r] * (float)o[r];
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o);
+    if (p.delta && lane == 0) p.delta[row] = d;
+}
+
+// dS of one pair from its score x (scaled, biased; softmax: in powers of two), dW and the row's statistics; w returns the weight
+template <int KIND> __device__ __forceinline__ float dscore(float x, float dw, float lse, float delta, bool seen, float &w)
+{
+    if (KIND == SOFTMAX) {
+        w = seen ? exp2f(x - lse) : 0.f;
+        return seen ? w * (dw - delta) : 0.f;
+    }
+    const float s = seen ? relu_(x) : 0.f;
+    w = s * s;
+    return seen ? 2.f * s * dw : 0.f;
+}
+
+// a wave's column tile as float16 operands: divides by the running power of two (see raise_exponent), returns what rescales the sums so far
+template <class T, int NS> __device__ __forceinline__ float hold(f4 (&x)[NS], int &e)
+{
+    if constexpr (!Ty<T>::scaled) return 1.f;
+    float t = 0.f;
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t = fmaxf(t, fabsf(x[n][r]));
+    const float f = raise_exponent(e, over_groups_max(t));
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[n][r] = ldexpf(x[n][r], -e);
+    return f;
+}
+template <class T> __device__ __forceinline__ float unhold(int e) { return !Ty<T>::scaled ? 1.f : (e == E_NONE ? 0.f : ldexpf(1.f, e)); }
+
+// dQ and the bias gradient: W waves, MT x 16 queries each; walks the keys.  dS^T has a query in the column: its registers are the B operand of
+// dQ^T = K^T dS^T.  The bias gradient needs sums along diagonals: a tile that lies beyond +-D of all its queries is one sum in registers, one near
+// the diagonal goes through a wave's own (KT x BM) LDS tile and each lane sums one diagonal -- no atomics, the order is fixed.
+template <class T, int KIND, int DK, int DVC, int MT, int W>
+__global__ void __launch_bounds__(64 * W) dq_kernel(const Args p)
+{
+    using V8 = typename Ty<T>::V8;
+    constexpr int KT = 32, NTH = 64 * W, BM = W * MT * 16, PAD = 16 / sizeof(T), LDK = DK + PAD, LDV = DVC + PAD, NS = 2, LT = MT * 16 + 1;
+    static_assert(KT + MT * 16 <= 64, "one diagonal of a wave's tile per lane");
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T *Ks = reinterpret_cast<T *>(smem), *Vs = Ks + KT * LDK;
+    const int TW = p.table ? 2 * p.D + 1 : 0;
+    float *tab = reinterpret_cast<float *>(Vs + KT * LDV);
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
+    float *dbw = tab + TW + w * TW, *tile = tab + TW + W * TW + w * KT * LT;         // this wave's distance sums and its dS tile
+    int id = blockIdx.x;
+    const int rt = id % p.nrow; id /= p.nrow;
+    const int ch = id % p.nchunk; id /= p.nchunk;
+    const int h = id % p.H, b = id / p.H, hk = h / (p.H / p.Hk);
+    const int q0 = row_start(p, b), c0 = ch * DVC, cend = p.dv - c0;
+    if (p.table) {
+        expand_bias<T, KIND>(p, h, tab, NTH);
+        for (int t = lane; t < TW; t += 64) dbw[t] = 0.f;
+    }
+    const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2];
+    const T *K = reinterpret_cast<const T *>(p.k) + b * p.ks[0] + hk * p.ks[2];
+    const T *V = reinterpret_cast<const T *>(p.v) + b * p.vs[0] + hk * p.vs[2] + c0;
+    const int i0 = rt * BM + w * MT * 16;                                             // the wave's first query
+    V8 qf[MT][DK / 32], df[MT][DVC / 32];
+    float lse[MT], del[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int i = i0 + mt * 16 + l;
+        const bool ok = i < p.Lq;
+        const long long row = ((long long)b * p.Lq + (ok ? i : 0)) * p.H + h;
+        const T *src = Q + (long long)(ok ? i : 0) * p.qs[1] + g * 8;
+#pragma unroll
+        for (int ks = 0; ks < DK / 32; ++ks) qf[mt][ks] = (ok && ks * 32 + g * 8 < p.dk) ? ld8(src + ks * 32) : zero8<T>();
+        const T *dsrc = reinterpret_cast<const T *>(p.dO) + row * p.dv + c0 + g * 8;
+#pragma unroll
+        for (int ks = 0; ks < DVC / 32; ++ks) df[mt][ks] = (ok && ks * 32 + g * 8 < cend) ? ld8(dsrc + ks * 32) : zero8<T>();
+        lse[mt] = KIND == SOFTMAX ? (ok ? p.lse[row] : INFINITY) : 0.f;
+        del[mt] = KIND == SOFTMAX && ok && ch == 0 ? p.delta[row] : 0.f;              // (dW comes in chunks of dv: the subtraction belongs to one of them)
+    }
+    int ke = key_end(p, b);
+    if (p.causal) ke = min(ke, min(p.Lq, rt * BM + BM) - 1 + q0 + 1);
+    const int pmin = i0 + q0, pmax = min(p.Lq, i0 + MT * 16) - 1 + q0;
+    f4 acc[DK / 16][MT];
+#pragma unroll
+    for (int n = 0; n < DK / 16; ++n)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[n][mt] = f4{0, 0, 0, 0};
+    int ex[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) ex[mt] = E_NONE;
+    float lo = 0.f, hi = 0.f;
+    const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
+    Stage<T, KT, DK, NTH> stk;
+    Stage<T, KT, DVC, NTH> stv;
+    if (0 < ke) { stk.load(K, p.ks[1], 0, ke, p.dk); stv.load(V, p.vs[1], 0, ke, cend); }
+    for (int j0 = 0; j0 < ke; j0 += KT) {
+        __syncthreads();
+        stk.store(Ks, LDK);
+        stv.store(Vs, LDV);
+        __syncthreads();
+        if (j0 + KT < ke) { stk.load(K, p.ks[1], j0 + KT, ke, p.dk); stv.load(V, p.vs[1], j0 + KT, ke, cend); }
+        if (i0 >= p.Lq || (p.causal && j0 > pmax)) continue;
+        f4 s[MT][NS], dp[MT][NS];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) { s[mt][n] = f4{0, 0, 0, 0}; dp[mt][n] = f4{0, 0, 0, 0}; }
+#pragma unroll
+            for (int ks = 0; ks < DK / 32; ++ks) {
+                const V8 a = ld8(Ks + (n * 16 + l) * LDK + ks * 32 + g * 8);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, qf[mt][ks], s[mt][n]);
+            }
+#pragma unroll
+            for (int ks = 0; ks < DVC / 32; ++ks) {
+                const V8 a = ld8(Vs + (n * 16 + l) * LDV + ks * 32 + g * 8);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) dp[mt][n] = Ty<T>::mma(a, df[mt][ks], dp[mt][n]);
+            }
+        }
+        const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin) && i0 + MT * 16 <= p.Lq;
+        const int where = !p.table ? 0 : (j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3));
+        const float far = where == 1 ? tab[TW - 1] : (where == 2 ? tab[0] : 0.f);
+        float all = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const int i = i0 + mt * 16 + l, pos = i + q0;
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int j = j0 + n * 16 + g * 4 + r;
+                    const float x = s[mt][n][r] * sc + (where == 3 ? bias_at(tab, p.D, j, pos) : far);
+                    const bool seen = full || (i < p.Lq && j < ke && !(p.causal && j > pos));
+                    float wgt;
+                    const float d = dscore<KIND>(x, dp[mt][n][r], lse[mt], del[mt], seen, wgt);
+                    s[mt][n][r] = d;
+                    all += d;
+                    if (where == 3) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = d;
+                }
+        }
+        if (where == 1) hi += all;
+        if (where == 2) lo += all;
+        if (where == 3) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            const int e = lane - (MT * 16 - 1);                                       // key - query within the tile
+            float sum = 0.f;
+            for (int c = 0; c < MT * 16; ++c)
+                if (c + e >= 0 && c + e < KT) sum += tile[(c + e) * LT + c];
+            const int d = e + j0 - i0 - q0;
+            if (lane < KT + MT * 16 - 1) {
+                if (d >= p.D) hi += sum;
+                else if (d <= -p.D) lo += sum;
+                else dbw[d + p.D] += sum;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const float f = hold<T, NS>(s[mt], ex[mt]);
+            if (Ty<T>::scaled && __any(f != 1.f))
+#pragma unroll
+                for (int n = 0; n < DK / 16; ++n) acc[n][mt] *= f;
+        }
+        V8 pb[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) pb[mt] = pack8<T>(s[mt][0], s[mt][1]);
+#pragma unroll
+        for (int n = 0; n < DK / 16; ++n) {
+            const V8 a = ld_col8<T>(Ks + n * 16, LDK, g, l);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) acc[n][mt] = Ty<T>::mma(a, pb[mt], acc[n][mt]);
+        }
+    }
+    if (p.table) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) { lo += __shfl_xor(lo, o); hi += __shfl_xor(hi, o); }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const long long nr = (long long)p.B * p.nchunk * p.nrow * W, at = (((long long)b * p.nchunk + ch) * p.nrow + rt) * W + w;
+        float *dst = p.db_part + ((long long)h * nr + at) * TW;
+        for (int t = lane; t < TW; t += 64) dst[t] = t == 0 ? lo + (p.D == 0 ? hi : 0.f) : (t == TW - 1 ? hi : dbw[t]);
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int i = i0 + mt * 16 + l;
+        if (i >= p.Lq) continue;
+        const long long row = ((long long)b * p.Lq + i) * p.H + h;
+        const float fin = p.scale * unhold<T>(ex[mt]);
+#pragma unroll
+        for (int n = 0; n < DK / 16; ++n) {
+            const int c = n * 16 + g * 4;
+            if (c >= p.dk) continue;
+            const f4 x = acc[n][mt] * fin;
+            if (p.nchunk > 1) {
+                *reinterpret_cast<f4 *>(p.dq_part + ((long long)ch * p.B * p.Lq * p.H + row) * p.dk + c) = x;
+            } else {
+                typename Ty<T>::V4 y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
+                *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.dq) + row * p.dk + c) = y;
+            }
+        }
+    }
+}
+
+// dK and dV: W waves, MT x 16 keys each; walks the queries of every head that shares the keys.  S has a key in the column: W and dS in registers
+// are the B operands of dV^T = dO^T W and dK^T = Q^T dS.
+template <class T, int KIND, int DK, int DVC, int MT, int W>
+__global__ void __launch_bounds__(64 * W) dkv_kernel(const Args p)
+{
+    using V8 = typename Ty<T>::V8;
+    constexpr int QT = 32, NTH = 64 * W, BN = W * MT * 16, PAD = 16 / sizeof(T), LDQ = DK + PAD, LDO = DVC + PAD, NS = 2;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T *Qs = reinterpret_cast<T *>(smem), *Os = Qs + QT * LDQ;
+    float *st = reinterpret_cast<float *>(Os + QT * LDO), *tab = st + 2 * QT;           // the tile's log-sum-exp and delta
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15, G = p.H / p.Hk, TW = 2 * p.D + 1;
+    int id = blockIdx.x;
+    const int rt = id % p.nrow; id /= p.nrow;
+    const int ch = id % p.nchunk; id /= p.nchunk;
+    const int hk = id % p.Hk, b = id / p.Hk;
+    const int q0 = row_start(p, b), ke = key_end(p, b), c0 = ch * DVC, cend = p.dv - c0;
+    const int j0 = rt * BN + w * MT * 16;                                               // the wave's first key
+    V8 kf[MT][DK / 32], vf[MT][DVC / 32];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int j = j0 + mt * 16 + l;
+        const bool ok = j < ke;
+        const T *kp = reinterpret_cast<const T *>(p.k) + b * p.ks[0] + (long long)(ok ? j : 0) * p.ks[1] + hk * p.ks[2] + g * 8;
+        const T *vp = reinterpret_cast<const T *>(p.v) + b * p.vs[0] + (long long)(ok ? j : 0) * p.vs[1] + hk * p.vs[2] + c0 + g * 8;
+#pragma unroll
+        for (int ks = 0; ks < DK / 32; ++ks) kf[mt][ks] = (ok && ks * 32 + g * 8 < p.dk) ? ld8(kp + ks * 32) : zero8<T>();
+#pragma unroll
+        for (int ks = 0; ks < DVC / 32; ++ks) vf[mt][ks] = (ok && ks * 32 + g * 8 < cend) ? ld8(vp + ks * 32) : zero8<T>();
+    }
+    f4 av[DVC / 16][MT], ak[DK / 16][MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int n = 0; n < DVC / 16; ++n) av[n][mt] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int n = 0; n < DK / 16; ++n) ak[n][mt] = f4{0, 0, 0, 0};
+    }
+    int ev[MT], ek[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) ev[mt] = ek[mt] = E_NONE;
+    const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
+    const int jmin = j0, jmax = min(ke, j0 + MT * 16) - 1;
+    // queries from the first that sees a key of this block
+    int ib = 0;
+    if (p.causal) ib = max(0, (rt * BN - q0) / QT * QT);
+    if (rt * BN >= ke) ib = p.Lq;                                                       // keys behind the length only: zeros
+    Stage<T, QT, DK, NTH> stq;
+    Stage<T, QT, DVC, NTH> sto;
+    for (int hg = 0; hg < G; ++hg) {
+        const int h = hk * G + hg;
+        const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2];
+        const T *dO = reinterpret_cast<const T *>(p.dO) + ((long long)b * p.Lq * p.H + h) * p.dv + c0;
+        const long long os = (long long)p.H * p.dv;
+        __syncthreads();
+        if (p.table && ib < p.Lq) expand_bias<T, KIND>(p, h, tab, NTH);
+        if (ib < p.Lq) { stq.load(Q, p.qs[1], ib, p.Lq, p.dk); sto.load(dO, os, ib, p.Lq, cend); }
+        for (int i0 = ib; i0 < p.Lq; i0 += QT) {
+            __syncthreads();
+            stq.store(Qs, LDQ);
+            sto.store(Os, LDO);
+            if (KIND == SOFTMAX && tid < QT) {
+                const int i = i0 + tid;
+                const long long row = ((long long)b * p.Lq + i) * p.H + h;
+                st[tid] = i < p.Lq ? p.lse[row] : INFINITY;
+                st[QT + tid] = i < p.Lq && ch == 0 ? p.delta[row] : 0.f;
+            }
+            __syncthreads();
+            if (i0 + QT < p.Lq) { stq.load(Q, p.qs[1], i0 + QT, p.Lq, p.dk); sto.load(dO, os, i0 + QT, p.Lq, cend); }
+            const int pmin = i0 + q0, pmax = min(p.Lq, i0 + QT) - 1 + q0;
+            if (jmax < jmin || (p.causal && jmin > pmax)) continue;
+            f4 s[MT][NS], dp[MT][NS];
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) { s[mt][n] = f4{0, 0, 0, 0}; dp[mt][n] = f4{0, 0, 0, 0}; }
+#pragma unroll
+                for (int ks = 0; ks < DK / 32; ++ks) {
+                    const V8 a = ld8(Qs + (n * 16 + l) * LDQ + ks * 32 + g * 8);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, kf[mt][ks], s[mt][n]);
+                }
+#pragma unroll
+                for (int ks = 0; ks < DVC / 32; ++ks) {
+                    const V8 a = ld8(Os + (n * 16 + l) * LDO + ks * 32 + g * 8);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) dp[mt][n] = Ty<T>::mma(a, vf[mt][ks], dp[mt][n]);
+                }
+            }
+            const bool full = i0 + QT <= p.Lq && j0 + MT * 16 <= ke && (!p.causal || j0 + MT * 16 - 1 <= pmin);
+            const int where = !p.table ? 0 : (jmin - pmax >= p.D ? 1 : (jmax - pmin <= -p.D ? 2 : 3));
+            const float far = where == 1 ? tab[TW - 1] : (where == 2 ? tab[0] : 0.f);
+            V8 wb[MT], db[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const int j = j0 + mt * 16 + l;
+                f4 wt[NS];
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    f4 ls = {0, 0, 0, 0}, dl = {0, 0, 0, 0};
+                    if (KIND == SOFTMAX) {
+                        ls = *reinterpret_cast<const f4 *>(st + n * 16 + g * 4);
+                        dl = *reinterpret_cast<const f4 *>(st + QT + n * 16 + g * 4);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = i0 + n * 16 + g * 4 + r, pos = i + q0;
+                        const float x = s[mt][n][r] * sc + (where == 3 ? bias_at(tab, p.D, j, pos) : far);
+                        const bool seen = full || (i < p.Lq && j < ke && !(p.causal && j > pos));
+                        float wgt;
+                        s[mt][n][r] = dscore<KIND>(x, dp[mt][n][r], ls[r], dl[r], seen, wgt);
+                        wt[n][r] = wgt;
+                    }
+                }
+                const float fv = hold<T, NS>(wt, ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
+                if (Ty<T>::scaled && __any(fv != 1.f))
+#pragma unroll
+                    for (int n = 0; n < DVC / 16; ++n) av[n][mt] *= fv;
+                if (Ty<T>::scaled && __any(fk != 1.f))
+#pragma unroll
+                    for (int n = 0; n < DK / 16; ++n) ak[n][mt] *= fk;
+                wb[mt] = pack8<T>(wt[0], wt[1]);
+                db[mt] = pack8<T>(s[mt][0], s[mt][1]);
+            }
+#pragma unroll
+            for (int n = 0; n < DVC / 16; ++n) {
+                const V8 a = ld_col8<T>(Os + n * 16, LDO, g, l);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) av[n][mt] = Ty<T>::mma(a, wb[mt], av[n][mt]);
+            }
+#pragma unroll
+            for (int n = 0; n < DK / 16; ++n) {
+                const V8 a = ld_col8<T>(Qs + n * 16, LDQ, g, l);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) ak[n][mt] = Ty<T>::mma(a, db[mt], ak[n][mt]);
+            }
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int j = j0 + mt * 16 + l;
+        if (j >= p.Lk) continue;
+        const long long row = ((long long)b * p.Lk + j) * p.Hk + hk;
+        const float finv = unhold<T>(ev[mt]), fink = p.scale * unhold<T>(ek[mt]);
+        typename Ty<T>::V4 y;
+#pragma unroll
+        for (int n = 0; n < DVC / 16; ++n) {
+            const int c = n * 16 + g * 4;
+            if (c >= cend) continue;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = (T)(av[n][mt][r] * finv);
+            *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.dv_) + row * p.dv + c0 + c) = y;
+        }
+#pragma unroll
+        for (int n = 0; n < DK / 16; ++n) {
+            const int c = n * 16 + g * 4;
+            if (c >= p.dk) continue;
+            const f4 x = ak[n][mt] * fink;
+            if (p.nchunk > 1) {
+                *reinterpret_cast<f4 *>(p.dk_part + ((long long)ch * p.B * p.Lk * p.Hk + row) * p.dk + c) = x;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
+                *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.dk_) + row * p.dk + c) = y;
+            }
+        }
+    }
+}
+
+// y = sum over chunks of the float32 partial sums, rounded once
+template <class T> __global__ void __launch_bounds__(256) sum_chunks_kernel(const float *part, T *y, long long n, int chunks)
+{
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    f4 x = *reinterpret_cast<const f4 *>(part + i);
+    for (int c = 1; c < chunks; ++c) x += *reinterpret_cast<const f4 *>(part + c * n + i);
+    typename Ty<T>::V4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (T)x[r];
+    *reinterpret_cast<typename Ty<T>::V4 *>(y + i) = v;
+}
+
+// host side, one instantiation per element type (tlk_gau_f16.hip, tlk_gau_bf16.hip, tlk_gau_f32.hip)
+struct BwdIo {
+    const void *dout, *o;
+    void *dq, *dk, *dv, *dgate, *dtable;
+    void *ws;
+};
+template <class T> int forward(Args a, int kind, void *ws, hipStream_t st);
+template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t st);
+
+}  // namespace gau
+}  // namespace tlk

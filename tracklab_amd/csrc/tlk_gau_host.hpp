@@ -1,0 +1,234 @@
+// tlk_gau_host.hpp -- launches of the gated attention unit's kernels for one element type (included by tlk_gau_{f16,bf16,f32}.hip).
+#pragma once
+#include "tlk_gau.hpp"
+
+namespace tlk {
+namespace gau {
+
+inline long long align_up(long long x) { return (x + 255) & ~255LL; }
+inline int div_up(int a, int b) { return (a + b - 1) / b; }
+
+// how the forward call of these sizes is cut; shared by the launch and the workspace query
+struct FwdPlan {
+    bool few;                // one tile of rows, waves side by side along dv; else waves below each other
+    int fold, mt, dvb, bm, nrow, nchunk, nsplit, split_keys, heads;
+};
+inline FwdPlan plan_forward(const Args &a)
+{
+    FwdPlan f;
+    const int G = a.H / a.Hk;
+    f.fold = G > 1 && a.Lq <= 32 && (long long)G * (2 * a.D + 1) <= 8192;
+    const long long rows = (long long)a.Lq * (f.fold ? G : 1);
+    f.few = rows <= 32;
+    f.mt = f.few && rows <= 16 ? 1 : 2;
+    f.bm = f.few ? f.mt * 16 : 128;
+    f.dvb = a.dv <= 64 ? 64 : (a.dv <= 128 ? 128 : (a.dv <= 256 || !f.few ? 256 : 512));
+    f.nrow = (int)((rows + f.bm - 1) / f.bm);
+    f.nchunk = div_up(a.dv, f.dvb);
+    f.heads = f.fold ? a.Hk : a.H;
+    const long long blocks = (long long)a.B * f.heads * f.nchunk * f.nrow;
+    f.nsplit = 1;
+    f.split_keys = a.Lk;
+    if (f.few && a.Lk > 512 && blocks < 1024) {
+        const int want = (int)((1024 + blocks - 1) / blocks), most = div_up(a.Lk, 256);
+        f.nsplit = want < most ? want : most;
+        f.split_keys = div_up(div_up(a.Lk, f.nsplit), 64) * 64;
+        f.nsplit = div_up(a.Lk, f.split_keys);
+    }
+    return f;
+}
+
+struct BwdPlan {
+    int dvc, nchunk, w_q, w_k, rows_q, rows_k, nrow_q, nrow_k;
+    long long nr;            // distance-sum rows per head
+};
+inline BwdPlan plan_backward(const Args &a, int elem)
+{
+    BwdPlan f;
+    f.dvc = a.dv <= 64 ? 64 : (a.dv <= 128 ? 128 : 256);
+    f.nchunk = div_up(a.dv, f.dvc);
+    const int kq = 32, kk = elem == 4 ? 16 : 32;                    // rows per wave
+    f.w_q = a.Lq <= kq ? 1 : 4;
+    f.w_k = a.Lk <= 2 * kk ? (a.Lk <= kk ? 1 : 2) : 4;
+    f.rows_q = kq * f.w_q;
+    f.rows_k = kk * f.w_k;
+    f.nrow_q = div_up(a.Lq, f.rows_q);
+    f.nrow_k = div_up(a.Lk, f.rows_k);
+    f.nr = (long long)a.B * f.nchunk * f.nrow_q * f.w_q;
+    return f;
+}
+constexpr int DB_SPLITS = 64;
+
+struct BwdWs {
+    long long dO, delta, dq, dk, db, db2, total;
+};
+inline BwdWs layout_backward(const Args &a, int kind, int elem, const BwdPlan &f)
+{
+    BwdWs w;
+    long long at = 0;
+    const long long rows = (long long)a.B * a.Lq * a.H, keys = (long long)a.B * a.Lk * a.Hk;
+    const auto take = [&](long long bytes) { const long long r = at; at += align_up(bytes); return r; };
+    w.dO = take(a.gate ? rows * a.dv * elem : 0);
+    w.delta = take(kind == SOFTMAX ? rows * 4 : 0);
+    w.dq = take(f.nchunk > 1 ? rows * a.dk * f.nchunk * 4 : 0);
+    w.dk = take(f.nchunk > 1 ? keys * a.dk * f.nchunk * 4 : 0);
+    w.db = take(a.table ? f.nr * a.H * (2 * a.D + 1) * 4 : 0);
+    w.db2 = take(a.table ? (long long)DB_SPLITS * a.H * (2 * a.D + 1) * 4 : 0);
+    w.total = at;
+    return w;
+}
+
+// sums of the waves' distance rows in a fixed order: (H, R, TW) -> (H, S, TW) -> bucket by bucket (num_buckets, H)
+static __global__ void __launch_bounds__(256) db_rows_kernel(const float *part, float *out, long long R, int TW)
+{
+    const int h = blockIdx.x / DB_SPLITS, s = blockIdx.x % DB_SPLITS;
+    const long long per = (R + DB_SPLITS - 1) / DB_SPLITS, r0 = s * per, r1 = r0 + per < R ? r0 + per : R;
+    for (int t = threadIdx.x; t < TW; t += 256) {
+        float x = 0.f;
+        for (long long r = r0; r < r1; ++r) x += part[(h * R + r) * TW + t];
+        out[(long long)blockIdx.x * TW + t] = x;
+    }
+}
+template <class T> __global__ void __launch_bounds__(256) db_buckets_kernel(const float *part, const int *bucket_of, void *dtable, int H, int TW, int nb, int f32)
+{
+    extern __shared__ float sums[];
+    int *bk = reinterpret_cast<int *>(sums + TW);
+    const int h = blockIdx.x;
+    for (int t = threadIdx.x; t < TW; t += 256) {
+        float x = 0.f;
+        for (int s = 0; s < DB_SPLITS; ++s) x += part[((long long)h * DB_SPLITS + s) * TW + t];
+        sums[t] = x;
+        const int b = bucket_of[t];
+        bk[t] = b < 0 ? 0 : (b >= nb ? nb - 1 : b);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < nb; b += 256) {
+        float x = 0.f;
+        for (int t = 0; t < TW; ++t) x += bk[t] == b ? sums[t] : 0.f;
+        if (f32) reinterpret_cast<float *>(dtable)[(long long)b * H + h] = x;
+        else reinterpret_cast<T *>(dtable)[(long long)b * H + h] = (T)x;
+    }
+}
+
+template <class K> int launch(K kernel, long long blocks, int threads, size_t smem, const Args &a, hipStream_t st)
+{
+    if (blocks <= 0) return TLK_OK;
+    if (blocks > 0x7fffffffLL) return fail(TLK_EINVAL, "tlk_gau_attention: more than 2^31 - 1 workgroups");
+    if (smem > 160 * 1024) return fail(TLK_EINVAL, "tlk_gau_attention: max_distance beyond the LDS tile");
+    if (smem > 64 * 1024) TLK_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), smem, st, a);
+    TLK_HIP(hipGetLastError());
+    return TLK_OK;
+}
+
+template <class T, int KIND, int DK, int MT, int NT, int WM, int WN> int launch_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
+{
+    constexpr int KT = 32, PAD = 16 / sizeof(T);
+    const size_t smem = sizeof(T) * KT * ((DK + PAD) + (WN * NT * 16 + 2 * PAD)) + (a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * (2 * a.D + 1) : 0);
+    return launch(fwd_kernel<T, KIND, DK, MT, NT, WM, WN, KT>, (long long)a.B * f.heads * f.nsplit * f.nchunk * f.nrow, 64 * WM * WN, smem, a, st);
+}
+template <class T, int KIND, int DK> int pick_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
+{
+    if (!f.few) {
+        if (f.dvb == 64) return launch_fwd<T, KIND, DK, 2, 4, 4, 1>(a, f, st);
+        if (f.dvb == 128) return launch_fwd<T, KIND, DK, 2, 8, 4, 1>(a, f, st);
+        return launch_fwd<T, KIND, DK, 2, 16, 4, 1>(a, f, st);
+    }
+    if (f.mt == 1) {
+        if (f.dvb == 64) return launch_fwd<T, KIND, DK, 1, 1, 1, 4>(a, f, st);
+        if (f.dvb == 128) return launch_fwd<T, KIND, DK, 1, 2, 1, 4>(a, f, st);
+        if (f.dvb == 256) return launch_fwd<T, KIND, DK, 1, 4, 1, 4>(a, f, st);
+        return launch_fwd<T, KIND, DK, 1, 8, 1, 4>(a, f, st);
+    }
+    if (f.dvb == 64) return launch_fwd<T, KIND, DK, 2, 1, 1, 4>(a, f, st);
+    if (f.dvb == 128) return launch_fwd<T, KIND, DK, 2, 2, 1, 4>(a, f, st);
+    if (f.dvb == 256) return launch_fwd<T, KIND, DK, 2, 4, 1, 4>(a, f, st);
+    return launch_fwd<T, KIND, DK, 2, 8, 1, 4>(a, f, st);
+}
+template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
+{
+    const FwdPlan f = plan_forward(a);
+    a.fold = f.fold; a.nrow = f.nrow; a.nchunk = f.nchunk; a.nsplit = f.nsplit; a.split_keys = f.split_keys;
+    const long long rows = (long long)a.B * a.Lq * a.H;
+    a.part = reinterpret_cast<float *>(ws);
+    a.ml = a.part + (f.nsplit > 1 ? rows * a.dv * f.nsplit : 0);
+    int rc;
+    if (kind == SOFTMAX) rc = a.dk <= 64 ? pick_fwd<T, SOFTMAX, 64>(a, f, st) : pick_fwd<T, SOFTMAX, 128>(a, f, st);
+    else rc = a.dk <= 64 ? pick_fwd<T, RELU2, 64>(a, f, st) : pick_fwd<T, RELU2, 128>(a, f, st);
+    if (rc != TLK_OK || f.nsplit == 1) return rc;
+    const long long blocks = (rows * (a.dv / 4) + 255) / 256;
+    return kind == SOFTMAX ? launch(join_kernel<T, SOFTMAX>, blocks, 256, 0, a, st) : launch(join_kernel<T, RELU2>, blocks, 256, 0, a, st);
+}
+
+template <class T, int KIND, int DK, int DVC, int W> int launch_dq(const Args &a, const BwdPlan &f, hipStream_t st)
+{
+    constexpr int PAD = 16 / sizeof(T);
+    const size_t smem = sizeof(T) * 32 * ((DK + PAD) + (DVC + PAD)) + (a.table ? sizeof(float) * ((1 + W) * (2 * a.D + 1) + W * 32 * 33) : 0);
+    return launch(dq_kernel<T, KIND, DK, DVC, 2, W>, (long long)a.B * a.H * f.nchunk * f.nrow_q, 64 * W, smem, a, st);
+}
+template <class T, int KIND, int DK, int DVC, int W> int launch_dkv(const Args &a, const BwdPlan &f, hipStream_t st)
+{
+    constexpr int PAD = 16 / sizeof(T);
+    const size_t smem = sizeof(T) * 32 * ((DK + PAD) + (DVC + PAD)) + 64 * sizeof(float) + (a.table ? sizeof(float) * (2 * a.D + 1) : 0);
+    return launch(dkv_kernel<T, KIND, DK, DVC, sizeof(T) == 4 ? 1 : 2, W>, (long long)a.B * a.Hk * f.nchunk * f.nrow_k, 64 * W, smem, a, st);
+}
+template <class T, int KIND, int DK, int DVC> int pick_bwd(Args a, const BwdPlan &f, hipStream_t st)
+{
+    a.nchunk = f.nchunk;
+    a.nrow = f.nrow_q;
+    int rc = f.w_q == 1 ? launch_dq<T, KIND, DK, DVC, 1>(a, f, st) : launch_dq<T, KIND, DK, DVC, 4>(a, f, st);
+    if (rc != TLK_OK) return rc;
+    a.nrow = f.nrow_k;
+    if (f.w_k == 1) return launch_dkv<T, KIND, DK, DVC, 1>(a, f, st);
+    if (f.w_k == 2) return launch_dkv<T, KIND, DK, DVC, 2>(a, f, st);
+    return launch_dkv<T, KIND, DK, DVC, 4>(a, f, st);
+}
+template <class T, int KIND> int pick_bwd_sizes(const Args &a, const BwdPlan &f, hipStream_t st)
+{
+    if (a.dk <= 64) return f.dvc == 64 ? pick_bwd<T, KIND, 64, 64>(a, f, st) : (f.dvc == 128 ? pick_bwd<T, KIND, 64, 128>(a, f, st) : pick_bwd<T, KIND, 64, 256>(a, f, st));
+    return f.dvc == 64 ? pick_bwd<T, KIND, 128, 64>(a, f, st) : (f.dvc == 128 ? pick_bwd<T, KIND, 128, 128>(a, f, st) : pick_bwd<T, KIND, 128, 256>(a, f, st));
+}
+template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t st)
+{
+    const BwdPlan f = plan_backward(a, sizeof(T));
+    const BwdWs w = layout_backward(a, kind, sizeof(T), f);
+    char *ws = reinterpret_cast<char *>(io.ws);
+    const long long rows = (long long)a.B * a.Lq * a.H, keys = (long long)a.B * a.Lk * a.Hk;
+    a.dO = io.dout;
+    if ((a.gate || kind == SOFTMAX) && rows > 0) {
+        GateArgs<T> ga;
+        ga.dout = reinterpret_cast<const T *>(io.dout); ga.gate = reinterpret_cast<const T *>(a.gate); ga.o = reinterpret_cast<const T *>(io.o);
+        for (int i = 0; i < 3; ++i) ga.gs[i] = a.gs[i];
+        ga.dO = a.gate ? reinterpret_cast<T *>(ws + w.dO) : nullptr;
+        ga.dgate = reinterpret_cast<T *>(io.dgate);
+        ga.delta = kind == SOFTMAX ? reinterpret_cast<float *>(ws + w.delta) : nullptr;
+        ga.rows = rows; ga.Lq = a.Lq; ga.H = a.H; ga.dv = a.dv;
+        if ((rows + 3) / 4 > 0x7fffffffLL) return fail(TLK_EINVAL, "tlk_gau_attention: more than 2^31 - 1 workgroups");
+        hipLaunchKernelGGL(gate_bwd_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, ga);
+        TLK_HIP(hipGetLastError());
+        if (a.gate) a.dO = ws + w.dO;
+        a.delta = ga.delta;
+    }
+    a.dq = io.dq; a.dk_ = io.dk; a.dv_ = io.dv;
+    a.dq_part = reinterpret_cast<float *>(ws + w.dq);
+    a.dk_part = reinterpret_cast<float *>(ws + w.dk);
+    a.db_part = reinterpret_cast<float *>(ws + w.db);
+    int rc = kind == SOFTMAX ? pick_bwd_sizes<T, SOFTMAX>(a, f, st) : pick_bwd_sizes<T, RELU2>(a, f, st);
+    if (rc != TLK_OK) return rc;
+    if (f.nchunk > 1) {
+        if (rows > 0) hipLaunchKernelGGL(sum_chunks_kernel<T>, dim3((unsigned)((rows * a.dk / 4 + 255) / 256)), dim3(256), 0, st, a.dq_part, reinterpret_cast<T *>(a.dq), rows * a.dk, f.nchunk);
+        if (keys > 0) hipLaunchKernelGGL(sum_chunks_kernel<T>, dim3((unsigned)((keys * a.dk / 4 + 255) / 256)), dim3(256), 0, st, a.dk_part, reinterpret_cast<T *>(a.dk_), keys * a.dk, f.nchunk);
+        TLK_HIP(hipGetLastError());
+    }
+    if (a.table) {
+        const int TW = 2 * a.D + 1;
+        float *p2 = reinterpret_cast<float *>(ws + w.db2);
+        hipLaunchKernelGGL(db_rows_kernel, dim3((unsigned)(a.H * DB_SPLITS)), dim3(256), 0, st, a.db_part, p2, f.nr, TW);
+        hipLaunchKernelGGL(db_buckets_kernel<T>, dim3((unsigned)a.H), dim3(256), (size_t)TW * 8, st, p2, a.bucket_of, io.dtable, a.H, TW, a.nb, a.table_f32);
+        TLK_HIP(hipGetLastError());
+    }
+    return TLK_OK;
+}
+
+}  // namespace gau
+}  // namespace tlk

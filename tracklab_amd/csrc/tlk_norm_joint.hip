@@ -1,0 +1,562 @@
+// tlk_norm_joint.hip -- the joint of two blocks in one pass over its rows (tlk_norm_gate_residual_fwd / _bwd):
+//     y = res_scale * x + gate * N1(h),   z = N2(y)
+// with N one of: ScaleNorm v g / max(|v| / sqrt d, eps), RMS norm v w / sqrt(mean v^2 + eps), layer norm, or nothing.
+//
+// Bound by HBM: every tensor is read or written once.  LPR lanes hold one row in registers (16-byte loads; odd widths and row strides: one value
+// at a time), statistics are reduced across those lanes in fp32, and y goes from the first norm to the second unrounded.  The backward pass keeps
+// nothing of the forward pass: it forms N1(h), y and both statistics again from the rows it has to read anyway.  Column sums (gradients of weights,
+// biases, res_scale and of a shared gate) stay in registers over all rows of a workgroup, are joined over its row slots through LDS, and a second
+// launch adds the workgroups' sums in a fixed order: no atomics, equal bits on every run.
+#include <initializer_list>
+
+#include "tlk_common.hpp"
+
+using namespace tlk;
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+
+enum { NONE = TLK_NORM_NONE, SCALE = TLK_NORM_SCALE, RMS = TLK_NORM_RMS, LAYER = TLK_NORM_LAYER };
+enum { A_RS, A_GATE, A_W1, A_B1, A_W2, A_B2, N_ACC };
+
+struct NormArgs {
+    const void *h, *x, *gate, *rs, *w1, *b1, *w2, *b2, *dy, *dz;
+    void *y, *z, *dh, *dx, *dgate;
+    long long hs, xs, gs;            // row strides
+    long long rows, per_gate;        // rows that share a gate row (1: one each)
+    int d, n1, n2;
+    float eps1, eps2;
+    float *part;                     // (workgroup, array, d)
+    int groups, per_group;           // workgroups: `per_group` for each of `groups` runs of rows_in_group rows
+    long long rows_in_group;
+    int slot[N_ACC], nacc;           // which arrays are kept, and where
+};
+
+// E = NV * V values a lane; value e of lane t sits in column (e / V * LPR + t) * V + e % V
+template <class T, int LPR, int NV, int V> struct Row {
+    static constexpr int E = NV * V;
+    static __device__ __forceinline__ int col(int e, int t) { return ((e / V) * LPR + t) * V + e % V; }
+    static __device__ __forceinline__ void load(const void *base, long long off, int d, int t, float (&r)[E], float pad = 0.f)
+    {
+        const T *p = reinterpret_cast<const T *>(base) + off;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * LPR + t) * V;
+            if constexpr (V == 1) {
+                r[v] = c < d ? (float)p[c] : pad;
+            } else {
+                u4 raw = {0, 0, 0, 0};
+                const bool in = c < d;
+                if (in) raw = *reinterpret_cast<const u4 *>(p + c);
+                T el[V];
+                __builtin_memcpy(el, &raw, 16);
+#pragma unroll
+                for (int i = 0; i < V; ++i) r[v * V + i] = in ? (float)el[i] : pad;
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(void *base, long long off, int d, int t, const float (&r)[E])
+    {
+        T *p = reinterpret_cast<T *>(base) + off;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * LPR + t) * V;
+            if (c >= d) continue;
+            if constexpr (V == 1) {
+                p[c] = (T)r[v];
+            } else {
+                T el[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) el[i] = (T)r[v * V + i];
+                u4 raw;
+                __builtin_memcpy(&raw, el, 16);
+                *reinterpret_cast<u4 *>(p + c) = raw;
+            }
+        }
+    }
+};
+
+// sum over the LPR lanes of a row; LPR = 256: four waves through LDS (two buffers in turn, so one barrier is enough)
+template <int LPR> struct Sum {
+    float *s;                        // [2][rows of the workgroup * 4]
+    int flip = 0;
+    __device__ __forceinline__ float operator()(float v)
+    {
+#pragma unroll
+        for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        if constexpr (LPR > 64) {
+            const int w = threadIdx.x >> 6, n = blockDim.x >> 6, first = w / (LPR / 64) * (LPR / 64);
+            if ((threadIdx.x & 63) == 0) s[flip * n + w] = v;
+            __syncthreads();
+            v = 0.f;
+#pragma unroll
+            for (int i = 0; i < LPR / 64; ++i) v += s[flip * n + first + i];
+            flip ^= 1;
+        }
+        return v;
+    }
+};
+
+// v -> hat (the normalised row before weight and bias), returns 1 / its norm; `live`: what of it follows the row (0 below ScaleNorm's floor)
+template <int E, class S> __device__ __forceinline__ float normalise(int kind, const float (&v)[E], float (&hat)[E], const bool (&in)[E], int d, float eps, S &sum, float &live)
+{
+    if (kind == NONE) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) hat[e] = v[e];
+        live = 1.f;
+        return 1.f;
+    }
+    float mean = 0.f;
+    if (kind == LAYER) {
+        float t = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) t += v[e];
+        mean = sum(t) / (float)d;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        hat[e] = in[e] ? v[e] - mean : 0.f;
+        q = __builtin_fmaf(hat[e], hat[e], q);
+    }
+    q = sum(q) / (float)d;
+    float inv;
+    if (kind == SCALE) {
+        const float n = sqrtf(q);
+        inv = 1.f / (n < eps ? eps : n);
+        live = n < eps ? 0.f : inv;
+    } else {
+        inv = live = 1.f / sqrtf(q + eps);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) hat[e] *= inv;
+    return inv;
+}
+
+// gradient of the row through `hat`: t = gradient of the weighted row times the weight, in place
+template <int E, class S> __device__ __forceinline__ void normalise_bwd(int kind, float (&t)[E], const float (&hat)[E], const bool (&in)[E], int d, float inv, float live, S &sum)
+{
+    if (kind == NONE) return;
+    float a = 0.f, m = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        a = __builtin_fmaf(t[e], hat[e], a);
+        m += t[e];
+    }
+    a = sum(a) / (float)d;
+    m = kind == LAYER ? sum(m) / (float)d : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) t[e] = in[e] ? (t[e] - m) * inv - hat[e] * live * a : 0.f;
+}
+
+template <class R, class T> __device__ __forceinline__ void load_weight(int kind, const void *w, int d, int t, float (&r)[R::E])
+{
+    if (kind == NONE || !w) {
+#pragma unroll
+        for (int e = 0; e < R::E; ++e) r[e] = 1.f;
+    } else if (kind == SCALE) {
+        const float g = (float)*reinterpret_cast<const T *>(w);
+#pragma unroll
+        for (int e = 0; e < R::E; ++e) r[e] = g;
+    } else {
+        R::load(w, 0, d, t, r);
+    }
+}
+
+template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(256) joint_fwd_kernel(const NormArgs p)
+{
+    using R = Row<T, LPR, NV, V>;
+    constexpr int E = R::E;
+    __shared__ float s[2 * 4];
+    const long long row0 = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    const int t = threadIdx.x % LPR;
+    const bool live_row = row0 < p.rows;
+    const long long row = live_row ? row0 : p.rows - 1;                  // (lanes without a row take part in the reductions)
+    Sum<LPR> sum{s};
+    bool in[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) in[e] = R::col(e, t) < p.d;
+    float v[E], y[E], u[E];
+    R::load(p.h, row * p.hs, p.d, t, v);
+    if (p.x) R::load(p.x, row * p.xs, p.d, t, u);
+    float unused;
+    (void)normalise<E>(p.n1, v, y, in, p.d, p.eps1, sum, unused);
+    if (p.n1 != NONE) {
+        float w[E];
+        load_weight<R, T>(p.n1, p.w1, p.d, t, w);
+        if (p.b1) {
+            float b[E];
+            R::load(p.b1, 0, p.d, t, b);
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = __builtin_fmaf(y[e], w[e], b[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] *= w[e];
+        }
+    }
+    if (p.gate) {
+        float gt[E];
+        R::load(p.gate, row / p.per_gate * p.gs, p.d, t, gt);
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] *= gt[e];
+    }
+    if (p.x) {
+        if (p.rs) {
+            float r[E];
+            R::load(p.rs, 0, p.d, t, r);
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = __builtin_fmaf(u[e], r[e], y[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] += u[e];
+        }
+    }
+    if (live_row) R::store(p.y, row * p.d, p.d, t, y);
+    if (!p.z) return;                                                    // (uniform over the launch)
+    (void)normalise<E>(p.n2, y, v, in, p.d, p.eps2, sum, unused);
+    float w[E];
+    load_weight<R, T>(p.n2, p.w2, p.d, t, w);
+    if (p.b2) {
+        float b[E];
+        R::load(p.b2, 0, p.d, t, b);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = __builtin_fmaf(v[e], w[e], b[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= w[e];
+    }
+    if (live_row) R::store(p.z, row * p.d, p.d, t, v);
+}
+
+constexpr int BT = 512;                                                  // threads of a backward workgroup: one per CU, rows in turn
+
+template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(BT) joint_bwd_kernel(const NormArgs p)
+{
+    using R = Row<T, LPR, NV, V>;
+    constexpr int E = R::E, SLOTS = BT / LPR;
+    extern __shared__ float lds[];
+    __shared__ float s[2 * (BT / 64)];
+    const int t = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+    const long long grp = blockIdx.x / p.per_group, first = grp * p.rows_in_group, in_grp = blockIdx.x % p.per_group;
+    Sum<LPR> sum{s};
+    bool in[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) in[e] = R::col(e, t) < p.d;
+    float acc[N_ACC][E];
+#pragma unroll
+    for (int a = 0; a < N_ACC; ++a)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[a][e] = 0.f;
+    const long long step = (long long)p.per_group * SLOTS;
+    for (long long r0 = in_grp * SLOTS; r0 < p.rows_in_group; r0 += step) {            // (uniform over the workgroup: the reductions hold barriers)
+        const bool live = r0 + slot < p.rows_in_group;
+        const long long row = first + (live ? r0 + slot : r0);
+        float h[E], x[E], gt[E], dy[E], dz[E], w[E];
+        R::load(p.h, row * p.hs, p.d, t, h);
+        if (p.x) R::load(p.x, row * p.xs, p.d, t, x);
+        if (p.gate) R::load(p.gate, row / p.per_gate * p.gs, p.d, t, gt);
+        if (p.dy) R::load(p.dy, row * p.d, p.d, t, dy);
+        else
+#pragma unroll
+            for (int e = 0; e < E; ++e) dy[e] = 0.f;
+        if (p.dz) R::load(p.dz, row * p.d, p.d, t, dz);
+        float hat1[E], n1[E], live1, live2, inv2 = 1.f;
+        const float inv1 = normalise<E>(p.n1, h, hat1, in, p.d, p.eps1, sum, live1);
+        load_weight<R, T>(p.n1, p.w1, p.d, t, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) n1[e] = hat1[e] * w[e];
+        if (p.b1) {
+            float b[E];
+            R::load(p.b1, 0, p.d, t, b);
+#pragma unroll
+            for (int e = 0; e < E; ++e) n1[e] += b[e];
+        }
+        float rs[E];
+        if (p.x && p.rs) R::load(p.rs, 0, p.d, t, rs);
+        else
+#pragma unroll
+            for (int e = 0; e < E; ++e) rs[e] = 1.f;
+        if (p.dz) {
+            float hat2[E], y[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                y[e] = p.gate ? n1[e] * gt[e] : n1[e];
+                if (p.x) y[e] = __builtin_fmaf(x[e], rs[e], y[e]);
+            }
+            inv2 = normalise<E>(p.n2, y, hat2, in, p.d, p.eps2, sum, live2);
+            if (live) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    acc[A_W2][e] = __builtin_fmaf(dz[e], hat2[e], acc[A_W2][e]);
+                    acc[A_B2][e] += dz[e];
+                }
+            }
+            float w2[E];
+            load_weight<R, T>(p.n2, p.w2, p.d, t, w2);
+#pragma unroll
+            for (int e = 0; e < E; ++e) dz[e] *= w2[e];
+            normalise_bwd<E>(p.n2, dz, hat2, in, p.d, inv2, live2, sum);
+#pragma unroll
+            for (int e = 0; e < E; ++e) dy[e] += dz[e];
+        }
+        if (p.x) {
+            if (live) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[A_RS][e] = __builtin_fmaf(dy[e], x[e], acc[A_RS][e]);
+            }
+            if (p.dx) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = dy[e] * rs[e];
+                if (live) R::store(p.dx, row * p.d, p.d, t, x);
+            }
+        }
+        if (p.gate) {
+            float dg[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) dg[e] = dy[e] * n1[e];
+            if (p.per_gate == 1) {
+                if (live && p.dgate) R::store(p.dgate, row * p.d, p.d, t, dg);
+            } else if (live) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[A_GATE][e] += dg[e];
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) dy[e] *= gt[e];
+        }
+        if (live) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                acc[A_W1][e] = __builtin_fmaf(dy[e], hat1[e], acc[A_W1][e]);
+                acc[A_B1][e] += dy[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) dy[e] *= w[e];
+        normalise_bwd<E>(p.n1, dy, hat1, in, p.d, inv1, live1, sum);
+        if (live && p.dh) R::store(p.dh, row * p.d, p.d, t, dy);
+    }
+    // the workgroup's column sums: its row slots joined in LDS, one array after the other
+    const int CW = LPR * E;
+#pragma unroll
+    for (int a = 0; a < N_ACC; ++a) {
+        if (p.slot[a] < 0) continue;
+        float *dst = p.part + ((long long)blockIdx.x * p.nacc + p.slot[a]) * p.d;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) lds[slot * CW + R::col(e, t)] = acc[a][e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < p.d; c += BT) {
+            float v = 0.f;
+            for (int i = 0; i < SLOTS; ++i) v += lds[i * CW + c];
+            dst[c] = v;
+        }
+    }
+}
+
+struct ColArgs {
+    const float *part;               // (workgroups, nacc, d)
+    void *out[N_ACC];
+    int slot[N_ACC], scalar[N_ACC], d, nacc, groups, per_group;
+};
+// adds the workgroups' column sums: 64 columns x 4 runs of workgroups a block; ScaleNorm's one weight is summed over the columns as well
+template <class T> __global__ void __launch_bounds__(256) joint_cols_kernel(const ColArgs p)
+{
+    __shared__ float s[4][64];
+    const int a = blockIdx.y, cg = threadIdx.x & 63, rg = threadIdx.x >> 6;
+    if (p.slot[a] < 0) return;
+    const bool per_gate = a == A_GATE;
+    const int ng = per_gate ? p.groups : 1, nb = per_gate ? p.per_group : p.groups * p.per_group;
+    if ((int)blockIdx.z >= ng) return;
+    const int first = blockIdx.z * nb, share = (nb + 3) / 4, b0 = rg * share, b1 = min(nb, b0 + share);
+    float total = 0.f;
+    for (int c0 = p.scalar[a] ? 0 : (int)blockIdx.x * 64; c0 < p.d; c0 += 64) {
+        const int c = c0 + cg;
+        float v = 0.f;
+        if (c < p.d)
+            for (int b = b0; b < b1; ++b) v += p.part[((long long)(first + b) * p.nacc + p.slot[a]) * p.d + c];
+        total += v;
+        if (!p.scalar[a]) break;
+    }
+    if (p.scalar[a] && blockIdx.x > 0) return;                             // (uniform over the block)
+    s[rg][cg] = total;
+    __syncthreads();
+    if (rg) return;
+    float v = s[0][cg] + s[1][cg] + s[2][cg] + s[3][cg];
+    if (p.scalar[a]) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        if (cg == 0) *reinterpret_cast<T *>(p.out[a]) = (T)v;
+        return;
+    }
+    const int c = blockIdx.x * 64 + cg;
+    if (c < p.d) reinterpret_cast<T *>(p.out[a])[(long long)blockIdx.z * p.d + c] = (T)v;
+}
+
+template <class T, int LPR, int NV, int V> int fwd_launch(const NormArgs &a, hipStream_t st)
+{
+    const long long blocks = (a.rows + 256 / LPR - 1) / (256 / LPR);
+    if (blocks > 0x7fffffffLL) return fail(TLK_EINVAL, "tlk_norm_gate_residual: more than 2^31 - 1 workgroups");
+    hipLaunchKernelGGL((joint_fwd_kernel<T, LPR, NV, V>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    TLK_HIP(hipGetLastError());
+    return TLK_OK;
+}
+template <class T, int LPR, int NV, int V> int bwd_launch(const NormArgs &a, hipStream_t st)
+{
+    const size_t smem = (size_t)BT * NV * V * sizeof(float);
+    if (smem > 48 * 1024) TLK_HIP(hipFuncSetAttribute((const void *)joint_bwd_kernel<T, LPR, NV, V>, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+    hipLaunchKernelGGL((joint_bwd_kernel<T, LPR, NV, V>), dim3((unsigned)(a.groups * a.per_group)), dim3(BT), smem, st, a);
+    TLK_HIP(hipGetLastError());
+    return TLK_OK;
+}
+
+// lanes a row: enough that a lane holds at most 16 values (8192 columns in float32: 32)
+template <class T> int pick(const NormArgs &a, bool vec, bool bwd, hipStream_t st)
+{
+    constexpr int V = 16 / sizeof(T);
+#define GO(L, N, W) (bwd ? bwd_launch<T, L, N, W>(a, st) : fwd_launch<T, L, N, W>(a, st))
+    if (vec) {
+        const int v = (a.d + V - 1) / V;                                   // 16-byte vectors of a row
+        if (v <= 32) return GO(32, 1, V);
+        if (v <= 64) return GO(64, 1, V);
+        if (v <= 128) return GO(64, 2, V);
+        if (v <= 256) return GO(256, 1, V);
+        if (v <= 512) return GO(256, 2, V);
+        if (v <= 1024) return GO(256, 4, V);
+        if constexpr (V == 4) return GO(256, 8, V);
+        return fail(TLK_EINVAL, "tlk_norm_gate_residual: more than 8192 columns");
+    }
+    if (a.d <= 256) return GO(64, 4, 1);
+    if (a.d <= 1024) return GO(64, 16, 1);
+    if (a.d <= 4096) return GO(256, 16, 1);
+    return GO(256, 32, 1);
+#undef GO
+}
+
+// 256 workgroups walk the rows (one per CU); a shared gate's gradient is kept per run of rows, so every run gets workgroups of its own
+void cut(const tlk_norm_args *a, NormArgs &n)
+{
+    const long long groups = a->gate && a->gate_rows > 1 ? (a->rows + a->gate_rows - 1) / a->gate_rows : 1;
+    n.groups = (int)(groups < 1 ? 1 : groups);
+    n.rows_in_group = a->rows / n.groups;
+    const int slots = a->dim <= 256 ? 16 : 2;
+    long long per = (256 + n.groups - 1) / n.groups, most = (n.rows_in_group + slots - 1) / slots;
+    n.per_group = (int)(per < most ? per : (most < 1 ? 1 : most));
+}
+int arrays(const tlk_norm_args *a, int (&slot)[N_ACC])
+{
+    int n = 0;
+    slot[A_RS] = a->res_scale ? n++ : -1;
+    slot[A_GATE] = a->gate && a->gate_rows > 1 ? n++ : -1;
+    slot[A_W1] = a->norm != TLK_NORM_NONE ? n++ : -1;
+    slot[A_B1] = a->norm == TLK_NORM_LAYER && a->bias ? n++ : -1;
+    slot[A_W2] = a->next_norm != TLK_NORM_NONE ? n++ : -1;
+    slot[A_B2] = a->next_norm == TLK_NORM_LAYER && a->next_bias ? n++ : -1;
+    return n;
+}
+
+int check(const tlk_norm_args *a, const char *fn)
+{
+    const std::string f(fn);
+    if (!a) return fail(TLK_EINVAL, f + ": null arguments");
+    if (a->dtype != TLK_F32 && a->dtype != TLK_F16 && a->dtype != TLK_BF16) return fail(TLK_EINVAL, f + ": dtype must be TLK_F32, TLK_F16 or TLK_BF16");
+    if (a->norm < 0 || a->norm > TLK_NORM_LAYER || a->next_norm < 0 || a->next_norm > TLK_NORM_LAYER) return fail(TLK_EINVAL, f + ": unknown norm");
+    if (a->rows < 0 || a->dim < 1 || a->dim > 8192) return fail(TLK_EINVAL, f + ": rows must be >= 0 and 1 <= dim <= 8192");
+    if (!(a->eps >= 0.f) || !(a->next_eps >= 0.f)) return fail(TLK_EINVAL, f + ": eps must not be negative");
+    if (a->rows > 0 && !a->h) return fail(TLK_EINVAL, f + ": null input");
+    if ((a->norm != TLK_NORM_NONE && !a->weight) || (a->next_norm != TLK_NORM_NONE && !a->next_weight)) return fail(TLK_EINVAL, f + ": a norm needs its weight");
+    if ((a->norm != TLK_NORM_LAYER && a->bias) || (a->next_norm != TLK_NORM_LAYER && a->next_bias)) return fail(TLK_EINVAL, f + ": only the layer norm takes a bias");
+    if (a->res_scale && !a->x) return fail(TLK_EINVAL, f + ": res_scale without a residual");
+    if (a->h_stride < a->dim || (a->x && a->x_stride < a->dim) || (a->gate && a->gate_stride < a->dim)) return fail(TLK_EINVAL, f + ": row strides must be >= dim");
+    if (a->gate && (a->gate_rows < 1 || (a->rows > 0 && a->rows % a->gate_rows != 0))) return fail(TLK_EINVAL, f + ": rows must be a multiple of gate_rows");
+    if (a->gate && a->gate_rows > 1 && a->rows / a->gate_rows > 65535) return fail(TLK_EINVAL, f + ": more than 65535 shared gate rows");
+    return TLK_OK;
+}
+
+bool vector_rows(const tlk_norm_args *a, std::initializer_list<const void *> more)
+{
+    const int size = a->dtype == TLK_F32 ? 4 : 2, v = 16 / size;
+    uintptr_t bits = (uintptr_t)a->h | (uintptr_t)a->x | (uintptr_t)a->gate | (uintptr_t)a->res_scale | (uintptr_t)a->bias | (uintptr_t)a->next_bias;
+    if (a->norm == TLK_NORM_RMS || a->norm == TLK_NORM_LAYER) bits |= (uintptr_t)a->weight;
+    if (a->next_norm == TLK_NORM_RMS || a->next_norm == TLK_NORM_LAYER) bits |= (uintptr_t)a->next_weight;
+    for (const void *p : more) bits |= (uintptr_t)p;
+    return (bits & 15) == 0 && a->dim % v == 0 && a->h_stride % v == 0 && (!a->x || a->x_stride % v == 0) && (!a->gate || a->gate_stride % v == 0);
+}
+
+NormArgs common(const tlk_norm_args *a)
+{
+    NormArgs n;
+    memset(&n, 0, sizeof(n));
+    n.h = a->h; n.x = a->x; n.gate = a->gate; n.rs = a->res_scale;
+    n.w1 = a->weight; n.b1 = a->bias; n.w2 = a->next_weight; n.b2 = a->next_bias;
+    n.hs = a->h_stride; n.xs = a->x_stride; n.gs = a->gate_stride;
+    n.rows = a->rows; n.per_gate = a->gate ? a->gate_rows : 1;
+    n.d = a->dim; n.n1 = a->norm; n.n2 = a->next_norm; n.eps1 = a->eps; n.eps2 = a->next_eps;
+    return n;
+}
+
+}  // namespace
+
+extern "C" int tlk_norm_gate_residual_fwd(const tlk_norm_args *a, void *y_dev, void *z_dev, void *hip_stream)
+{
+    const int rc = check(a, "tlk_norm_gate_residual_fwd");
+    if (rc != TLK_OK) return rc;
+    if (a->rows == 0) return TLK_OK;
+    if ((a->next_norm != TLK_NORM_NONE) != (z_dev != nullptr)) return fail(TLK_EINVAL, "tlk_norm_gate_residual_fwd: z goes with the next norm");
+    if (!y_dev) return fail(TLK_EINVAL, "tlk_norm_gate_residual_fwd: null output");
+    NormArgs n = common(a);
+    n.y = y_dev; n.z = z_dev;
+    const bool vec = vector_rows(a, {y_dev, z_dev});
+    hipStream_t st = (hipStream_t)hip_stream;
+    if (a->dtype == TLK_F32) return pick<float>(n, vec, false, st);
+    return a->dtype == TLK_F16 ? pick<_Float16>(n, vec, false, st) : pick<__bf16>(n, vec, false, st);
+}
+
+extern "C" long long tlk_norm_gate_residual_workspace(const tlk_norm_args *a)
+{
+    const int rc = check(a, "tlk_norm_gate_residual_workspace");
+    if (rc != TLK_OK) return rc;
+    if (a->rows == 0) return 0;
+    NormArgs n = common(a);
+    cut(a, n);
+    int slot[N_ACC];
+    return (long long)n.groups * n.per_group * arrays(a, slot) * a->dim * (long long)sizeof(float);
+}
+
+extern "C" int tlk_norm_gate_residual_bwd(const tlk_norm_args *a, const void *dy_dev, const void *dz_dev, const tlk_norm_grads *g, void *workspace_dev,
+                                          long long workspace_bytes, void *hip_stream)
+{
+    const int rc = check(a, "tlk_norm_gate_residual_bwd");
+    if (rc != TLK_OK) return rc;
+    if (!g) return fail(TLK_EINVAL, "tlk_norm_gate_residual_bwd: null gradients");
+    if (dz_dev && a->next_norm == TLK_NORM_NONE) return fail(TLK_EINVAL, "tlk_norm_gate_residual_bwd: a gradient of z without the next norm");
+    int slot[N_ACC];
+    const int nacc = arrays(a, slot);
+    void *out[N_ACC] = {g->dres_scale, g->dgate, g->dweight, g->dbias, g->dnext_weight, g->dnext_bias};
+    for (int i = 0; i < N_ACC; ++i)
+        if (slot[i] >= 0 && !out[i]) return fail(TLK_EINVAL, "tlk_norm_gate_residual_bwd: a parameter's gradient has no place");
+    if (a->rows > 0 && (!g->dh || (a->x && !g->dx) || (a->gate && !g->dgate))) return fail(TLK_EINVAL, "tlk_norm_gate_residual_bwd: a gradient has no place");
+    if (a->rows == 0) return nacc ? fail(TLK_EINVAL, "tlk_norm_gate_residual_bwd: no rows") : TLK_OK;
+    NormArgs n = common(a);
+    cut(a, n);
+    if (nacc && (!workspace_dev || workspace_bytes < (long long)n.groups * n.per_group * nacc * a->dim * (long long)sizeof(float)))
+        return fail(TLK_EINVAL, "tlk_norm_gate_residual_bwd: workspace too small (tlk_norm_gate_residual_workspace)");
+    n.dy = dy_dev; n.dz = dz_dev; n.dh = g->dh; n.dx = g->dx; n.dgate = a->gate && a->gate_rows == 1 ? g->dgate : nullptr;
+    n.part = reinterpret_cast<float *>(workspace_dev);
+    n.nacc = nacc;
+    memcpy(n.slot, slot, sizeof(slot));
+    const bool vec = vector_rows(a, {dy_dev, dz_dev, g->dh, g->dx, n.dgate});
+    hipStream_t st = (hipStream_t)hip_stream;
+    const int rb = a->dtype == TLK_F32 ? pick<float>(n, vec, true, st) : (a->dtype == TLK_F16 ? pick<_Float16>(n, vec, true, st) : pick<__bf16>(n, vec, true, st));
+    if (rb != TLK_OK || !nacc) return rb;
+    ColArgs c;
+    c.part = n.part; c.d = n.d; c.nacc = nacc; c.groups = n.groups; c.per_group = n.per_group;
+    for (int i = 0; i < N_ACC; ++i) { c.out[i] = out[i]; c.slot[i] = slot[i]; c.scalar[i] = (i == A_W1 && a->norm == TLK_NORM_SCALE) || (i == A_W2 && a->next_norm == TLK_NORM_SCALE); }
+    const dim3 grid((unsigned)((n.d + 63) / 64), N_ACC, (unsigned)(slot[A_GATE] >= 0 ? n.groups : 1));
+    if (a->dtype == TLK_F32) hipLaunchKernelGGL(joint_cols_kernel<float>, grid, dim3(256), 0, st, c);
+    else if (a->dtype == TLK_F16) hipLaunchKernelGGL(joint_cols_kernel<_Float16>, grid, dim3(256), 0, st, c);
+    else hipLaunchKernelGGL(joint_cols_kernel<__bf16>, grid, dim3(256), 0, st, c);
+    TLK_HIP(hipGetLastError());
+    return TLK_OK;
+}

@@ -23,6 +23,7 @@ class HipRTMPose(ImageLevelModule):
         self.in_w, self.in_h = int(size[0]), int(size[1])
         self.arch = str(cfg_get(cfg, "arch", "m"))
         self.max_dets = int(cfg_get(cfg, "max_dets", 128))
+        self.rel_buckets = int(cfg_get(cfg, "rel_buckets", 0) or 0)                # > 0: the head's attention unit has a learned position bias
         self.checkpoint = cfg_get(cfg, "checkpoint", None)
         self._model = None
 
@@ -31,7 +32,7 @@ class HipRTMPose(ImageLevelModule):
             import torch
             from ..backbones.rtmpose import rtmpose
             self._torch = torch
-            self._model = rtmpose(self.arch, device=self.device, dtype=torch.float16, channels_last=True)
+            self._model = rtmpose(self.arch, device=self.device, dtype=torch.float16, channels_last=True, rel_buckets=self.rel_buckets)
             if self.checkpoint:          # state_dict, the reference's own ONNX artefact, or a BatchNorm ResNet-50 checkpoint (tracklab_amd/weights.py)
                 from ..weights import load_checkpoint
                 self.checkpoint_report = load_checkpoint(self._model, self.checkpoint, (torch.zeros(1, 3, self.in_h, self.in_w),))
