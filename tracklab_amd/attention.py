@@ -113,7 +113,7 @@ def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda
 def _fit(t, vn):
     """the tensor with a contiguous last dimension, 16-byte aligned rows and heads (as it is where it already has them), and its three strides"""
     s = t.stride()
-    if (t.shape[-1] > 1 and s[3] != 1) or t.data_ptr() % 16 or any(t.shape[i] > 1 and s[i] % vn for i in range(3)):
+    if (t.shape[-1] > 1 and s[3] != 1) or t.data_ptr() % 16 or any(t.shape[i] > 1 and s[i] % vn for i in range(3)) or (t.shape[1] > 1 and s[1] > 1 << 22):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()

@@ -26,7 +26,7 @@ int fill(const tlk_gau_args *a, gau::Args &p, const char *fn)
     if (a->batch < 0 || a->len_q < 0 || a->len_k < 0 || a->len_q > big || a->len_k > big) return fail(TLK_EINVAL, f + ": batch and lengths must lie in 0..2^28");
     if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads != 0 || a->heads > 65535) return fail(TLK_EINVAL, f + ": heads must be a positive multiple of kv_heads");
     if (a->dim_k < vn || a->dim_k % vn != 0 || a->dim_k > 128) return fail(TLK_EINVAL, f + ": dim_k must be a multiple of 16 bytes of elements, at most 128");
-    if (a->dim_v < vn || a->dim_v % vn != 0 || a->dim_v > 65536) return fail(TLK_EINVAL, f + ": dim_v must be a positive multiple of 16 bytes of elements");
+    if (a->dim_v < vn || a->dim_v % vn != 0 || a->dim_v > 65536 || (long long)a->heads * a->dim_v > 1 << 22) return fail(TLK_EINVAL, f + ": dim_v must be a positive multiple of 16 bytes of elements, heads * dim_v at most 2^22");
     if (a->num_buckets < 0 || a->max_distance < 0 || a->max_distance > 2048) return fail(TLK_EINVAL, f + ": max_distance must lie in 0..2048");
     if ((a->num_buckets > 0) != (a->table != nullptr) || (a->num_buckets > 0) != (a->bucket_of != nullptr)) return fail(TLK_EINVAL, f + ": a bias needs num_buckets, table and bucket_of");
     const long long rows = (long long)a->batch * a->len_q, keys = (long long)a->batch * a->len_k;
@@ -36,6 +36,7 @@ int fill(const tlk_gau_args *a, gau::Args &p, const char *fn)
     for (int i = 0; i < 3; ++i) {
         if (a->q_stride[i] % vn || a->k_stride[i] % vn || a->v_stride[i] % vn || (a->gate && a->gate_stride[i] % vn))
             return fail(TLK_EINVAL, f + ": strides must be multiples of 16 bytes");
+        if (i == 1 && (a->q_stride[i] > 1 << 22 || a->k_stride[i] > 1 << 22 || a->v_stride[i] > 1 << 22)) return fail(TLK_EINVAL, f + ": row strides of q, k and v must not pass 2^22 elements");
         if (a->q_stride[i] < 0 || a->k_stride[i] < 0 || a->v_stride[i] < 0 || (a->gate && a->gate_stride[i] < 0)) return fail(TLK_EINVAL, f + ": strides must not be negative");
     }
     memset(&p, 0, sizeof(p));
@@ -54,7 +55,7 @@ int kind_of(const tlk_gau_args *a) { return a->kind == TLK_GAU_SOFTMAX ? gau::SO
 long long workspace(const gau::Args &p, int kind, int size, bool backward)
 {
     if (!backward) {
-        const gau::FwdPlan f = gau::plan_forward(p);
+        const gau::FwdPlan f = gau::plan_forward(p, size);
         return f.nsplit > 1 ? (long long)p.B * p.Lq * p.H * (p.dv + 2) * f.nsplit * 4 : 0;
     }
     return gau::layout_backward(p, kind, size, gau::plan_backward(p, size)).total;

@@ -84,27 +84,82 @@ template <class T> __device__ __forceinline__ typename Ty<T>::V8 zero8()
     return r;
 }
 
-// eight consecutive values of a row
+// eight consecutive values of a row in global memory
 template <class T> __device__ __forceinline__ typename Ty<T>::V8 ld8(const T *p) { return *reinterpret_cast<const typename Ty<T>::V8 *>(p); }
 
-// values (row0 + 4 g + 0..3, col0 + l) of a row-major LDS tile, g = lane / 16, l = lane % 16: four rows of one column
-template <class T> __device__ __forceinline__ typename Ty<T>::V4 ld_col4(const T *tile, int ld, int g, int l)
-{
-    if constexpr (sizeof(T) == 2) {
-        const T *p = tile + (g * 4 + (l >> 2)) * ld + (l & 3) * 4;
-        s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(p));
-        return __builtin_bit_cast(typename Ty<T>::V4, r);
-    } else {
-        typename Ty<T>::V4 r;
+// A ROWS x COLS tile in LDS, filled by direct-to-LDS loads: 64 lanes x 16 bytes land in 1024 consecutive bytes, so the tile has no padding; instead the
+// 16-byte chunk c of row r stands at c ^ twist(r), which spreads the 16 rows of a fragment read and of a transposing read over all banks.  The loads go
+// through a buffer descriptor: rows behind the end and columns behind the width get an offset out of its range and arrive as zeros.
+template <class T, int ROWS, int COLS, int NW> struct Tile {
+    static constexpr int VN = 16 / sizeof(T), C = COLS / VN, ROWB = COLS * sizeof(T), BYTES = ROWS * ROWB, N = (ROWS * C / 64 + NW - 1) / NW;
+    static constexpr unsigned OOB = 0x80000000u;
+    static_assert(C >= 8 && (C & (C - 1)) == 0 && ROWS * C % 64 == 0, "whole wave loads of rows of at least 128 bytes");
+    static __device__ __forceinline__ int twist(int r) { return C >= 16 ? ((r << 1) & 15) | ((r >> 3) & 1) : (r >> 1) & 7; }
+    unsigned off[N];
+    int wave;
+    __device__ __forceinline__ void init(int w, int lane, long long rs, int cend)
+    {
+        wave = w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = tile[(g * 4 + i) * ld + l];
-        return r;
+        for (int i = 0; i < N; ++i) {
+            const int at = (i * NW + w) * 64 + lane, row = at / C, c = (at % C) ^ twist(row);
+            off[i] = c * VN < cend ? (unsigned)(row * (int)rs * (int)sizeof(T) + c * 16) : OOB;
+        }
     }
-}
-template <class T> __device__ __forceinline__ typename Ty<T>::V8 ld_col8(const T *tile, int ld, int g, int l)      // rows 4 g + 0..3 and 16 + 4 g + 0..3
+    // `rows`: how many of the tile's rows there are (uniform); `base`: its first row (uniform)
+    __device__ __forceinline__ void issue(const T *base, int rows, char *lds, int lane) const
+    {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int inst = i * NW + wave;
+            if (ROWS * C / 64 % NW != 0 && inst >= ROWS * C / 64) break;
+            unsigned o = off[i];
+            if (rows < ROWS) o = (inst * 64 + lane) / C < rows ? o : OOB;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + inst * 1024), 16, (int)o, 0, 0, 0);
+        }
+    }
+    // eight consecutive values of row r, from column k (a multiple of 8)
+    static __device__ __forceinline__ typename Ty<T>::V8 row8(const char *lds, int r, int k)
+    {
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const typename Ty<T>::V8 *>(lds + r * ROWB + ((k / 8 ^ twist(r)) << 4));
+        } else {
+            const f4 a = *reinterpret_cast<const f4 *>(lds + r * ROWB + ((k / 4 ^ twist(r)) << 4));
+            const f4 b = *reinterpret_cast<const f4 *>(lds + r * ROWB + (((k / 4 + 1) ^ twist(r)) << 4));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // rows r0 + 4 g + 0..3 of column c0 + l (g = lane / 16, l = lane % 16, r0 and c0 multiples of 16)
+    static __device__ __forceinline__ typename Ty<T>::V4 col4(const char *lds, int r0, int c0, int g, int l)
+    {
+        if constexpr (sizeof(T) == 2) {
+            const int r = g * 4 + (l >> 2), c = (c0 >> 3) + ((l >> 1) & 1);
+            const char *p = lds + (r0 + r) * ROWB + ((c ^ twist(r0 + r)) << 4) + (l & 1) * 8;
+            return __builtin_bit_cast(typename Ty<T>::V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(p)));
+        } else {
+            typename Ty<T>::V4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = r0 + g * 4 + i;
+                v[i] = *reinterpret_cast<const float *>(lds + r * ROWB + ((((c0 + l) >> 2) ^ twist(r)) << 4) + (l & 3) * 4);
+            }
+            return v;
+        }
+    }
+    static __device__ __forceinline__ typename Ty<T>::V8 col8(const char *lds, int r0, int c0, int g, int l)      // rows r0 + 4 g + 0..3 and r0 + 16 + 4 g + 0..3
+    {
+        return __builtin_shufflevector(col4(lds, r0, c0, g, l), col4(lds, r0 + 16, c0, g, l), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+// every load of this wave has landed in LDS and every read has returned; then the same for the workgroup
+__device__ __forceinline__ void tiles_ready()
 {
-    return __builtin_shufflevector(ld_col4(tile, ld, g, l), ld_col4(tile + 16 * ld, ld, g, l), 0, 1, 2, 3, 4, 5, 6, 7);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
 }
+
 template <class T> __device__ __forceinline__ typename Ty<T>::V8 pack8(f4 a, f4 b)
 {
     typename Ty<T>::V8 r;
@@ -115,29 +170,6 @@ template <class T> __device__ __forceinline__ typename Ty<T>::V8 pack8(f4 a, f4 
     }
     return r;
 }
-
-// a (ROWS x COLS) tile on its way from HBM to LDS through registers: 16 bytes a lane; rows from `rend` and columns from `cend` read as zero
-template <class T, int ROWS, int COLS, int NTH> struct Stage {
-    static constexpr int VN = 16 / sizeof(T), CV = COLS / VN, TOT = ROWS * CV, N = (TOT + NTH - 1) / NTH;
-    u4 r[N];
-    __device__ __forceinline__ void load(const T *base, long long rs, int row0, int rend, int cend)
-    {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int idx = i * NTH + (int)threadIdx.x, row = idx / CV, c = (idx - row * CV) * VN;
-            r[i] = u4{0, 0, 0, 0};
-            if (idx < TOT && row0 + row < rend && c < cend) r[i] = *reinterpret_cast<const u4 *>(base + (long long)(row0 + row) * rs + c);
-        }
-    }
-    __device__ __forceinline__ void store(T *lds, int ld) const
-    {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int idx = i * NTH + (int)threadIdx.x, row = idx / CV, c = (idx - row * CV) * VN;
-            if (idx < TOT) *reinterpret_cast<u4 *>(lds + row * ld + c) = r[i];
-        }
-    }
-};
 
 // the learned table over distances -D .. D of head h, into LDS; softmax works in powers of two, so its bias carries log2 e (finite values stay finite)
 template <class T, int KIND> __device__ __forceinline__ void expand_bias(const Args &p, int h, float *dst, int nth)
@@ -204,13 +236,15 @@ __device__ __forceinline__ float bias_at(const float *tab, int D, int j, int pos
 // WM x WN waves; a wave owns MT x 16 rows and NT x 16 columns of the output.  Rows of a block are (head of the group, query) pairs when p.fold
 // (few queries: the heads that share keys and values are answered in one pass over them).
 template <class T, int KIND, int DK, int MT, int NT, int WM, int WN, int KT>
-__global__ void __launch_bounds__(64 * WM * WN) fwd_kernel(const Args p)
+__global__ void __launch_bounds__(64 * WM * WN, 2) fwd_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
-    constexpr int NTH = 64 * WM * WN, BM = WM * MT * 16, DVB = WN * NT * 16, PAD = 16 / sizeof(T), LDK = DK + PAD, LDV = DVB + 2 * PAD, NS = KT / 16;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    T *Ks = reinterpret_cast<T *>(smem), *Vs = Ks + KT * LDK;
-    float *tab = reinterpret_cast<float *>(Vs + KT * LDV);
+    constexpr int NTH = 64 * WM * WN, BM = WM * MT * 16, DVB = WN * NT * 16, NS = KT / 16;
+    using TK = Tile<T, KT, DK, WM * WN>;
+    using TV = Tile<T, KT, DVB, WM * WN>;
+    constexpr int BUF = TK::BYTES + TV::BYTES;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    float *tab = reinterpret_cast<float *>(smem + (p.Lk > KT ? 2 : 1) * BUF);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / WN, wn = w - wm * WN, g = lane >> 4, l = lane & 15;
     const int G = p.H / p.Hk, GB = p.fold ? G : 1, HB = p.H / GB, rows = p.Lq * GB, TW = 2 * p.D + 1;
     int id = blockIdx.x;
@@ -221,12 +255,27 @@ __global__ void __launch_bounds__(64 * WM * WN) fwd_kernel(const Args p)
     const int hk = p.fold ? hb : hb / G, h0 = p.fold ? hb * G : hb;
     const int kend_all = key_end(p, b), q0 = row_start(p, b);
     const int c0 = ch * DVB, cend = p.dv - c0;
-    if (p.table)
-        for (int i = 0; i < GB; ++i) expand_bias<T, KIND>(p, h0 + i, tab + i * TW, NTH);
-
     const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0];
     const T *K = reinterpret_cast<const T *>(p.k) + b * p.ks[0] + hk * p.ks[2];
     const T *V = reinterpret_cast<const T *>(p.v) + b * p.vs[0] + hk * p.vs[2] + c0;
+    // keys of this block: its split, below the length, and not beyond its last row's position
+    int kb = sp * p.split_keys, ke = min(kend_all, p.nsplit > 1 ? kb + p.split_keys : kend_all);
+    if (p.causal) {
+        const int r0 = rt * BM, r1 = min(rows, r0 + BM) - 1;
+        const int last = (r0 / p.Lq == r1 / p.Lq) ? r1 % p.Lq : p.Lq - 1;
+        ke = min(ke, last + q0 + 1);
+    }
+    TK tk;
+    TV tv;
+    tk.init(w, lane, p.ks[1], p.dk);
+    tv.init(w, lane, p.vs[1], cend);
+    const auto issue = [&](int j, int buf) {
+        tk.issue(K + (long long)j * p.ks[1], ke - j, smem + buf * BUF, lane);
+        tv.issue(V + (long long)j * p.vs[1], ke - j, smem + buf * BUF + TK::BYTES, lane);
+    };
+    if (kb < ke) issue(kb, 0);
+    if (p.table)
+        for (int i = 0; i < GB; ++i) expand_bias<T, KIND>(p, h0 + i, tab + i * TW, NTH);
     int qi[MT], qh[MT], pos[MT];
     bool ok[MT];
     V8 qf[MT][DK / 32];
@@ -246,13 +295,6 @@ __global__ void __launch_bounds__(64 * WM * WN) fwd_kernel(const Args p)
     }
     pmin = __builtin_amdgcn_readfirstlane(wave_min_i(pmin));
     pmax = __builtin_amdgcn_readfirstlane(wave_max_i(pmax));
-    // keys of this block: its split, below the length, and not beyond its last row's position
-    int kb = sp * p.split_keys, ke = min(kend_all, p.nsplit > 1 ? kb + p.split_keys : kend_all);
-    if (p.causal) {
-        const int r0 = rt * BM, r1 = min(rows, r0 + BM) - 1;
-        const int last = (r0 / p.Lq == r1 / p.Lq) ? r1 % p.Lq : p.Lq - 1;
-        ke = min(ke, last + q0 + 1);
-    }
     f4 acc[NT][MT];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -264,16 +306,12 @@ __global__ void __launch_bounds__(64 * WM * WN) fwd_kernel(const Args p)
     for (int mt = 0; mt < MT; ++mt) { m[mt] = NEG; lsum[mt] = 0.f; ex[mt] = E_NONE; }
     const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
 
-    Stage<T, KT, DK, NTH> stk;
-    Stage<T, KT, DVB, NTH> stv;
-    if (kb < ke) { stk.load(K, p.ks[1], kb, ke, p.dk); stv.load(V, p.vs[1], kb, ke, cend); }
-    for (int j0 = kb; j0 < ke; j0 += KT) {
-        __syncthreads();
-        stk.store(Ks, LDK);
-        stv.store(Vs, LDV);
-        __syncthreads();
-        if (j0 + KT < ke) { stk.load(K, p.ks[1], j0 + KT, ke, p.dk); stv.load(V, p.vs[1], j0 + KT, ke, cend); }
+    int buf = 0;
+    for (int j0 = kb; j0 < ke; j0 += KT, buf ^= 1) {
+        tiles_ready();                                             // this tile has landed, and the other buffer is free
+        if (j0 + KT < ke) issue(j0 + KT, buf ^ 1);
         if (pmin > pmax || (p.causal && j0 > pmax)) continue;      // no row of this wave, or none that sees this tile (uniform over the wave)
+        const char *Ks = smem + buf * BUF, *Vs = Ks + TK::BYTES;
         f4 s[MT][NS];
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
@@ -281,7 +319,7 @@ __global__ void __launch_bounds__(64 * WM * WN) fwd_kernel(const Args p)
             for (int mt = 0; mt < MT; ++mt) s[mt][n] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int ks = 0; ks < DK / 32; ++ks) {
-                const V8 a = ld8(Ks + (n * 16 + l) * LDK + ks * 32 + g * 8);
+                const V8 a = TK::row8(Ks, n * 16 + l, ks * 32 + g * 8);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, qf[mt][ks], s[mt][n]);
             }
@@ -289,19 +327,32 @@ __global__ void __launch_bounds__(64 * WM * WN) fwd_kernel(const Args p)
         // scores: scale, bias, mask
         const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin);
         const int where = !p.table ? 0 : (j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3));
+        if (full && where != 3) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const float *tb = tab + qh[mt] * TW;
-            const float far = where == 1 ? tb[TW - 1] : (where == 2 ? tb[0] : 0.f);
+            for (int mt = 0; mt < MT; ++mt) {
+                const float far = where ? tab[qh[mt] * TW + (where == 1 ? TW - 1 : 0)] : 0.f;
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
+                for (int n = 0; n < NS; ++n)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = j0 + n * 16 + g * 4 + r;
-                    float x = s[mt][n][r] * sc + (where == 3 ? bias_at(tb, p.D, j, pos[mt]) : far);
-                    if (!full && (j >= ke || (p.causal && j > pos[mt]))) x = KIND == SOFTMAX ? -INFINITY : 0.f;
-                    s[mt][n][r] = KIND == SOFTMAX ? x : relu_(x);
-                }
+                    for (int r = 0; r < 4; ++r) {
+                        const float x = __builtin_fmaf(s[mt][n][r], sc, far);
+                        s[mt][n][r] = KIND == SOFTMAX ? x : relu_(x);
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float *tb = tab + qh[mt] * TW;
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = j0 + n * 16 + g * 4 + r;
+                        float x = __builtin_fmaf(s[mt][n][r], sc, where ? bias_at(tb, p.D, j, pos[mt]) : 0.f);
+                        if (j >= ke || (p.causal && j > pos[mt])) x = KIND == SOFTMAX ? -INFINITY : 0.f;
+                        s[mt][n][r] = KIND == SOFTMAX ? x : relu_(x);
+                    }
+            }
         }
         // weights
         float fac[MT];
@@ -355,7 +406,7 @@ __global__ void __launch_bounds__(64 * WM * WN) fwd_kernel(const Args p)
             for (int mt = 0; mt < MT; ++mt) pb[mt] = pack8<T>(s[mt][2 * kk], s[mt][2 * kk + 1]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const V8 a = ld_col8<T>(Vs + kk * 32 * LDV + (wn * NT + n) * 16, LDV, g, l);
+                const V8 a = TV::col8(Vs, kk * 32, (wn * NT + n) * 16, g, l);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) acc[n][mt] = Ty<T>::mma(a, pb[mt], acc[n][mt]);
             }
@@ -525,15 +576,17 @@ template <class T> __device__ __forceinline__ float unhold(int e) { return !Ty<T
 // dQ^T = K^T dS^T.  The bias gradient needs sums along diagonals: a tile that lies beyond +-D of all its queries is one sum in registers, one near
 // the diagonal goes through a wave's own (KT x BM) LDS tile and each lane sums one diagonal -- no atomics, the order is fixed.
 template <class T, int KIND, int DK, int DVC, int MT, int W>
-__global__ void __launch_bounds__(64 * W) dq_kernel(const Args p)
+__global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
-    constexpr int KT = 32, NTH = 64 * W, BM = W * MT * 16, PAD = 16 / sizeof(T), LDK = DK + PAD, LDV = DVC + PAD, NS = 2, LT = MT * 16 + 1;
+    constexpr int KT = 32, NTH = 64 * W, BM = W * MT * 16, NS = 2, LT = MT * 16 + 1;
     static_assert(KT + MT * 16 <= 64, "one diagonal of a wave's tile per lane");
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    T *Ks = reinterpret_cast<T *>(smem), *Vs = Ks + KT * LDK;
+    using TK = Tile<T, KT, DK, W>;
+    using TV = Tile<T, KT, DVC, W>;
+    constexpr int BUF = TK::BYTES + TV::BYTES;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int TW = p.table ? 2 * p.D + 1 : 0;
-    float *tab = reinterpret_cast<float *>(Vs + KT * LDV);
+    float *tab = reinterpret_cast<float *>(smem + (p.Lk > KT ? 2 : 1) * BUF);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
     float *dbw = tab + TW + w * TW, *tile = tab + TW + W * TW + w * KT * LT;         // this wave's distance sums and its dS tile
     int id = blockIdx.x;
@@ -541,13 +594,24 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args p)
     const int ch = id % p.nchunk; id /= p.nchunk;
     const int h = id % p.H, b = id / p.H, hk = h / (p.H / p.Hk);
     const int q0 = row_start(p, b), c0 = ch * DVC, cend = p.dv - c0;
+    int ke = key_end(p, b);
+    if (p.causal) ke = min(ke, min(p.Lq, rt * BM + BM) - 1 + q0 + 1);
+    const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2];
+    const T *K = reinterpret_cast<const T *>(p.k) + b * p.ks[0] + hk * p.ks[2];
+    const T *V = reinterpret_cast<const T *>(p.v) + b * p.vs[0] + hk * p.vs[2] + c0;
+    TK tk;
+    TV tv;
+    tk.init(w, lane, p.ks[1], p.dk);
+    tv.init(w, lane, p.vs[1], cend);
+    const auto issue = [&](int j, int buf) {
+        tk.issue(K + (long long)j * p.ks[1], ke - j, smem + buf * BUF, lane);
+        tv.issue(V + (long long)j * p.vs[1], ke - j, smem + buf * BUF + TK::BYTES, lane);
+    };
+    if (0 < ke) issue(0, 0);
     if (p.table) {
         expand_bias<T, KIND>(p, h, tab, NTH);
         for (int t = lane; t < TW; t += 64) dbw[t] = 0.f;
     }
-    const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2];
-    const T *K = reinterpret_cast<const T *>(p.k) + b * p.ks[0] + hk * p.ks[2];
-    const T *V = reinterpret_cast<const T *>(p.v) + b * p.vs[0] + hk * p.vs[2] + c0;
     const int i0 = rt * BM + w * MT * 16;                                             // the wave's first query
     V8 qf[MT][DK / 32], df[MT][DVC / 32];
     float lse[MT], del[MT];
@@ -565,8 +629,6 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args p)
         lse[mt] = KIND == SOFTMAX ? (ok ? p.lse[row] : INFINITY) : 0.f;
         del[mt] = KIND == SOFTMAX && ok && ch == 0 ? p.delta[row] : 0.f;              // (dW comes in chunks of dv: the subtraction belongs to one of them)
     }
-    int ke = key_end(p, b);
-    if (p.causal) ke = min(ke, min(p.Lq, rt * BM + BM) - 1 + q0 + 1);
     const int pmin = i0 + q0, pmax = min(p.Lq, i0 + MT * 16) - 1 + q0;
     f4 acc[DK / 16][MT];
 #pragma unroll
@@ -578,16 +640,12 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args p)
     for (int mt = 0; mt < MT; ++mt) ex[mt] = E_NONE;
     float lo = 0.f, hi = 0.f;
     const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
-    Stage<T, KT, DK, NTH> stk;
-    Stage<T, KT, DVC, NTH> stv;
-    if (0 < ke) { stk.load(K, p.ks[1], 0, ke, p.dk); stv.load(V, p.vs[1], 0, ke, cend); }
-    for (int j0 = 0; j0 < ke; j0 += KT) {
-        __syncthreads();
-        stk.store(Ks, LDK);
-        stv.store(Vs, LDV);
-        __syncthreads();
-        if (j0 + KT < ke) { stk.load(K, p.ks[1], j0 + KT, ke, p.dk); stv.load(V, p.vs[1], j0 + KT, ke, cend); }
+    int buf = 0;
+    for (int j0 = 0; j0 < ke; j0 += KT, buf ^= 1) {
+        tiles_ready();
+        if (j0 + KT < ke) issue(j0 + KT, buf ^ 1);
         if (i0 >= p.Lq || (p.causal && j0 > pmax)) continue;
+        const char *Ks = smem + buf * BUF, *Vs = Ks + TK::BYTES;
         f4 s[MT][NS], dp[MT][NS];
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
@@ -595,37 +653,50 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args p)
             for (int mt = 0; mt < MT; ++mt) { s[mt][n] = f4{0, 0, 0, 0}; dp[mt][n] = f4{0, 0, 0, 0}; }
 #pragma unroll
             for (int ks = 0; ks < DK / 32; ++ks) {
-                const V8 a = ld8(Ks + (n * 16 + l) * LDK + ks * 32 + g * 8);
+                const V8 a = TK::row8(Ks, n * 16 + l, ks * 32 + g * 8);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, qf[mt][ks], s[mt][n]);
             }
 #pragma unroll
             for (int ks = 0; ks < DVC / 32; ++ks) {
-                const V8 a = ld8(Vs + (n * 16 + l) * LDV + ks * 32 + g * 8);
+                const V8 a = TV::row8(Vs, n * 16 + l, ks * 32 + g * 8);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) dp[mt][n] = Ty<T>::mma(a, df[mt][ks], dp[mt][n]);
             }
         }
         const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin) && i0 + MT * 16 <= p.Lq;
         const int where = !p.table ? 0 : (j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3));
-        const float far = where == 1 ? tab[TW - 1] : (where == 2 ? tab[0] : 0.f);
         float all = 0.f;
+        if (full && where != 3) {
+            const float far = where ? tab[where == 1 ? TW - 1 : 0] : 0.f;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const int i = i0 + mt * 16 + l, pos = i + q0;
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
+                for (int n = 0; n < NS; ++n)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = j0 + n * 16 + g * 4 + r;
-                    const float x = s[mt][n][r] * sc + (where == 3 ? bias_at(tab, p.D, j, pos) : far);
-                    const bool seen = full || (i < p.Lq && j < ke && !(p.causal && j > pos));
-                    float wgt;
-                    const float d = dscore<KIND>(x, dp[mt][n][r], lse[mt], del[mt], seen, wgt);
-                    s[mt][n][r] = d;
-                    all += d;
-                    if (where == 3) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = d;
-                }
+                    for (int r = 0; r < 4; ++r) {
+                        float wgt;
+                        s[mt][n][r] = dscore<KIND>(__builtin_fmaf(s[mt][n][r], sc, far), dp[mt][n][r], lse[mt], del[mt], true, wgt);
+                        all += s[mt][n][r];
+                    }
+        } else {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const int i = i0 + mt * 16 + l, pos = i + q0;
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = j0 + n * 16 + g * 4 + r;
+                        const float x = __builtin_fmaf(s[mt][n][r], sc, where ? bias_at(tab, p.D, j, pos) : 0.f);
+                        const bool seen = i < p.Lq && j < ke && !(p.causal && j > pos);
+                        float wgt;
+                        const float d = dscore<KIND>(x, dp[mt][n][r], lse[mt], del[mt], seen, wgt);
+                        s[mt][n][r] = d;
+                        all += d;
+                        if (where == 3) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = d;
+                    }
+            }
         }
         if (where == 1) hi += all;
         if (where == 2) lo += all;
@@ -658,7 +729,7 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args p)
         for (int mt = 0; mt < MT; ++mt) pb[mt] = pack8<T>(s[mt][0], s[mt][1]);
 #pragma unroll
         for (int n = 0; n < DK / 16; ++n) {
-            const V8 a = ld_col8<T>(Ks + n * 16, LDK, g, l);
+            const V8 a = TK::col8(Ks, 0, n * 16, g, l);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) acc[n][mt] = Ty<T>::mma(a, pb[mt], acc[n][mt]);
         }
@@ -699,13 +770,15 @@ __global__ void __launch_bounds__(64 * W) dq_kernel(const Args p)
 // dK and dV: W waves, MT x 16 keys each; walks the queries of every head that shares the keys.  S has a key in the column: W and dS in registers
 // are the B operands of dV^T = dO^T W and dK^T = Q^T dS.
 template <class T, int KIND, int DK, int DVC, int MT, int W>
-__global__ void __launch_bounds__(64 * W) dkv_kernel(const Args p)
+__global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
-    constexpr int QT = 32, NTH = 64 * W, BN = W * MT * 16, PAD = 16 / sizeof(T), LDQ = DK + PAD, LDO = DVC + PAD, NS = 2;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    T *Qs = reinterpret_cast<T *>(smem), *Os = Qs + QT * LDQ;
-    float *st = reinterpret_cast<float *>(Os + QT * LDO), *tab = st + 2 * QT;           // the tile's log-sum-exp and delta
+    constexpr int QT = 32, NTH = 64 * W, BN = W * MT * 16, NS = 2;
+    using TQ = Tile<T, QT, DK, W>;
+    using TO = Tile<T, QT, DVC, W>;
+    constexpr int BUF = TQ::BYTES + TO::BYTES;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    float *stats = reinterpret_cast<float *>(smem + (p.Lq > QT ? 2 : 1) * BUF), *tab = stats + 4 * QT;      // two tiles' log-sum-exp and delta
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15, G = p.H / p.Hk, TW = 2 * p.D + 1;
     int id = blockIdx.x;
     const int rt = id % p.nrow; id /= p.nrow;
@@ -742,28 +815,40 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args p)
     int ib = 0;
     if (p.causal) ib = max(0, (rt * BN - q0) / QT * QT);
     if (rt * BN >= ke) ib = p.Lq;                                                       // keys behind the length only: zeros
-    Stage<T, QT, DK, NTH> stq;
-    Stage<T, QT, DVC, NTH> sto;
+    TQ tq;
+    TO to;
+    tq.init(w, lane, p.qs[1], p.dk);
+    to.init(w, lane, (long long)p.H * p.dv, cend);
     for (int hg = 0; hg < G; ++hg) {
         const int h = hk * G + hg;
         const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2];
         const T *dO = reinterpret_cast<const T *>(p.dO) + ((long long)b * p.Lq * p.H + h) * p.dv + c0;
-        const long long os = (long long)p.H * p.dv;
-        __syncthreads();
-        if (p.table && ib < p.Lq) expand_bias<T, KIND>(p, h, tab, NTH);
-        if (ib < p.Lq) { stq.load(Q, p.qs[1], ib, p.Lq, p.dk); sto.load(dO, os, ib, p.Lq, cend); }
-        for (int i0 = ib; i0 < p.Lq; i0 += QT) {
-            __syncthreads();
-            stq.store(Qs, LDQ);
-            sto.store(Os, LDO);
+        float ls0 = INFINITY, dl0 = 0.f;
+        const auto issue = [&](int i, int buf) {
+            tq.issue(Q + (long long)i * p.qs[1], p.Lq - i, smem + buf * BUF, lane);
+            to.issue(dO + (long long)i * p.H * p.dv, p.Lq - i, smem + buf * BUF + TQ::BYTES, lane);
             if (KIND == SOFTMAX && tid < QT) {
-                const int i = i0 + tid;
-                const long long row = ((long long)b * p.Lq + i) * p.H + h;
-                st[tid] = i < p.Lq ? p.lse[row] : INFINITY;
-                st[QT + tid] = i < p.Lq && ch == 0 ? p.delta[row] : 0.f;
+                const long long row = ((long long)b * p.Lq + i + tid) * p.H + h;
+                ls0 = i + tid < p.Lq ? p.lse[row] : INFINITY;
+                dl0 = i + tid < p.Lq && ch == 0 ? p.delta[row] : 0.f;
             }
-            __syncthreads();
-            if (i0 + QT < p.Lq) { stq.load(Q, p.qs[1], i0 + QT, p.Lq, p.dk); sto.load(dO, os, i0 + QT, p.Lq, cend); }
+        };
+        const auto keep = [&](int buf) {
+            if (KIND == SOFTMAX && tid < QT) { stats[buf * 2 * QT + tid] = ls0; stats[buf * 2 * QT + QT + tid] = dl0; }
+        };
+        __syncthreads();                                                                  // the previous head's tiles and table are no longer read
+        if (ib < p.Lq) {
+            issue(ib, 0);
+            if (p.table) expand_bias<T, KIND>(p, h, tab, NTH);
+            keep(0);
+        }
+        int buf = 0;
+        for (int i0 = ib; i0 < p.Lq; i0 += QT, buf ^= 1) {
+            if (i0 > ib) keep(buf);
+            tiles_ready();
+            if (i0 + QT < p.Lq) issue(i0 + QT, buf ^ 1);
+            const char *Qs = smem + buf * BUF, *Os = Qs + TQ::BYTES;
+            const float *st = stats + buf * 2 * QT;
             const int pmin = i0 + q0, pmax = min(p.Lq, i0 + QT) - 1 + q0;
             if (jmax < jmin || (p.causal && jmin > pmax)) continue;
             f4 s[MT][NS], dp[MT][NS];
@@ -773,13 +858,13 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args p)
                 for (int mt = 0; mt < MT; ++mt) { s[mt][n] = f4{0, 0, 0, 0}; dp[mt][n] = f4{0, 0, 0, 0}; }
 #pragma unroll
                 for (int ks = 0; ks < DK / 32; ++ks) {
-                    const V8 a = ld8(Qs + (n * 16 + l) * LDQ + ks * 32 + g * 8);
+                    const V8 a = TQ::row8(Qs, n * 16 + l, ks * 32 + g * 8);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, kf[mt][ks], s[mt][n]);
                 }
 #pragma unroll
                 for (int ks = 0; ks < DVC / 32; ++ks) {
-                    const V8 a = ld8(Os + (n * 16 + l) * LDO + ks * 32 + g * 8);
+                    const V8 a = TO::row8(Os, n * 16 + l, ks * 32 + g * 8);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) dp[mt][n] = Ty<T>::mma(a, vf[mt][ks], dp[mt][n]);
                 }
@@ -787,6 +872,7 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args p)
             const bool full = i0 + QT <= p.Lq && j0 + MT * 16 <= ke && (!p.causal || j0 + MT * 16 - 1 <= pmin);
             const int where = !p.table ? 0 : (jmin - pmax >= p.D ? 1 : (jmax - pmin <= -p.D ? 2 : 3));
             const float far = where == 1 ? tab[TW - 1] : (where == 2 ? tab[0] : 0.f);
+            const bool fast = full && where != 3;
             V8 wb[MT], db[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -799,14 +885,23 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args p)
                         ls = *reinterpret_cast<const f4 *>(st + n * 16 + g * 4);
                         dl = *reinterpret_cast<const f4 *>(st + QT + n * 16 + g * 4);
                     }
+                    if (fast) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = i0 + n * 16 + g * 4 + r, pos = i + q0;
-                        const float x = s[mt][n][r] * sc + (where == 3 ? bias_at(tab, p.D, j, pos) : far);
-                        const bool seen = full || (i < p.Lq && j < ke && !(p.causal && j > pos));
-                        float wgt;
-                        s[mt][n][r] = dscore<KIND>(x, dp[mt][n][r], ls[r], dl[r], seen, wgt);
-                        wt[n][r] = wgt;
+                        for (int r = 0; r < 4; ++r) {
+                            float wgt;
+                            s[mt][n][r] = dscore<KIND>(__builtin_fmaf(s[mt][n][r], sc, far), dp[mt][n][r], ls[r], dl[r], true, wgt);
+                            wt[n][r] = wgt;
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int i = i0 + n * 16 + g * 4 + r, pos = i + q0;
+                            const float x = __builtin_fmaf(s[mt][n][r], sc, where ? bias_at(tab, p.D, j, pos) : 0.f);
+                            const bool seen = i < p.Lq && j < ke && !(p.causal && j > pos);
+                            float wgt;
+                            s[mt][n][r] = dscore<KIND>(x, dp[mt][n][r], ls[r], dl[r], seen, wgt);
+                            wt[n][r] = wgt;
+                        }
                     }
                 }
                 const float fv = hold<T, NS>(wt, ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
@@ -821,13 +916,13 @@ __global__ void __launch_bounds__(64 * W) dkv_kernel(const Args p)
             }
 #pragma unroll
             for (int n = 0; n < DVC / 16; ++n) {
-                const V8 a = ld_col8<T>(Os + n * 16, LDO, g, l);
+                const V8 a = TO::col8(Os, 0, n * 16, g, l);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) av[n][mt] = Ty<T>::mma(a, wb[mt], av[n][mt]);
             }
 #pragma unroll
             for (int n = 0; n < DK / 16; ++n) {
-                const V8 a = ld_col8<T>(Qs + n * 16, LDQ, g, l);
+                const V8 a = TQ::col8(Qs, 0, n * 16, g, l);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) ak[n][mt] = Ty<T>::mma(a, db[mt], ak[n][mt]);
             }

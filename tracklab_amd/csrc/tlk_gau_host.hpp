@@ -13,7 +13,7 @@ struct FwdPlan {
     bool few;                // one tile of rows, waves side by side along dv; else waves below each other
     int fold, mt, dvb, bm, nrow, nchunk, nsplit, split_keys, heads;
 };
-inline FwdPlan plan_forward(const Args &a)
+inline FwdPlan plan_forward(const Args &a, int elem)
 {
     FwdPlan f;
     const int G = a.H / a.Hk;
@@ -22,7 +22,7 @@ inline FwdPlan plan_forward(const Args &a)
     f.few = rows <= 32;
     f.mt = f.few && rows <= 16 ? 1 : 2;
     f.bm = f.few ? f.mt * 16 : 128;
-    f.dvb = a.dv <= 64 ? 64 : (a.dv <= 128 ? 128 : (a.dv <= 256 || !f.few ? 256 : 512));
+    f.dvb = a.dv <= 64 ? 64 : (a.dv <= 128 ? 128 : (a.dv <= 256 || !f.few || elem == 4 ? 256 : 512));
     f.nrow = (int)((rows + f.bm - 1) / f.bm);
     f.nchunk = div_up(a.dv, f.dvb);
     f.heads = f.fold ? a.Hk : a.H;
@@ -123,8 +123,8 @@ template <class K> int launch(K kernel, long long blocks, int threads, size_t sm
 
 template <class T, int KIND, int DK, int MT, int NT, int WM, int WN> int launch_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
 {
-    constexpr int KT = 32, PAD = 16 / sizeof(T);
-    const size_t smem = sizeof(T) * KT * ((DK + PAD) + (WN * NT * 16 + 2 * PAD)) + (a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * (2 * a.D + 1) : 0);
+    constexpr int KT = 32;
+    const size_t smem = sizeof(T) * KT * (DK + WN * NT * 16) * (a.Lk > KT ? 2 : 1) + (a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * (2 * a.D + 1) : 0);
     return launch(fwd_kernel<T, KIND, DK, MT, NT, WM, WN, KT>, (long long)a.B * f.heads * f.nsplit * f.nchunk * f.nrow, 64 * WM * WN, smem, a, st);
 }
 template <class T, int KIND, int DK> int pick_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
@@ -137,17 +137,19 @@ template <class T, int KIND, int DK> int pick_fwd(const Args &a, const FwdPlan &
     if (f.mt == 1) {
         if (f.dvb == 64) return launch_fwd<T, KIND, DK, 1, 1, 1, 4>(a, f, st);
         if (f.dvb == 128) return launch_fwd<T, KIND, DK, 1, 2, 1, 4>(a, f, st);
-        if (f.dvb == 256) return launch_fwd<T, KIND, DK, 1, 4, 1, 4>(a, f, st);
-        return launch_fwd<T, KIND, DK, 1, 8, 1, 4>(a, f, st);
+        if constexpr (sizeof(T) == 2)
+            if (f.dvb == 512) return launch_fwd<T, KIND, DK, 1, 8, 1, 4>(a, f, st);
+        return launch_fwd<T, KIND, DK, 1, 4, 1, 4>(a, f, st);
     }
     if (f.dvb == 64) return launch_fwd<T, KIND, DK, 2, 1, 1, 4>(a, f, st);
     if (f.dvb == 128) return launch_fwd<T, KIND, DK, 2, 2, 1, 4>(a, f, st);
-    if (f.dvb == 256) return launch_fwd<T, KIND, DK, 2, 4, 1, 4>(a, f, st);
-    return launch_fwd<T, KIND, DK, 2, 8, 1, 4>(a, f, st);
+    if constexpr (sizeof(T) == 2)
+        if (f.dvb == 512) return launch_fwd<T, KIND, DK, 2, 8, 1, 4>(a, f, st);
+    return launch_fwd<T, KIND, DK, 2, 4, 1, 4>(a, f, st);
 }
 template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
 {
-    const FwdPlan f = plan_forward(a);
+    const FwdPlan f = plan_forward(a, sizeof(T));
     a.fold = f.fold; a.nrow = f.nrow; a.nchunk = f.nchunk; a.nsplit = f.nsplit; a.split_keys = f.split_keys;
     const long long rows = (long long)a.B * a.Lq * a.H;
     a.part = reinterpret_cast<float *>(ws);
@@ -162,14 +164,12 @@ template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
 
 template <class T, int KIND, int DK, int DVC, int W> int launch_dq(const Args &a, const BwdPlan &f, hipStream_t st)
 {
-    constexpr int PAD = 16 / sizeof(T);
-    const size_t smem = sizeof(T) * 32 * ((DK + PAD) + (DVC + PAD)) + (a.table ? sizeof(float) * ((1 + W) * (2 * a.D + 1) + W * 32 * 33) : 0);
+    const size_t smem = sizeof(T) * 32 * (DK + DVC) * (a.Lk > 32 ? 2 : 1) + (a.table ? sizeof(float) * ((1 + W) * (2 * a.D + 1) + W * 32 * 33) : 0);
     return launch(dq_kernel<T, KIND, DK, DVC, 2, W>, (long long)a.B * a.H * f.nchunk * f.nrow_q, 64 * W, smem, a, st);
 }
 template <class T, int KIND, int DK, int DVC, int W> int launch_dkv(const Args &a, const BwdPlan &f, hipStream_t st)
 {
-    constexpr int PAD = 16 / sizeof(T);
-    const size_t smem = sizeof(T) * 32 * ((DK + PAD) + (DVC + PAD)) + 64 * sizeof(float) + (a.table ? sizeof(float) * (2 * a.D + 1) : 0);
+    const size_t smem = sizeof(T) * 32 * (DK + DVC) * (a.Lq > 32 ? 2 : 1) + 128 * sizeof(float) + (a.table ? sizeof(float) * (2 * a.D + 1) : 0);
     return launch(dkv_kernel<T, KIND, DK, DVC, sizeof(T) == 4 ? 1 : 2, W>, (long long)a.B * a.Hk * f.nchunk * f.nrow_k, 64 * W, smem, a, st);
 }
 template <class T, int KIND, int DK, int DVC> int pick_bwd(Args a, const BwdPlan &f, hipStream_t st)
