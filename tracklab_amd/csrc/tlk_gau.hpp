@@ -42,12 +42,12 @@ struct Args {
     void *out, *o;
     float *lse;                                 // (B, Lq, H): log2 of the row's sum of 2^(S log2 e), +inf for a row without keys
     float *part, *ml;                           // split keys: (split, B, Lq, H, dv) sums and (split, B, Lq, H, 2) maximum and sum
-    int nsplit, split_keys, nchunk, nrow, fold;
+    int nsplit, split_keys, nchunk, nrow, fold, nparts;
     // backward
     const void *dO;                             // (B, Lq, H, dv) contiguous: the gradient behind the gate
     const float *delta;                         // (B, Lq, H): sum_d dO o (softmax)
     void *dq, *dk_, *dv_;
-    float *dq_part, *dk_part;                   // (chunk, B, L, heads, dk) when dv is walked in several chunks
+    float *dq_part, *dk_part, *dv_part;         // (chunk, B, Lq, H, dk); (chunk x part, B, Lk, Hk, dk), (part, B, Lk, Hk, dv): sums of several blocks, joined afterwards
     float *db_part;                             // (heads, B * chunk * nrow * waves, 2 D + 1)
 };
 
@@ -171,11 +171,16 @@ template <class T> __device__ __forceinline__ typename Ty<T>::V8 pack8(f4 a, f4 
     return r;
 }
 
-// the learned table over distances -D .. D of head h, into LDS; softmax works in powers of two, so its bias carries log2 e (finite values stay finite)
+// The learned table over distances of head h, in LDS: -D .. D with MARGIN more entries of the end values on both sides, so that a tile that reaches
+// across +-D is looked up without clipping (a wave's tile spans fewer than MARGIN distances).  Softmax works in powers of two, so its bias carries
+// log2 e (finite values stay finite).
+constexpr int MARGIN = 128;
+__host__ __device__ __forceinline__ int table_width(int D) { return 2 * D + 1 + 2 * MARGIN; }
 template <class T, int KIND> __device__ __forceinline__ void expand_bias(const Args &p, int h, float *dst, int nth)
 {
-    for (int t = threadIdx.x; t < 2 * p.D + 1; t += nth) {
-        int b = p.bucket_of[t];
+    const int TW = table_width(p.D);
+    for (int t = threadIdx.x; t < TW; t += nth) {
+        int b = p.bucket_of[min(max(t - MARGIN, 0), 2 * p.D)];
         b = b < 0 ? 0 : (b >= p.nb ? p.nb - 1 : b);
         const long long at = (long long)b * p.H + h;
         float x = p.table_f32 ? reinterpret_cast<const float *>(p.table)[at] : (float)reinterpret_cast<const T *>(p.table)[at];
@@ -224,19 +229,30 @@ __device__ __forceinline__ float raise_exponent(int &e, float t)
 }
 constexpr int E_NONE = -120;                      // exponent before the first non-zero value
 
-// bias of key j at query position pos: LDS gather near the diagonal, the two end values beyond it
-__device__ __forceinline__ float bias_at(const float *tab, int D, int j, int pos)
+// scores of a wave's column tile: scale and bias.  `near`: the table at this lane's first distance, STEP entries further with every row of the tile; where
+// the whole tile lies beyond +-D (or there is no bias) one value does for all (uniform over the wave).
+template <int STEP, int NS> __device__ __forceinline__ void add_bias(f4 (&s)[NS], float sc, bool is_near, const float *near, float far)
 {
-    int d = j - pos;
-    d = d < -D ? -D : (d > D ? D : d);
-    return tab[d + D];
+    if (is_near) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[n][r] = __builtin_fmaf(s[n][r], sc, near[STEP * (n * 16 + r)]);
+    } else {
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[n][r] = __builtin_fmaf(s[n][r], sc, far);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------ forward
 // WM x WN waves; a wave owns MT x 16 rows and NT x 16 columns of the output.  Rows of a block are (head of the group, query) pairs when p.fold
 // (few queries: the heads that share keys and values are answered in one pass over them).
+// Block order, here and in the backward kernels: sequences, key heads and chunks of dv vary fastest, so that the blocks that walk the same keys land on
+// one XCD (workgroups go to the 8 XCDs in turn) and share its L2; row tiles vary slowest, the longest causal walks first.
 template <class T, int KIND, int DK, int MT, int NT, int WM, int WN, int KT>
-__global__ void __launch_bounds__(64 * WM * WN, 2) fwd_kernel(const Args p)
+__global__ void __launch_bounds__(64 * WM * WN, WN > 1 && MT * NT <= 8 ? 4 : 2) fwd_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
     constexpr int NTH = 64 * WM * WN, BM = WM * MT * 16, DVB = WN * NT * 16, NS = KT / 16;
@@ -246,13 +262,13 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) fwd_kernel(const Args p)
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     float *tab = reinterpret_cast<float *>(smem + (p.Lk > KT ? 2 : 1) * BUF);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / WN, wn = w - wm * WN, g = lane >> 4, l = lane & 15;
-    const int G = p.H / p.Hk, GB = p.fold ? G : 1, HB = p.H / GB, rows = p.Lq * GB, TW = 2 * p.D + 1;
+    const int G = p.H / p.Hk, GB = p.fold ? G : 1, HB = p.H / GB, rows = p.Lq * GB, TW = table_width(p.D);
     int id = blockIdx.x;
-    const int rt = id % p.nrow; id /= p.nrow;
+    const int b = id % p.B; id /= p.B;
+    const int hk = id % p.Hk; id /= p.Hk;
     const int ch = id % p.nchunk; id /= p.nchunk;
     const int sp = id % p.nsplit; id /= p.nsplit;
-    const int hb = id % HB, b = id / HB;
-    const int hk = p.fold ? hb : hb / G, h0 = p.fold ? hb * G : hb;
+    const int hg = id % (HB / p.Hk), rt = p.nrow - 1 - id / (HB / p.Hk), h0 = hk * G + hg;
     const int kend_all = key_end(p, b), q0 = row_start(p, b);
     const int c0 = ch * DVB, cend = p.dv - c0;
     const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0];
@@ -293,8 +309,23 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) fwd_kernel(const Args p)
 #pragma unroll
         for (int ks = 0; ks < DK / 32; ++ks) qf[mt][ks] = (ok[mt] && ks * 32 + g * 8 < p.dk) ? ld8(src + ks * 32) : zero8<T>();
     }
+    // few rows: the gate is fetched along with everything else (a block has one or two tiles to walk; behind them its latency would show)
+    constexpr bool EARLY = WN > 1;
+    typename Ty<T>::V4 early[EARLY ? NT : 1][MT];
+    if (EARLY && p.gate && p.nsplit == 1) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const T *gp = reinterpret_cast<const T *>(p.gate) + b * p.gs[0] + (long long)qi[mt] * p.gs[1] + (h0 + qh[mt]) * p.gs[2] + c0 + wn * NT * 16 + g * 4;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                if (ok[mt] && wn * NT * 16 + n * 16 + g * 4 < cend) early[n][mt] = *reinterpret_cast<const typename Ty<T>::V4 *>(gp + n * 16);
+        }
+    }
     pmin = __builtin_amdgcn_readfirstlane(wave_min_i(pmin));
     pmax = __builtin_amdgcn_readfirstlane(wave_max_i(pmax));
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+        if (!ok[mt]) pos[mt] = pmax;                               // (lanes without a row stay within the wave's distances)
     f4 acc[NT][MT];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -327,32 +358,23 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) fwd_kernel(const Args p)
         // scores: scale, bias, mask
         const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin);
         const int where = !p.table ? 0 : (j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3));
-        if (full && where != 3) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const float far = where ? tab[qh[mt] * TW + (where == 1 ? TW - 1 : 0)] : 0.f;
-#pragma unroll
-                for (int n = 0; n < NS; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float x = __builtin_fmaf(s[mt][n][r], sc, far);
-                        s[mt][n][r] = KIND == SOFTMAX ? x : relu_(x);
-                    }
-            }
-        } else {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const float *tb = tab + qh[mt] * TW;
+        for (int mt = 0; mt < MT; ++mt) {
+            const float *tb = tab + qh[mt] * TW;
+            add_bias<1>(s[mt], sc, where == 3, tb + (p.D + MARGIN + j0 + g * 4 - pos[mt]), where ? tb[where == 1 ? TW - 1 : 0] : 0.f);
+            if (!full) {
+                const int last = p.causal ? min(ke - 1, pos[mt]) : ke - 1;
 #pragma unroll
                 for (int n = 0; n < NS; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = j0 + n * 16 + g * 4 + r;
-                        float x = __builtin_fmaf(s[mt][n][r], sc, where ? bias_at(tb, p.D, j, pos[mt]) : 0.f);
-                        if (j >= ke || (p.causal && j > pos[mt])) x = KIND == SOFTMAX ? -INFINITY : 0.f;
-                        s[mt][n][r] = KIND == SOFTMAX ? x : relu_(x);
-                    }
+                    for (int r = 0; r < 4; ++r)
+                        if (j0 + n * 16 + g * 4 + r > last) s[mt][n][r] = KIND == SOFTMAX ? -INFINITY : 0.f;
             }
+            if (KIND == RELU2)
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[mt][n][r] = relu_(s[mt][n][r]);
         }
         // weights
         float fac[MT];
@@ -449,7 +471,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) fwd_kernel(const Args p)
                 *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.o) + row * p.dv + c) = y;
             }
             if (gp) {
-                const typename Ty<T>::V4 u = *reinterpret_cast<const typename Ty<T>::V4 *>(gp + c);
+                typename Ty<T>::V4 u;
+                if constexpr (EARLY) u = early[n][mt];
+                else u = *reinterpret_cast<const typename Ty<T>::V4 *>(gp + c);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[r] *= (float)u[r];
             }
@@ -542,16 +566,16 @@ template <class T> __global__ void __launch_bounds__(256) gate_bwd_kernel(const 
     if (p.delta && lane == 0) p.delta[row] = d;
 }
 
-// dS of one pair from its score x (scaled, biased; softmax: in powers of two), dW and the row's statistics; w returns the weight
-template <int KIND> __device__ __forceinline__ float dscore(float x, float dw, float lse, float delta, bool seen, float &w)
+// dS of one pair from its score x (scaled, biased, masked: -inf; softmax in powers of two), dW and the row's statistics; w returns the weight
+template <int KIND> __device__ __forceinline__ float dscore(float x, float dw, float lse, float delta, float &w)
 {
     if (KIND == SOFTMAX) {
-        w = seen ? exp2f(x - lse) : 0.f;
-        return seen ? w * (dw - delta) : 0.f;
+        w = exp2f(x - lse);
+        return w * (dw - delta);
     }
-    const float s = seen ? relu_(x) : 0.f;
+    const float s = relu_(x);
     w = s * s;
-    return seen ? 2.f * s * dw : 0.f;
+    return 2.f * s * dw;
 }
 
 // a wave's column tile as float16 operands: divides by the running power of two (see raise_exponent), returns what rescales the sums so far
@@ -585,14 +609,15 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
     using TV = Tile<T, KT, DVC, W>;
     constexpr int BUF = TK::BYTES + TV::BYTES;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    const int TW = p.table ? 2 * p.D + 1 : 0;
+    const int TW = p.table ? table_width(p.D) : 0, NB = p.table ? 2 * p.D + 1 : 0;
     float *tab = reinterpret_cast<float *>(smem + (p.Lk > KT ? 2 : 1) * BUF);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
-    float *dbw = tab + TW + w * TW, *tile = tab + TW + W * TW + w * KT * LT;         // this wave's distance sums and its dS tile
+    float *dbw = tab + TW + w * NB, *tile = tab + TW + W * NB + w * KT * LT;         // this wave's distance sums and its dS tile
     int id = blockIdx.x;
-    const int rt = id % p.nrow; id /= p.nrow;
+    const int b = id % p.B; id /= p.B;
+    const int hk = id % p.Hk; id /= p.Hk;
     const int ch = id % p.nchunk; id /= p.nchunk;
-    const int h = id % p.H, b = id / p.H, hk = h / (p.H / p.Hk);
+    const int G = p.H / p.Hk, h = hk * G + id % G, rt = p.nrow - 1 - id / G;
     const int q0 = row_start(p, b), c0 = ch * DVC, cend = p.dv - c0;
     int ke = key_end(p, b);
     if (p.causal) ke = min(ke, min(p.Lq, rt * BM + BM) - 1 + q0 + 1);
@@ -610,7 +635,7 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
     if (0 < ke) issue(0, 0);
     if (p.table) {
         expand_bias<T, KIND>(p, h, tab, NTH);
-        for (int t = lane; t < TW; t += 64) dbw[t] = 0.f;
+        for (int t = lane; t < NB; t += 64) dbw[t] = 0.f;
     }
     const int i0 = rt * BM + w * MT * 16;                                             // the wave's first query
     V8 qf[MT][DK / 32], df[MT][DVC / 32];
@@ -666,37 +691,33 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         }
         const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin) && i0 + MT * 16 <= p.Lq;
         const int where = !p.table ? 0 : (j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3));
+        const float far = where ? tab[where == 1 ? TW - 1 : 0] : 0.f;
         float all = 0.f;
-        if (full && where != 3) {
-            const float far = where ? tab[where == 1 ? TW - 1 : 0] : 0.f;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int n = 0; n < NS; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float wgt;
-                        s[mt][n][r] = dscore<KIND>(__builtin_fmaf(s[mt][n][r], sc, far), dp[mt][n][r], lse[mt], del[mt], true, wgt);
-                        all += s[mt][n][r];
-                    }
-        } else {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const int i = i0 + mt * 16 + l, pos = i + q0;
+        for (int mt = 0; mt < MT; ++mt) {
+            const int i = i0 + mt * 16 + l;
+            add_bias<1>(s[mt], sc, where == 3, tab + (p.D + MARGIN + j0 + g * 4 - i - q0), far);
+            if (!full) {
+                const int last = i >= p.Lq ? -1 : (p.causal ? min(ke - 1, i + q0) : ke - 1);
 #pragma unroll
                 for (int n = 0; n < NS; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = j0 + n * 16 + g * 4 + r;
-                        const float x = __builtin_fmaf(s[mt][n][r], sc, where ? bias_at(tab, p.D, j, pos) : 0.f);
-                        const bool seen = i < p.Lq && j < ke && !(p.causal && j > pos);
-                        float wgt;
-                        const float d = dscore<KIND>(x, dp[mt][n][r], lse[mt], del[mt], seen, wgt);
-                        s[mt][n][r] = d;
-                        all += d;
-                        if (where == 3) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = d;
-                    }
+                    for (int r = 0; r < 4; ++r)
+                        if (j0 + n * 16 + g * 4 + r > last) s[mt][n][r] = -INFINITY;
             }
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float wgt;
+                    s[mt][n][r] = dscore<KIND>(s[mt][n][r], dp[mt][n][r], lse[mt], del[mt], wgt);
+                    all += s[mt][n][r];
+                }
+            if (where == 3)
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = s[mt][n][r];
         }
         if (where == 1) hi += all;
         if (where == 2) lo += all;
@@ -741,8 +762,8 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         const long long nr = (long long)p.B * p.nchunk * p.nrow * W, at = (((long long)b * p.nchunk + ch) * p.nrow + rt) * W + w;
-        float *dst = p.db_part + ((long long)h * nr + at) * TW;
-        for (int t = lane; t < TW; t += 64) dst[t] = t == 0 ? lo + (p.D == 0 ? hi : 0.f) : (t == TW - 1 ? hi : dbw[t]);
+        float *dst = p.db_part + ((long long)h * nr + at) * NB;
+        for (int t = lane; t < NB; t += 64) dst[t] = t == 0 ? lo + (p.D == 0 ? hi : 0.f) : (t == NB - 1 ? hi : dbw[t]);
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -779,11 +800,12 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(con
     constexpr int BUF = TQ::BYTES + TO::BYTES;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     float *stats = reinterpret_cast<float *>(smem + (p.Lq > QT ? 2 : 1) * BUF), *tab = stats + 4 * QT;      // two tiles' log-sum-exp and delta
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15, G = p.H / p.Hk, TW = 2 * p.D + 1;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15, G = p.H / p.Hk, TW = table_width(p.D);
     int id = blockIdx.x;
-    const int rt = id % p.nrow; id /= p.nrow;
+    const int b = id % p.B; id /= p.B;
+    const int hk = id % p.Hk; id /= p.Hk;
     const int ch = id % p.nchunk; id /= p.nchunk;
-    const int hk = id % p.Hk, b = id / p.Hk;
+    const int part = id % p.nparts, rt = id / p.nparts;
     const int q0 = row_start(p, b), ke = key_end(p, b), c0 = ch * DVC, cend = p.dv - c0;
     const int j0 = rt * BN + w * MT * 16;                                               // the wave's first key
     V8 kf[MT][DK / 32], vf[MT][DVC / 32];
@@ -819,7 +841,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(con
     TO to;
     tq.init(w, lane, p.qs[1], p.dk);
     to.init(w, lane, (long long)p.H * p.dv, cend);
-    for (int hg = 0; hg < G; ++hg) {
+    for (int hg = part * G / p.nparts; hg < (part + 1) * G / p.nparts; ++hg) {             // (a part of the heads that share the keys)
         const int h = hk * G + hg;
         const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2];
         const T *dO = reinterpret_cast<const T *>(p.dO) + ((long long)b * p.Lq * p.H + h) * p.dv + c0;
@@ -871,13 +893,21 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(con
             }
             const bool full = i0 + QT <= p.Lq && j0 + MT * 16 <= ke && (!p.causal || j0 + MT * 16 - 1 <= pmin);
             const int where = !p.table ? 0 : (jmin - pmax >= p.D ? 1 : (jmax - pmin <= -p.D ? 2 : 3));
-            const float far = where == 1 ? tab[TW - 1] : (where == 2 ? tab[0] : 0.f);
-            const bool fast = full && where != 3;
+            const float far = where ? tab[where == 1 ? TW - 1 : 0] : 0.f;
             V8 wb[MT], db[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 const int j = j0 + mt * 16 + l;
                 f4 wt[NS];
+                add_bias<-1>(s[mt], sc, where == 3, tab + (p.D + MARGIN + j - (i0 + g * 4 + q0)), far);
+                if (!full) {
+                    const int first = j >= ke ? p.Lq : (p.causal ? j - q0 : 0);             // the first query that sees this lane's key
+#pragma unroll
+                    for (int n = 0; n < NS; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (i0 + n * 16 + g * 4 + r < first || i0 + n * 16 + g * 4 + r >= p.Lq) s[mt][n][r] = -INFINITY;
+                }
 #pragma unroll
                 for (int n = 0; n < NS; ++n) {
                     f4 ls = {0, 0, 0, 0}, dl = {0, 0, 0, 0};
@@ -885,23 +915,11 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(con
                         ls = *reinterpret_cast<const f4 *>(st + n * 16 + g * 4);
                         dl = *reinterpret_cast<const f4 *>(st + QT + n * 16 + g * 4);
                     }
-                    if (fast) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float wgt;
-                            s[mt][n][r] = dscore<KIND>(__builtin_fmaf(s[mt][n][r], sc, far), dp[mt][n][r], ls[r], dl[r], true, wgt);
-                            wt[n][r] = wgt;
-                        }
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int i = i0 + n * 16 + g * 4 + r, pos = i + q0;
-                            const float x = __builtin_fmaf(s[mt][n][r], sc, where ? bias_at(tab, p.D, j, pos) : 0.f);
-                            const bool seen = i < p.Lq && j < ke && !(p.causal && j > pos);
-                            float wgt;
-                            s[mt][n][r] = dscore<KIND>(x, dp[mt][n][r], ls[r], dl[r], seen, wgt);
-                            wt[n][r] = wgt;
-                        }
+                    for (int r = 0; r < 4; ++r) {
+                        float wgt;
+                        s[mt][n][r] = dscore<KIND>(s[mt][n][r], dp[mt][n][r], ls[r], dl[r], wgt);
+                        wt[n][r] = wgt;
                     }
                 }
                 const float fv = hold<T, NS>(wt, ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
@@ -939,6 +957,10 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(con
         for (int n = 0; n < DVC / 16; ++n) {
             const int c = n * 16 + g * 4;
             if (c >= cend) continue;
+            if (p.nparts > 1) {
+                *reinterpret_cast<f4 *>(p.dv_part + ((long long)part * p.B * p.Lk * p.Hk + row) * p.dv + c0 + c) = av[n][mt] * finv;
+                continue;
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[r] = (T)(av[n][mt][r] * finv);
             *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.dv_) + row * p.dv + c0 + c) = y;
@@ -948,8 +970,8 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(con
             const int c = n * 16 + g * 4;
             if (c >= p.dk) continue;
             const f4 x = ak[n][mt] * fink;
-            if (p.nchunk > 1) {
-                *reinterpret_cast<f4 *>(p.dk_part + ((long long)ch * p.B * p.Lk * p.Hk + row) * p.dk + c) = x;
+            if (p.nchunk * p.nparts > 1) {
+                *reinterpret_cast<f4 *>(p.dk_part + ((long long)(ch * p.nparts + part) * p.B * p.Lk * p.Hk + row) * p.dk + c) = x;
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
@@ -959,13 +981,13 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(con
     }
 }
 
-// y = sum over chunks of the float32 partial sums, rounded once
-template <class T> __global__ void __launch_bounds__(256) sum_chunks_kernel(const float *part, T *y, long long n, int chunks)
+// y = sum over the blocks' float32 partial sums, rounded once
+template <class T> __global__ void __launch_bounds__(256) sum_parts_kernel(const float *part, T *y, long long n, int parts)
 {
     const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     f4 x = *reinterpret_cast<const f4 *>(part + i);
-    for (int c = 1; c < chunks; ++c) x += *reinterpret_cast<const f4 *>(part + c * n + i);
+    for (int c = 1; c < parts; ++c) x += *reinterpret_cast<const f4 *>(part + c * n + i);
     typename Ty<T>::V4 v;
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = (T)x[r];

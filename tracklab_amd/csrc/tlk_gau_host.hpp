@@ -17,7 +17,7 @@ inline FwdPlan plan_forward(const Args &a, int elem)
 {
     FwdPlan f;
     const int G = a.H / a.Hk;
-    f.fold = G > 1 && a.Lq <= 32 && (long long)G * (2 * a.D + 1) <= 8192;
+    f.fold = G > 1 && a.Lq <= 32 && (long long)G * table_width(a.D) <= 8192;
     const long long rows = (long long)a.Lq * (f.fold ? G : 1);
     f.few = rows <= 32;
     f.mt = f.few && rows <= 16 ? 1 : 2;
@@ -29,8 +29,8 @@ inline FwdPlan plan_forward(const Args &a, int elem)
     const long long blocks = (long long)a.B * f.heads * f.nchunk * f.nrow;
     f.nsplit = 1;
     f.split_keys = a.Lk;
-    if (f.few && a.Lk > 512 && blocks < 1024) {
-        const int want = (int)((1024 + blocks - 1) / blocks), most = div_up(a.Lk, 256);
+    if (f.few && a.Lk > 512 && blocks < 2048) {
+        const int want = (int)((2048 + blocks - 1) / blocks), most = div_up(a.Lk, 256);
         f.nsplit = want < most ? want : most;
         f.split_keys = div_up(div_up(a.Lk, f.nsplit), 64) * 64;
         f.nsplit = div_up(a.Lk, f.split_keys);
@@ -39,7 +39,7 @@ inline FwdPlan plan_forward(const Args &a, int elem)
 }
 
 struct BwdPlan {
-    int dvc, nchunk, w_q, w_k, rows_q, rows_k, nrow_q, nrow_k;
+    int dvc, nchunk, w_q, w_k, rows_q, rows_k, nrow_q, nrow_k, nparts;
     long long nr;            // distance-sum rows per head
 };
 inline BwdPlan plan_backward(const Args &a, int elem)
@@ -47,20 +47,24 @@ inline BwdPlan plan_backward(const Args &a, int elem)
     BwdPlan f;
     f.dvc = a.dv <= 64 ? 64 : (a.dv <= 128 ? 128 : 256);
     f.nchunk = div_up(a.dv, f.dvc);
-    const int kq = 32, kk = elem == 4 ? 16 : 32;                    // rows per wave
-    f.w_q = a.Lq <= kq ? 1 : 4;
-    f.w_k = a.Lk <= 2 * kk ? (a.Lk <= kk ? 1 : 2) : 4;
-    f.rows_q = kq * f.w_q;
-    f.rows_k = kk * f.w_k;
+    const int per = elem == 4 ? 16 : 32;                            // rows (keys) of a wave: float32 operands take twice the registers
+    f.w_q = a.Lq <= 2 * per ? (a.Lq <= per ? 1 : 2) : 4;
+    f.w_k = a.Lk <= 2 * per ? (a.Lk <= per ? 1 : 2) : 4;
+    f.rows_q = per * f.w_q;
+    f.rows_k = per * f.w_k;
     f.nrow_q = div_up(a.Lq, f.rows_q);
     f.nrow_k = div_up(a.Lk, f.rows_k);
+    // heads that share keys are walked by one block in turn; in parts where that leaves CUs without work
+    const long long blocks = (long long)a.B * a.Hk * f.nchunk * f.nrow_k;
+    const int G = a.H / a.Hk;
+    f.nparts = blocks >= 1024 || blocks == 0 ? 1 : (int)(1024 / blocks < G ? 1024 / blocks : G);
     f.nr = (long long)a.B * f.nchunk * f.nrow_q * f.w_q;
     return f;
 }
 constexpr int DB_SPLITS = 64;
 
 struct BwdWs {
-    long long dO, delta, dq, dk, db, db2, total;
+    long long dO, delta, dq, dk, dv, db, db2, total;
 };
 inline BwdWs layout_backward(const Args &a, int kind, int elem, const BwdPlan &f)
 {
@@ -71,7 +75,8 @@ inline BwdWs layout_backward(const Args &a, int kind, int elem, const BwdPlan &f
     w.dO = take(a.gate ? rows * a.dv * elem : 0);
     w.delta = take(kind == SOFTMAX ? rows * 4 : 0);
     w.dq = take(f.nchunk > 1 ? rows * a.dk * f.nchunk * 4 : 0);
-    w.dk = take(f.nchunk > 1 ? keys * a.dk * f.nchunk * 4 : 0);
+    w.dk = take(f.nchunk * f.nparts > 1 ? keys * a.dk * f.nchunk * f.nparts * 4 : 0);
+    w.dv = take(f.nparts > 1 ? keys * a.dv * f.nparts * 4 : 0);
     w.db = take(a.table ? f.nr * a.H * (2 * a.D + 1) * 4 : 0);
     w.db2 = take(a.table ? (long long)DB_SPLITS * a.H * (2 * a.D + 1) * 4 : 0);
     w.total = at;
@@ -85,6 +90,7 @@ static __global__ void __launch_bounds__(256) db_rows_kernel(const float *part, 
     const long long per = (R + DB_SPLITS - 1) / DB_SPLITS, r0 = s * per, r1 = r0 + per < R ? r0 + per : R;
     for (int t = threadIdx.x; t < TW; t += 256) {
         float x = 0.f;
+#pragma unroll 8
         for (long long r = r0; r < r1; ++r) x += part[(h * R + r) * TW + t];
         out[(long long)blockIdx.x * TW + t] = x;
     }
@@ -96,6 +102,7 @@ template <class T> __global__ void __launch_bounds__(256) db_buckets_kernel(cons
     const int h = blockIdx.x;
     for (int t = threadIdx.x; t < TW; t += 256) {
         float x = 0.f;
+#pragma unroll 16
         for (int s = 0; s < DB_SPLITS; ++s) x += part[((long long)h * DB_SPLITS + s) * TW + t];
         sums[t] = x;
         const int b = bucket_of[t];
@@ -104,6 +111,7 @@ template <class T> __global__ void __launch_bounds__(256) db_buckets_kernel(cons
     __syncthreads();
     for (int b = threadIdx.x; b < nb; b += 256) {
         float x = 0.f;
+#pragma unroll 16
         for (int t = 0; t < TW; ++t) x += bk[t] == b ? sums[t] : 0.f;
         if (f32) reinterpret_cast<float *>(dtable)[(long long)b * H + h] = x;
         else reinterpret_cast<T *>(dtable)[(long long)b * H + h] = (T)x;
@@ -124,7 +132,7 @@ template <class K> int launch(K kernel, long long blocks, int threads, size_t sm
 template <class T, int KIND, int DK, int MT, int NT, int WM, int WN> int launch_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
 {
     constexpr int KT = 32;
-    const size_t smem = sizeof(T) * KT * (DK + WN * NT * 16) * (a.Lk > KT ? 2 : 1) + (a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * (2 * a.D + 1) : 0);
+    const size_t smem = sizeof(T) * KT * (DK + WN * NT * 16) * (a.Lk > KT ? 2 : 1) + (a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * table_width(a.D) : 0);
     return launch(fwd_kernel<T, KIND, DK, MT, NT, WM, WN, KT>, (long long)a.B * f.heads * f.nsplit * f.nchunk * f.nrow, 64 * WM * WN, smem, a, st);
 }
 template <class T, int KIND, int DK> int pick_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
@@ -164,19 +172,21 @@ template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
 
 template <class T, int KIND, int DK, int DVC, int W> int launch_dq(const Args &a, const BwdPlan &f, hipStream_t st)
 {
-    const size_t smem = sizeof(T) * 32 * (DK + DVC) * (a.Lk > 32 ? 2 : 1) + (a.table ? sizeof(float) * ((1 + W) * (2 * a.D + 1) + W * 32 * 33) : 0);
-    return launch(dq_kernel<T, KIND, DK, DVC, 2, W>, (long long)a.B * a.H * f.nchunk * f.nrow_q, 64 * W, smem, a, st);
+    constexpr int MT = sizeof(T) == 4 ? 1 : 2;
+    const size_t smem = sizeof(T) * 32 * (DK + DVC) * (a.Lk > 32 ? 2 : 1) + (a.table ? sizeof(float) * (table_width(a.D) + W * (2 * a.D + 1) + W * 32 * (MT * 16 + 1)) : 0);
+    return launch(dq_kernel<T, KIND, DK, DVC, MT, W>, (long long)a.B * a.H * f.nchunk * f.nrow_q, 64 * W, smem, a, st);
 }
 template <class T, int KIND, int DK, int DVC, int W> int launch_dkv(const Args &a, const BwdPlan &f, hipStream_t st)
 {
-    const size_t smem = sizeof(T) * 32 * (DK + DVC) * (a.Lq > 32 ? 2 : 1) + 128 * sizeof(float) + (a.table ? sizeof(float) * (2 * a.D + 1) : 0);
-    return launch(dkv_kernel<T, KIND, DK, DVC, sizeof(T) == 4 ? 1 : 2, W>, (long long)a.B * a.Hk * f.nchunk * f.nrow_k, 64 * W, smem, a, st);
+    const size_t smem = sizeof(T) * 32 * (DK + DVC) * (a.Lq > 32 ? 2 : 1) + 128 * sizeof(float) + (a.table ? sizeof(float) * table_width(a.D) : 0);
+    return launch(dkv_kernel<T, KIND, DK, DVC, sizeof(T) == 4 ? 1 : 2, W>, (long long)a.B * a.Hk * f.nchunk * f.nparts * f.nrow_k, 64 * W, smem, a, st);
 }
 template <class T, int KIND, int DK, int DVC> int pick_bwd(Args a, const BwdPlan &f, hipStream_t st)
 {
     a.nchunk = f.nchunk;
+    a.nparts = f.nparts;
     a.nrow = f.nrow_q;
-    int rc = f.w_q == 1 ? launch_dq<T, KIND, DK, DVC, 1>(a, f, st) : launch_dq<T, KIND, DK, DVC, 4>(a, f, st);
+    int rc = f.w_q == 1 ? launch_dq<T, KIND, DK, DVC, 1>(a, f, st) : (f.w_q == 2 ? launch_dq<T, KIND, DK, DVC, 2>(a, f, st) : launch_dq<T, KIND, DK, DVC, 4>(a, f, st));
     if (rc != TLK_OK) return rc;
     a.nrow = f.nrow_k;
     if (f.w_k == 1) return launch_dkv<T, KIND, DK, DVC, 1>(a, f, st);
@@ -212,14 +222,20 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
     a.dq = io.dq; a.dk_ = io.dk; a.dv_ = io.dv;
     a.dq_part = reinterpret_cast<float *>(ws + w.dq);
     a.dk_part = reinterpret_cast<float *>(ws + w.dk);
+    a.dv_part = reinterpret_cast<float *>(ws + w.dv);
     a.db_part = reinterpret_cast<float *>(ws + w.db);
     int rc = kind == SOFTMAX ? pick_bwd_sizes<T, SOFTMAX>(a, f, st) : pick_bwd_sizes<T, RELU2>(a, f, st);
     if (rc != TLK_OK) return rc;
-    if (f.nchunk > 1) {
-        if (rows > 0) hipLaunchKernelGGL(sum_chunks_kernel<T>, dim3((unsigned)((rows * a.dk / 4 + 255) / 256)), dim3(256), 0, st, a.dq_part, reinterpret_cast<T *>(a.dq), rows * a.dk, f.nchunk);
-        if (keys > 0) hipLaunchKernelGGL(sum_chunks_kernel<T>, dim3((unsigned)((keys * a.dk / 4 + 255) / 256)), dim3(256), 0, st, a.dk_part, reinterpret_cast<T *>(a.dk_), keys * a.dk, f.nchunk);
+    const auto join = [&](const float *part, void *y, long long n, int parts) -> int {
+        if (parts <= 1 || n <= 0) return TLK_OK;
+        if ((n / 4 + 255) / 256 > 0x7fffffffLL) return fail(TLK_EINVAL, "tlk_gau_attention: more than 2^31 - 1 workgroups");
+        hipLaunchKernelGGL(sum_parts_kernel<T>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, part, reinterpret_cast<T *>(y), n, parts);
         TLK_HIP(hipGetLastError());
-    }
+        return TLK_OK;
+    };
+    if ((rc = join(a.dq_part, a.dq, rows * a.dk, f.nchunk)) != TLK_OK) return rc;
+    if ((rc = join(a.dk_part, a.dk_, keys * a.dk, f.nchunk * f.nparts)) != TLK_OK) return rc;
+    if ((rc = join(a.dv_part, a.dv_, keys * a.dv, f.nparts)) != TLK_OK) return rc;
     if (a.table) {
         const int TW = 2 * a.D + 1;
         float *p2 = reinterpret_cast<float *>(ws + w.db2);
