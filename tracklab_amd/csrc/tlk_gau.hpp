@@ -107,56 +107,88 @@ template <class T, int ROWS, int COLS, int NW> struct Tile {
         }
     }
     // `rows`: how many of the tile's rows there are (uniform); `base`: its first row (uniform)
-    __device__ __forceinline__ void issue(const T *base, int rows, char *lds, int lane) const
+    __device__ __forceinline__ void load(const T *base, int rows, char *lds, int lane, const bool whole) const
     {
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int inst = i * NW + wave;
             if (ROWS * C / 64 % NW != 0 && inst >= ROWS * C / 64) break;
-            unsigned o = off[i];
-            if (rows < ROWS) o = (inst * 64 + lane) / C < rows ? o : OOB;
+            const unsigned o = whole || (inst * 64 + lane) / C < rows ? off[i] : OOB;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + inst * 1024), 16, (int)o, 0, 0, 0);
         }
     }
-    // eight consecutive values of row r, from column k (a multiple of 8)
-    static __device__ __forceinline__ typename Ty<T>::V8 row8(const char *lds, int r, int k)
+    __device__ __forceinline__ void issue(const T *base, int rows, char *lds, int lane) const
     {
+        if (rows >= ROWS) load(base, rows, lds, lane, true);
+        else load(base, rows, lds, lane, false);
+    }
+    // Fragment reads.  A lane's place in the first fragment (row_at, col_at) is made once per tile and hidden from the optimiser; the place in any other is
+    // one exclusive or with a constant (rows begin at multiples of the twisted field) plus a constant.  Left visible, all places of a tile are kept in
+    // registers across the loop -- up to 24 of them, where the accumulators leave none.  (One step from the buffer's start to the address: after a few
+    // steps the compiler loses track of which object a pointer came from, and waits for loads it need not wait for.)
+    static constexpr int M = (C < 16 ? C : 16) - 1;
+    static __device__ __forceinline__ int chunk(int c) { return c / (M + 1) * ((M + 1) * 16); }
+    static __device__ __forceinline__ int row_at(int at, int g, int l)
+    {
+        int o = at + l * ROWB + (((sizeof(T) == 2 ? g : 2 * g) ^ twist(l)) << 4);
+        asm volatile("" : "+v"(o));
+        return o;
+    }
+    // values 32 ks + 8 g .. + 7 of row 16 n + l
+    static __device__ __forceinline__ typename Ty<T>::V8 row8(const char *buf, int place, int n, int ks)
+    {
+        const int c = ks * 32 / VN, o = (place ^ ((c & M) << 4)) + chunk(c) + n * 16 * ROWB;
         if constexpr (sizeof(T) == 2) {
-            return *reinterpret_cast<const typename Ty<T>::V8 *>(lds + r * ROWB + ((k / 8 ^ twist(r)) << 4));
+            return *reinterpret_cast<const typename Ty<T>::V8 *>(buf + o);
         } else {
-            const f4 a = *reinterpret_cast<const f4 *>(lds + r * ROWB + ((k / 4 ^ twist(r)) << 4));
-            const f4 b = *reinterpret_cast<const f4 *>(lds + r * ROWB + (((k / 4 + 1) ^ twist(r)) << 4));
+            const int o1 = (place ^ ((c & M) << 4) ^ 16) + chunk(c) + n * 16 * ROWB;
+            const f4 a = *reinterpret_cast<const f4 *>(buf + o);
+            const f4 b = *reinterpret_cast<const f4 *>(buf + o1);
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    // rows r0 + 4 g + 0..3 of column c0 + l (g = lane / 16, l = lane % 16, r0 and c0 multiples of 16)
-    static __device__ __forceinline__ typename Ty<T>::V4 col4(const char *lds, int r0, int c0, int g, int l)
+    struct Col { int o[sizeof(T) == 2 ? 1 : 4]; };
+    static __device__ __forceinline__ Col col_at(int at, int g, int l)
     {
+        Col p;
+#pragma unroll
+        for (int i = 0; i < (sizeof(T) == 2 ? 1 : 4); ++i) {
+            const int r = g * 4 + (sizeof(T) == 2 ? l >> 2 : i);
+            p.o[i] = sizeof(T) == 2 ? at + r * ROWB + ((((l >> 1) & 1) ^ twist(r)) << 4) + (l & 1) * 8 : at + r * ROWB + (((l >> 2) ^ twist(r)) << 4) + (l & 3) * 4;
+            asm volatile("" : "+v"(p.o[i]));
+        }
+        return p;
+    }
+    // rows r0 + 4 g + 0..3 of column 16 n + l (r0 a multiple of 16)
+    static __device__ __forceinline__ typename Ty<T>::V4 col4(const char *buf, const Col &place, int r0, int n)
+    {
+        const int c = n * 16 / VN;
         if constexpr (sizeof(T) == 2) {
-            const int r = g * 4 + (l >> 2), c = (c0 >> 3) + ((l >> 1) & 1);
-            const char *p = lds + (r0 + r) * ROWB + ((c ^ twist(r0 + r)) << 4) + (l & 1) * 8;
-            return __builtin_bit_cast(typename Ty<T>::V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(p)));
+            const int o = (place.o[0] ^ ((c & M) << 4)) + chunk(c) + r0 * ROWB;
+            return __builtin_bit_cast(typename Ty<T>::V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(buf + o)));
         } else {
             typename Ty<T>::V4 v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int r = r0 + g * 4 + i;
-                v[i] = *reinterpret_cast<const float *>(lds + r * ROWB + ((((c0 + l) >> 2) ^ twist(r)) << 4) + (l & 3) * 4);
+                const int o = (place.o[i] ^ ((c & M) << 4)) + chunk(c) + r0 * ROWB;
+                v[i] = *reinterpret_cast<const float *>(buf + o);
             }
             return v;
         }
     }
-    static __device__ __forceinline__ typename Ty<T>::V8 col8(const char *lds, int r0, int c0, int g, int l)      // rows r0 + 4 g + 0..3 and r0 + 16 + 4 g + 0..3
+    static __device__ __forceinline__ typename Ty<T>::V8 col8(const char *buf, const Col &place, int r0, int n)      // rows r0 + 4 g + 0..3 and r0 + 16 + 4 g + 0..3
     {
-        return __builtin_shufflevector(col4(lds, r0, c0, g, l), col4(lds, r0 + 16, c0, g, l), 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_shufflevector(col4(buf, place, r0, n), col4(buf, place, r0 + 16, n), 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
 // every load of this wave has landed in LDS and every read has returned; then the same for the workgroup
 __device__ __forceinline__ void tiles_ready()
 {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x70);               // vmcnt(0) lgkmcnt(0), as a builtin: the compiler then knows that nothing is in flight into this tile
     __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -169,6 +201,30 @@ template <class T> __device__ __forceinline__ typename Ty<T>::V8 pack8(f4 a, f4 
         r[4 + i] = (T)b[i];
     }
     return r;
+}
+
+// N fragments from LDS, each used by a few matrix instructions: B of them are read while the B before are multiplied.  (An LDS read takes longer than
+// the two instructions that one fragment feeds; left to itself the compiler keeps one or two reads in flight and every fragment waits.)
+// `first`: the first B fragments, read by fragments() earlier, behind other work.
+template <int B, class V8, class Load> __device__ __forceinline__ void fragments(V8 (&f)[B], int from, Load load)
+{
+#pragma unroll
+    for (int i = 0; i < B; ++i) f[i] = load(from + i);
+}
+template <int N, int B, class V8, class Load, class Use> __device__ __forceinline__ void stream(V8 (&first)[B], Load load, Use use)
+{
+    static_assert(N % B == 0, "whole batches");
+    V8 f[2][B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) f[0][i] = first[i];
+#pragma unroll
+    for (int s = 0; s < N / B; ++s) {
+        if (s + 1 < N / B) fragments(f[(s + 1) & 1], (s + 1) * B, load);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < B; ++i) use(s * B + i, f[s & 1][i]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // The learned table over distances of head h, in LDS: -D .. D with MARGIN more entries of the end values on both sides, so that a tile that reaches
@@ -213,7 +269,8 @@ __device__ __forceinline__ int wave_max_i(int x)
     for (int o = 32; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o));
     return x;
 }
-__device__ __forceinline__ float relu_(float x) { return x < 0.f ? 0.f : x; }          // (NaN stays NaN)
+__device__ __forceinline__ float relu_(float x) { return __builtin_elementwise_maximum(x, 0.f); }      // (v_maximum3: NaN stays NaN)
+__device__ __forceinline__ float pow2_(float x) { return __builtin_amdgcn_exp2f(x); }                  // (one instruction, 1 ulp; below 2^-126: zero)
 
 // running power of two of a column's float16 operands: values times 2^-e stay below 2^7; `t` = largest magnitude of this tile's column.
 // Returns the factor for what has been summed so far (1 where nothing changes).
@@ -229,20 +286,16 @@ __device__ __forceinline__ float raise_exponent(int &e, float t)
 }
 constexpr int E_NONE = -120;                      // exponent before the first non-zero value
 
-// scores of a wave's column tile: scale and bias.  `near`: the table at this lane's first distance, STEP entries further with every row of the tile; where
+// four scores of a lane: scale and bias.  `near`: the table at the first one's distance, STEP entries further with every row; where
 // the whole tile lies beyond +-D (or there is no bias) one value does for all (uniform over the wave).
-template <int STEP, int NS> __device__ __forceinline__ void add_bias(f4 (&s)[NS], float sc, bool is_near, const float *near, float far)
+template <int STEP> __device__ __forceinline__ void add_bias(f4 &s, float sc, bool is_near, const float *near, float far)
 {
     if (is_near) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[n][r] = __builtin_fmaf(s[n][r], sc, near[STEP * (n * 16 + r)]);
+        for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(s[r], sc, near[STEP * r]);
     } else {
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[n][r] = __builtin_fmaf(s[n][r], sc, far);
+        for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(s[r], sc, far);
     }
 }
 
@@ -251,16 +304,18 @@ template <int STEP, int NS> __device__ __forceinline__ void add_bias(f4 (&s)[NS]
 // (few queries: the heads that share keys and values are answered in one pass over them).
 // Block order, here and in the backward kernels: sequences, key heads and chunks of dv vary fastest, so that the blocks that walk the same keys land on
 // one XCD (workgroups go to the 8 XCDs in turn) and share its L2; row tiles vary slowest, the longest causal walks first.
-template <class T, int KIND, int DK, int MT, int NT, int WM, int WN, int KT>
-__global__ void __launch_bounds__(64 * WM * WN, WN > 1 && MT * NT <= 8 ? 4 : 2) fwd_kernel(const Args p)
+template <class T, int KIND, int DK, int MT, int NT, int WM, int WN, int KT, bool ONE>
+__global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT * NT <= 4 ? 4 : (MT * NT <= 8 ? 3 : 2)) : 2) fwd_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
     constexpr int NTH = 64 * WM * WN, BM = WM * MT * 16, DVB = WN * NT * 16, NS = KT / 16;
     using TK = Tile<T, KT, DK, WM * WN>;
     using TV = Tile<T, KT, DVB, WM * WN>;
     constexpr int BUF = TK::BYTES + TV::BYTES;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    float *tab = reinterpret_cast<float *>(smem + (p.Lk > KT ? 2 : 1) * BUF);
+    // (two objects and a loop that names them in turn, not one with an offset: the compiler then knows that a transposing read of one cannot see the loads
+    // in flight into the other; with one object it drains them before the first such read.  ONE: all keys are one tile, one buffer.)
+    __shared__ __attribute__((aligned(1024))) char buf0[BUF], buf1[ONE ? 16 : BUF];
+    extern __shared__ __attribute__((aligned(16))) float tab[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / WN, wn = w - wm * WN, g = lane >> 4, l = lane & 15;
     const int G = p.H / p.Hk, GB = p.fold ? G : 1, HB = p.H / GB, rows = p.Lq * GB, TW = table_width(p.D);
     int id = blockIdx.x;
@@ -285,11 +340,16 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && MT * NT <= 8 ? 4 : 2) 
     TV tv;
     tk.init(w, lane, p.ks[1], p.dk);
     tv.init(w, lane, p.vs[1], cend);
-    const auto issue = [&](int j, int buf) {
-        tk.issue(K + (long long)j * p.ks[1], ke - j, smem + buf * BUF, lane);
-        tv.issue(V + (long long)j * p.vs[1], ke - j, smem + buf * BUF + TK::BYTES, lane);
+    K += kb * p.ks[1];
+    V += kb * p.vs[1];
+    const long long kstep = KT * p.ks[1], vstep = KT * p.vs[1];
+    const auto issue = [&](int j, char *buf) __attribute__((always_inline)) {        // the tiles in turn: K and V move along
+        tk.issue(K, ke - j, buf, lane);
+        tv.issue(V, ke - j, buf + TK::BYTES, lane);
+        K += kstep;
+        V += vstep;
     };
-    if (kb < ke) issue(kb, 0);
+    if (kb < ke) issue(kb, buf0);
     if (p.table)
         for (int i = 0; i < GB; ++i) expand_bias<T, KIND>(p, h0 + i, tab + i * TW, NTH);
     int qi[MT], qh[MT], pos[MT];
@@ -336,45 +396,59 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && MT * NT <= 8 ? 4 : 2) 
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) { m[mt] = NEG; lsum[mt] = 0.f; ex[mt] = E_NONE; }
     const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
-
-    int buf = 0;
-    for (int j0 = kb; j0 < ke; j0 += KT, buf ^= 1) {
-        tiles_ready();                                             // this tile has landed, and the other buffer is free
-        if (j0 + KT < ke) issue(j0 + KT, buf ^ 1);
-        if (pmin > pmax || (p.causal && j0 > pmax)) continue;      // no row of this wave, or none that sees this tile (uniform over the wave)
-        const char *Ks = smem + buf * BUF, *Vs = Ks + TK::BYTES;
-        f4 s[MT][NS];
+    float flo[MT], fhi[MT];                                        // the bias beyond +-D
+    if (p.table) __syncthreads();
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
+    for (int mt = 0; mt < MT; ++mt) {
+        flo[mt] = p.table ? tab[qh[mt] * TW] : 0.f;
+        fhi[mt] = p.table ? tab[qh[mt] * TW + TW - 1] : 0.f;
+    }    const auto step = [&](const char *cur, char *next, int j0) __attribute__((always_inline)) {
+        tiles_ready();                                             // this tile has landed, and the other buffer is free
+        if (!ONE && j0 + KT < ke) issue(j0 + KT, next);
+        if (pmin > pmax || (p.causal && j0 > pmax)) return;        // no row of this wave, or none that sees this tile (uniform over the wave)
+        f4 s[MT][NS];
+        constexpr int KS = DK / 32, BK = NS * KS < 4 ? NS * KS : 4, BV = NT < 4 ? NT : 4;
+        const int krow = TK::row_at(0, g, l);
+        const typename TV::Col vcol = TV::col_at(TK::BYTES, g, l);
+        const auto key = [&](int i) __attribute__((always_inline)) { return TK::row8(cur, krow, i / KS, i % KS); };
+        const auto val = [&](int i) __attribute__((always_inline)) { return TV::col8(cur, vcol, i / NT * 32, wn * NT + i % NT); };
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) s[mt][n] = f4{0, 0, 0, 0};
+        V8 kf[BK], vf[BV];
+        fragments(kf, 0, key);
+        stream<NS * KS, BK>(kf, key, [&](int i, V8 a) __attribute__((always_inline)) {
 #pragma unroll
-            for (int ks = 0; ks < DK / 32; ++ks) {
-                const V8 a = TK::row8(Ks, n * 16 + l, ks * 32 + g * 8);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, qf[mt][ks], s[mt][n]);
-            }
-        }
-        // scores: scale, bias, mask
+            for (int mt = 0; mt < MT; ++mt) s[mt][i / KS] = Ty<T>::mma(a, qf[mt][i % KS], s[mt][i / KS]);
+        });
+        fragments(vf, 0, val);
+        __builtin_amdgcn_sched_barrier(0);
+        // scores: scale, bias, mask; most tiles lie beyond +-D of all rows and are seen by all of them
         const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin);
-        const int where = !p.table ? 0 : (j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3));
+        const int where = !p.table || j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3);
+        if (full && where != 3) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const float *tb = tab + qh[mt] * TW;
-            add_bias<1>(s[mt], sc, where == 3, tb + (p.D + MARGIN + j0 + g * 4 - pos[mt]), where ? tb[where == 1 ? TW - 1 : 0] : 0.f);
-            if (!full) {
+            for (int mt = 0; mt < MT; ++mt) {
+                const float far = where == 1 ? fhi[mt] : flo[mt];
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[mt][n][r] = __builtin_fmaf(s[mt][n][r], sc, far);
+            }
+        } else {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
                 const int last = p.causal ? min(ke - 1, pos[mt]) : ke - 1;
 #pragma unroll
-                for (int n = 0; n < NS; ++n)
+                for (int n = 0; n < NS; ++n) {
+                    add_bias<1>(s[mt][n], sc, where == 3, tab + qh[mt] * TW + (p.D + MARGIN + j0 + n * 16 + g * 4 - pos[mt]), where == 1 ? fhi[mt] : flo[mt]);
+                    if (!full)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (j0 + n * 16 + g * 4 + r > last) s[mt][n][r] = KIND == SOFTMAX ? -INFINITY : 0.f;
+                        for (int r = 0; r < 4; ++r)
+                            if (j0 + n * 16 + g * 4 + r > last) s[mt][n][r] = KIND == SOFTMAX ? -INFINITY : 0.f;
+                }
             }
-            if (KIND == RELU2)
-#pragma unroll
-                for (int n = 0; n < NS; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[mt][n][r] = relu_(s[mt][n][r]);
         }
         // weights
         float fac[MT];
@@ -382,6 +456,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && MT * NT <= 8 ? 4 : 2) 
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             fac[mt] = 1.f;
+            float down = 1.f;
             if (KIND == SOFTMAX || Ty<T>::scaled) {
                 float t = s[mt][0][0];
 #pragma unroll
@@ -391,12 +466,13 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && MT * NT <= 8 ? 4 : 2) 
                 t = over_groups_max(t);
                 if (KIND == SOFTMAX) {
                     const float mn = fmaxf(m[mt], t);
-                    fac[mt] = exp2f(m[mt] - mn);
+                    fac[mt] = pow2_(m[mt] - mn);
                     m[mt] = mn;
                     lsum[mt] *= fac[mt];
                 } else {
                     const float f = raise_exponent(ex[mt], t);
                     fac[mt] = f * f;
+                    down = ldexpf(1.f, -ex[mt]);
                 }
                 any |= fac[mt] != 1.f;
             }
@@ -406,10 +482,11 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && MT * NT <= 8 ? 4 : 2) 
                 for (int r = 0; r < 4; ++r) {
                     float x = s[mt][n][r];
                     if (KIND == SOFTMAX) {
-                        x = exp2f(x - m[mt]);
+                        x = pow2_(x - m[mt]);
                         lsum[mt] += x;
                     } else {
-                        if (Ty<T>::scaled) x = ldexpf(x, -ex[mt]);
+                        x = relu_(x);
+                        if (Ty<T>::scaled) x *= down;
                         x = x * x;
                     }
                     s[mt][n][r] = x;
@@ -421,17 +498,22 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && MT * NT <= 8 ? 4 : 2) 
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) acc[n][mt] *= fac[mt];
         }
+        V8 pb[NS / 2][MT];
 #pragma unroll
-        for (int kk = 0; kk < NS / 2; ++kk) {
-            V8 pb[MT];
+        for (int kk = 0; kk < NS / 2; ++kk)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) pb[mt] = pack8<T>(s[mt][2 * kk], s[mt][2 * kk + 1]);
+            for (int mt = 0; mt < MT; ++mt) pb[kk][mt] = pack8<T>(s[mt][2 * kk], s[mt][2 * kk + 1]);
+        stream<NS / 2 * NT, BV>(vf, val, [&](int i, V8 a) __attribute__((always_inline)) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const V8 a = TV::col8(Vs, kk * 32, (wn * NT + n) * 16, g, l);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) acc[n][mt] = Ty<T>::mma(a, pb[mt], acc[n][mt]);
-            }
+            for (int mt = 0; mt < MT; ++mt) acc[i % NT][mt] = Ty<T>::mma(a, pb[i / NT][mt], acc[i % NT][mt]);
+        });
+    };
+    if constexpr (ONE) {
+        if (kb < ke) step(buf0, buf1, kb);
+    } else {
+        for (int j0 = kb; j0 < ke; j0 += 2 * KT) {
+            step(buf0, buf1, j0);
+            if (j0 + KT < ke) step(buf1, buf0, j0 + KT);
         }
     }
 #pragma unroll
@@ -497,7 +579,7 @@ template <class T, int KIND> __global__ void __launch_bounds__(256) join_kernel(
         float m = NEG, s = 0.f;
         for (int i = 0; i < p.nsplit; ++i) m = fmaxf(m, p.ml[2 * (i * nrow + row)]);
         for (int i = 0; i < p.nsplit; ++i) {
-            const float f = exp2f(p.ml[2 * (i * nrow + row)] - m);
+            const float f = pow2_(p.ml[2 * (i * nrow + row)] - m);
             s += f * p.ml[2 * (i * nrow + row) + 1];
             x += *reinterpret_cast<const f4 *>(p.part + (i * nrow + row) * p.dv + c) * f;
         }
@@ -570,7 +652,7 @@ template <class T> __global__ void __launch_bounds__(256) gate_bwd_kernel(const 
 template <int KIND> __device__ __forceinline__ float dscore(float x, float dw, float lse, float delta, float &w)
 {
     if (KIND == SOFTMAX) {
-        w = exp2f(x - lse);
+        w = pow2_(x - lse);
         return w * (dw - delta);
     }
     const float s = relu_(x);
@@ -587,11 +669,11 @@ template <class T, int NS> __device__ __forceinline__ float hold(f4 (&x)[NS], in
     for (int n = 0; n < NS; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) t = fmaxf(t, fabsf(x[n][r]));
-    const float f = raise_exponent(e, over_groups_max(t));
+    const float f = raise_exponent(e, over_groups_max(t)), down = ldexpf(1.f, -e);
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[n][r] = ldexpf(x[n][r], -e);
+        for (int r = 0; r < 4; ++r) x[n][r] *= down;
     return f;
 }
 template <class T> __device__ __forceinline__ float unhold(int e) { return !Ty<T>::scaled ? 1.f : (e == E_NONE ? 0.f : ldexpf(1.f, e)); }
@@ -599,7 +681,7 @@ template <class T> __device__ __forceinline__ float unhold(int e) { return !Ty<T
 // dQ and the bias gradient: W waves, MT x 16 queries each; walks the keys.  dS^T has a query in the column: its registers are the B operand of
 // dQ^T = K^T dS^T.  The bias gradient needs sums along diagonals: a tile that lies beyond +-D of all its queries is one sum in registers, one near
 // the diagonal goes through a wave's own (KT x BM) LDS tile and each lane sums one diagonal -- no atomics, the order is fixed.
-template <class T, int KIND, int DK, int DVC, int MT, int W>
+template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
 __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
@@ -608,9 +690,9 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
     using TK = Tile<T, KT, DK, W>;
     using TV = Tile<T, KT, DVC, W>;
     constexpr int BUF = TK::BYTES + TV::BYTES;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    __shared__ __attribute__((aligned(1024))) char buf0[BUF], buf1[ONE ? 16 : BUF];     // (two objects: see fwd_kernel)
+    extern __shared__ __attribute__((aligned(16))) float tab[];
     const int TW = p.table ? table_width(p.D) : 0, NB = p.table ? 2 * p.D + 1 : 0;
-    float *tab = reinterpret_cast<float *>(smem + (p.Lk > KT ? 2 : 1) * BUF);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15;
     float *dbw = tab + TW + w * NB, *tile = tab + TW + W * NB + w * KT * LT;         // this wave's distance sums and its dS tile
     int id = blockIdx.x;
@@ -628,11 +710,14 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
     TV tv;
     tk.init(w, lane, p.ks[1], p.dk);
     tv.init(w, lane, p.vs[1], cend);
-    const auto issue = [&](int j, int buf) {
-        tk.issue(K + (long long)j * p.ks[1], ke - j, smem + buf * BUF, lane);
-        tv.issue(V + (long long)j * p.vs[1], ke - j, smem + buf * BUF + TK::BYTES, lane);
+    const long long kstep = KT * p.ks[1], vstep = KT * p.vs[1];
+    const auto issue = [&](int j, char *buf) __attribute__((always_inline)) {        // the tiles in turn: K and V move along
+        tk.issue(K, ke - j, buf, lane);
+        tv.issue(V, ke - j, buf + TK::BYTES, lane);
+        K += kstep;
+        V += vstep;
     };
-    if (0 < ke) issue(0, 0);
+    if (0 < ke) issue(0, buf0);
     if (p.table) {
         expand_bias<T, KIND>(p, h, tab, NTH);
         for (int t = lane; t < NB; t += 64) dbw[t] = 0.f;
@@ -665,46 +750,63 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
     for (int mt = 0; mt < MT; ++mt) ex[mt] = E_NONE;
     float lo = 0.f, hi = 0.f;
     const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
-    int buf = 0;
-    for (int j0 = 0; j0 < ke; j0 += KT, buf ^= 1) {
+    if (p.table) __syncthreads();
+    const float flo = p.table ? tab[0] : 0.f, fhi = p.table ? tab[TW - 1] : 0.f;          // the bias beyond +-D
+    const auto step = [&](const char *cur, char *next, int j0) __attribute__((always_inline)) {
         tiles_ready();
-        if (j0 + KT < ke) issue(j0 + KT, buf ^ 1);
-        if (i0 >= p.Lq || (p.causal && j0 > pmax)) continue;
-        const char *Ks = smem + buf * BUF, *Vs = Ks + TK::BYTES;
-        f4 s[MT][NS], dp[MT][NS];
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) { s[mt][n] = f4{0, 0, 0, 0}; dp[mt][n] = f4{0, 0, 0, 0}; }
-#pragma unroll
-            for (int ks = 0; ks < DK / 32; ++ks) {
-                const V8 a = TK::row8(Ks, n * 16 + l, ks * 32 + g * 8);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, qf[mt][ks], s[mt][n]);
-            }
-#pragma unroll
-            for (int ks = 0; ks < DVC / 32; ++ks) {
-                const V8 a = TV::row8(Vs, n * 16 + l, ks * 32 + g * 8);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) dp[mt][n] = Ty<T>::mma(a, df[mt][ks], dp[mt][n]);
-            }
-        }
+        if (!ONE && j0 + KT < ke) issue(j0 + KT, next);
+        if (i0 >= p.Lq || (p.causal && j0 > pmax)) return;
         const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin) && i0 + MT * 16 <= p.Lq;
-        const int where = !p.table ? 0 : (j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3));
-        const float far = where ? tab[where == 1 ? TW - 1 : 0] : 0.f;
+        const int where = !p.table || j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3);
+        const float far = where == 1 ? fhi : flo;
         float all = 0.f;
+        f4 s[MT][NS], dp[MT][NS];
+        constexpr int KS = DK / 32, VS = DVC / 32, B = DK + DVC > 256 ? 2 : 4;           // (fragments in flight: what the registers leave)
+        const int krow = TK::row_at(0, g, l), vrow = TV::row_at(TK::BYTES, g, l);
+        const typename TK::Col kplace = TK::col_at(0, g, l);
+        const auto key = [&](int i) __attribute__((always_inline)) { return TK::row8(cur, krow, i / KS, i % KS); };
+        const auto val = [&](int i) __attribute__((always_inline)) { return TV::row8(cur, vrow, i / VS, i % VS); };
+        const auto kcol = [&](int i) __attribute__((always_inline)) { return TK::col8(cur, kplace, 0, i); };
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const int i = i0 + mt * 16 + l;
-            add_bias<1>(s[mt], sc, where == 3, tab + (p.D + MARGIN + j0 + g * 4 - i - q0), far);
-            if (!full) {
-                const int last = i >= p.Lq ? -1 : (p.causal ? min(ke - 1, i + q0) : ke - 1);
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int n = 0; n < NS; ++n) { s[mt][n] = f4{0, 0, 0, 0}; dp[mt][n] = f4{0, 0, 0, 0}; }
+        V8 kf[B], vf[B], cf[B];
+        fragments(kf, 0, key);
+        stream<NS * KS, B>(kf, key, [&](int i, V8 a) __attribute__((always_inline)) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) s[mt][i / KS] = Ty<T>::mma(a, qf[mt][i % KS], s[mt][i / KS]);
+        });
+        fragments(vf, 0, val);
+        stream<NS * VS, B>(vf, val, [&](int i, V8 a) __attribute__((always_inline)) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) dp[mt][i / VS] = Ty<T>::mma(a, df[mt][i % VS], dp[mt][i / VS]);
+        });
+        fragments(cf, 0, kcol);
+        __builtin_amdgcn_sched_barrier(0);
+        if (full && where != 3) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int n = 0; n < NS; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (j0 + n * 16 + g * 4 + r > last) s[mt][n][r] = -INFINITY;
+                    for (int r = 0; r < 4; ++r) s[mt][n][r] = __builtin_fmaf(s[mt][n][r], sc, far);
+        } else {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const int i = i0 + mt * 16 + l, last = i >= p.Lq ? -1 : (p.causal ? min(ke - 1, i + q0) : ke - 1);
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    add_bias<1>(s[mt][n], sc, where == 3, tab + (p.D + MARGIN + j0 + n * 16 + g * 4 - i - q0), far);
+                    if (!full)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (j0 + n * 16 + g * 4 + r > last) s[mt][n][r] = -INFINITY;
+                }
             }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int n = 0; n < NS; ++n)
 #pragma unroll
@@ -713,12 +815,13 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
                     s[mt][n][r] = dscore<KIND>(s[mt][n][r], dp[mt][n][r], lse[mt], del[mt], wgt);
                     all += s[mt][n][r];
                 }
-            if (where == 3)
+        if (where == 3)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int n = 0; n < NS; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = s[mt][n][r];
-        }
         if (where == 1) hi += all;
         if (where == 2) lo += all;
         if (where == 3) {
@@ -748,11 +851,17 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         V8 pb[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) pb[mt] = pack8<T>(s[mt][0], s[mt][1]);
-#pragma unroll
-        for (int n = 0; n < DK / 16; ++n) {
-            const V8 a = TK::col8(Ks, 0, n * 16, g, l);
+        stream<DK / 16, B>(cf, kcol, [&](int n, V8 a) __attribute__((always_inline)) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) acc[n][mt] = Ty<T>::mma(a, pb[mt], acc[n][mt]);
+        });
+    };
+    if constexpr (ONE) {
+        if (0 < ke) step(buf0, buf1, 0);
+    } else {
+        for (int j0 = 0; j0 < ke; j0 += 2 * KT) {
+            step(buf0, buf1, j0);
+            if (j0 + KT < ke) step(buf1, buf0, j0 + KT);
         }
     }
     if (p.table) {
@@ -790,16 +899,17 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
 
 // dK and dV: W waves, MT x 16 keys each; walks the queries of every head that shares the keys.  S has a key in the column: W and dS in registers
 // are the B operands of dV^T = dO^T W and dK^T = Q^T dS.
-template <class T, int KIND, int DK, int DVC, int MT, int W>
-__global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(const Args p)
+template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
+__global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK + DVC == 256) ? 1 : 2) dkv_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
     constexpr int QT = 32, NTH = 64 * W, BN = W * MT * 16, NS = 2;
     using TQ = Tile<T, QT, DK, W>;
     using TO = Tile<T, QT, DVC, W>;
     constexpr int BUF = TQ::BYTES + TO::BYTES;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];
-    float *stats = reinterpret_cast<float *>(smem + (p.Lq > QT ? 2 : 1) * BUF), *tab = stats + 4 * QT;      // two tiles' log-sum-exp and delta
+    __shared__ __attribute__((aligned(1024))) char buf0[BUF], buf1[ONE ? 16 : BUF];     // (two objects: see fwd_kernel)
+    __shared__ __attribute__((aligned(16))) float stats0[2 * QT], stats1[2 * QT];       // the tiles' log-sum-exp and delta
+    extern __shared__ __attribute__((aligned(16))) float tab[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15, G = p.H / p.Hk, TW = table_width(p.D);
     int id = blockIdx.x;
     const int b = id % p.B; id /= p.B;
@@ -843,106 +953,134 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 ? 1 : 2) dkv_kernel(con
     to.init(w, lane, (long long)p.H * p.dv, cend);
     for (int hg = part * G / p.nparts; hg < (part + 1) * G / p.nparts; ++hg) {             // (a part of the heads that share the keys)
         const int h = hk * G + hg;
-        const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2];
-        const T *dO = reinterpret_cast<const T *>(p.dO) + ((long long)b * p.Lq * p.H + h) * p.dv + c0;
+        const long long qstep = QT * p.qs[1], ostep = (long long)QT * p.H * p.dv;
+        const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2] + ib * p.qs[1];              // (the tiles in turn: Q and dO move along)
+        const T *dO = reinterpret_cast<const T *>(p.dO) + (((long long)b * p.Lq + ib) * p.H + h) * p.dv + c0;
         float ls0 = INFINITY, dl0 = 0.f;
-        const auto issue = [&](int i, int buf) {
-            tq.issue(Q + (long long)i * p.qs[1], p.Lq - i, smem + buf * BUF, lane);
-            to.issue(dO + (long long)i * p.H * p.dv, p.Lq - i, smem + buf * BUF + TQ::BYTES, lane);
+        const auto issue = [&](int i, char *buf) __attribute__((always_inline)) {
+            tq.issue(Q, p.Lq - i, buf, lane);
+            to.issue(dO, p.Lq - i, buf + TQ::BYTES, lane);
+            Q += qstep;
+            dO += ostep;
             if (KIND == SOFTMAX && tid < QT) {
                 const long long row = ((long long)b * p.Lq + i + tid) * p.H + h;
                 ls0 = i + tid < p.Lq ? p.lse[row] : INFINITY;
                 dl0 = i + tid < p.Lq && ch == 0 ? p.delta[row] : 0.f;
             }
         };
-        const auto keep = [&](int buf) {
-            if (KIND == SOFTMAX && tid < QT) { stats[buf * 2 * QT + tid] = ls0; stats[buf * 2 * QT + QT + tid] = dl0; }
+        const auto keep = [&](float *st) __attribute__((always_inline)) {
+            if (KIND == SOFTMAX && tid < QT) { st[tid] = ls0; st[QT + tid] = dl0; }
         };
         __syncthreads();                                                                  // the previous head's tiles and table are no longer read
         if (ib < p.Lq) {
-            issue(ib, 0);
-            if (p.table) expand_bias<T, KIND>(p, h, tab, NTH);
-            keep(0);
-        }
-        int buf = 0;
-        for (int i0 = ib; i0 < p.Lq; i0 += QT, buf ^= 1) {
-            if (i0 > ib) keep(buf);
-            tiles_ready();
-            if (i0 + QT < p.Lq) issue(i0 + QT, buf ^ 1);
-            const char *Qs = smem + buf * BUF, *Os = Qs + TQ::BYTES;
-            const float *st = stats + buf * 2 * QT;
-            const int pmin = i0 + q0, pmax = min(p.Lq, i0 + QT) - 1 + q0;
-            if (jmax < jmin || (p.causal && jmin > pmax)) continue;
-            f4 s[MT][NS], dp[MT][NS];
-#pragma unroll
-            for (int n = 0; n < NS; ++n) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) { s[mt][n] = f4{0, 0, 0, 0}; dp[mt][n] = f4{0, 0, 0, 0}; }
-#pragma unroll
-                for (int ks = 0; ks < DK / 32; ++ks) {
-                    const V8 a = TQ::row8(Qs, n * 16 + l, ks * 32 + g * 8);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, kf[mt][ks], s[mt][n]);
-                }
-#pragma unroll
-                for (int ks = 0; ks < DVC / 32; ++ks) {
-                    const V8 a = TO::row8(Os, n * 16 + l, ks * 32 + g * 8);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) dp[mt][n] = Ty<T>::mma(a, vf[mt][ks], dp[mt][n]);
-                }
+            issue(ib, buf0);
+            if (p.table) {
+                expand_bias<T, KIND>(p, h, tab, NTH);
+                __syncthreads();
             }
+        }
+        const float flo = p.table && ib < p.Lq ? tab[0] : 0.f, fhi = p.table && ib < p.Lq ? tab[TW - 1] : 0.f;          // the bias beyond +-D
+        const auto step = [&](const char *cur, float *st, char *next, int i0) __attribute__((always_inline)) {
+            keep(st);
+            tiles_ready();
+            if (!ONE && i0 + QT < p.Lq) issue(i0 + QT, next);
+            const int pmin = i0 + q0, pmax = min(p.Lq, i0 + QT) - 1 + q0;
+            if (jmax < jmin || (p.causal && jmin > pmax)) return;
             const bool full = i0 + QT <= p.Lq && j0 + MT * 16 <= ke && (!p.causal || j0 + MT * 16 - 1 <= pmin);
-            const int where = !p.table ? 0 : (jmin - pmax >= p.D ? 1 : (jmax - pmin <= -p.D ? 2 : 3));
-            const float far = where ? tab[where == 1 ? TW - 1 : 0] : 0.f;
-            V8 wb[MT], db[MT];
+            const int where = !p.table || jmin - pmax >= p.D ? 1 : (jmax - pmin <= -p.D ? 2 : 3);
+            const float far = where == 1 ? fhi : flo;
+            f4 s[MT][NS], wt[MT][NS];                              // (wt: dW first, then the weights)
+            constexpr int KS = DK / 32, VS = DVC / 32, BK = NS * KS < 4 ? NS * KS : 4;
+            const int qplace = TQ::row_at(0, g, l), oplace = TO::row_at(TQ::BYTES, g, l);
+            const typename TQ::Col qcplace = TQ::col_at(0, g, l);
+            const typename TO::Col ocplace = TO::col_at(TQ::BYTES, g, l);
+            const auto qrow = [&](int i) __attribute__((always_inline)) { return TQ::row8(cur, qplace, i / KS, i % KS); };
+            const auto orow = [&](int i) __attribute__((always_inline)) { return TO::row8(cur, oplace, i / VS, i % VS); };
+            const auto ocol = [&](int i) __attribute__((always_inline)) { return TO::col8(cur, ocplace, 0, i); };
+            const auto qcol = [&](int i) __attribute__((always_inline)) { return TQ::col8(cur, qcplace, 0, i); };
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const int j = j0 + mt * 16 + l;
-                f4 wt[NS];
-                add_bias<-1>(s[mt], sc, where == 3, tab + (p.D + MARGIN + j - (i0 + g * 4 + q0)), far);
-                if (!full) {
-                    const int first = j >= ke ? p.Lq : (p.causal ? j - q0 : 0);             // the first query that sees this lane's key
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int n = 0; n < NS; ++n) { s[mt][n] = f4{0, 0, 0, 0}; wt[mt][n] = f4{0, 0, 0, 0}; }
+            V8 qb[BK], ob[4];
+            fragments(qb, 0, qrow);
+            stream<NS * KS, BK>(qb, qrow, [&](int i, V8 a) __attribute__((always_inline)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][i / KS] = Ty<T>::mma(a, kf[mt][i % KS], s[mt][i / KS]);
+            });
+            fragments(ob, 0, orow);
+            stream<NS * VS, 4>(ob, orow, [&](int i, V8 a) __attribute__((always_inline)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) wt[mt][i / VS] = Ty<T>::mma(a, vf[mt][i % VS], wt[mt][i / VS]);
+            });
+            fragments(ob, 0, ocol);
+            __builtin_amdgcn_sched_barrier(0);
+            if (full && where != 3) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int n = 0; n < NS; ++n)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (i0 + n * 16 + g * 4 + r < first || i0 + n * 16 + g * 4 + r >= p.Lq) s[mt][n][r] = -INFINITY;
+                        for (int r = 0; r < 4; ++r) s[mt][n][r] = __builtin_fmaf(s[mt][n][r], sc, far);
+            } else {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const int j = j0 + mt * 16 + l, first = j >= ke ? p.Lq : (p.causal ? j - q0 : 0);             // the first query that sees this lane's key
+#pragma unroll
+                    for (int n = 0; n < NS; ++n) {
+                        add_bias<-1>(s[mt][n], sc, where == 3, tab + (p.D + MARGIN + j - (i0 + n * 16 + g * 4 + q0)), far);
+                        if (!full)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (i0 + n * 16 + g * 4 + r < first || i0 + n * 16 + g * 4 + r >= p.Lq) s[mt][n][r] = -INFINITY;
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                f4 ls = {0, 0, 0, 0}, dl = {0, 0, 0, 0};
+                if (KIND == SOFTMAX) {
+                    ls = *reinterpret_cast<const f4 *>(st + n * 16 + g * 4);
+                    dl = *reinterpret_cast<const f4 *>(st + QT + n * 16 + g * 4);
                 }
 #pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    f4 ls = {0, 0, 0, 0}, dl = {0, 0, 0, 0};
-                    if (KIND == SOFTMAX) {
-                        ls = *reinterpret_cast<const f4 *>(st + n * 16 + g * 4);
-                        dl = *reinterpret_cast<const f4 *>(st + QT + n * 16 + g * 4);
-                    }
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float wgt;
-                        s[mt][n][r] = dscore<KIND>(s[mt][n][r], dp[mt][n][r], ls[r], dl[r], wgt);
-                        wt[n][r] = wgt;
+                        s[mt][n][r] = dscore<KIND>(s[mt][n][r], wt[mt][n][r], ls[r], dl[r], wgt);
+                        wt[mt][n][r] = wgt;
                     }
-                }
-                const float fv = hold<T, NS>(wt, ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
+            }
+            V8 wb[MT], db[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float fv = hold<T, NS>(wt[mt], ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
                 if (Ty<T>::scaled && __any(fv != 1.f))
 #pragma unroll
                     for (int n = 0; n < DVC / 16; ++n) av[n][mt] *= fv;
                 if (Ty<T>::scaled && __any(fk != 1.f))
 #pragma unroll
                     for (int n = 0; n < DK / 16; ++n) ak[n][mt] *= fk;
-                wb[mt] = pack8<T>(wt[0], wt[1]);
+                wb[mt] = pack8<T>(wt[mt][0], wt[mt][1]);
                 db[mt] = pack8<T>(s[mt][0], s[mt][1]);
             }
-#pragma unroll
-            for (int n = 0; n < DVC / 16; ++n) {
-                const V8 a = TO::col8(Os, 0, n * 16, g, l);
+            stream<DVC / 16, 4>(ob, ocol, [&](int n, V8 a) __attribute__((always_inline)) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) av[n][mt] = Ty<T>::mma(a, wb[mt], av[n][mt]);
-            }
-#pragma unroll
-            for (int n = 0; n < DK / 16; ++n) {
-                const V8 a = TQ::col8(Qs, 0, n * 16, g, l);
+            });
+            fragments(ob, 0, qcol);
+            stream<DK / 16, 4>(ob, qcol, [&](int n, V8 a) __attribute__((always_inline)) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) ak[n][mt] = Ty<T>::mma(a, db[mt], ak[n][mt]);
+            });
+        };
+        if constexpr (ONE) {
+            if (ib < p.Lq) step(buf0, stats0, buf1, ib);
+        } else {
+            for (int i0 = ib; i0 < p.Lq; i0 += 2 * QT) {
+                step(buf0, stats0, buf1, i0);
+                if (i0 + QT < p.Lq) step(buf1, stats1, buf0, i0 + QT);
             }
         }
     }

@@ -118,12 +118,13 @@ template <class T> __global__ void __launch_bounds__(256) db_buckets_kernel(cons
     }
 }
 
-template <class K> int launch(K kernel, long long blocks, int threads, size_t smem, const Args &a, hipStream_t st)
+// `fixed`: the kernel's static LDS, `smem`: the bias table and sums behind it
+template <class K> int launch(K kernel, long long blocks, int threads, size_t fixed, size_t smem, const Args &a, hipStream_t st)
 {
     if (blocks <= 0) return TLK_OK;
     if (blocks > 0x7fffffffLL) return fail(TLK_EINVAL, "tlk_gau_attention: more than 2^31 - 1 workgroups");
-    if (smem > 160 * 1024) return fail(TLK_EINVAL, "tlk_gau_attention: max_distance beyond the LDS tile");
-    if (smem > 64 * 1024) TLK_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    if (fixed + smem + 1024 > 160 * 1024) return fail(TLK_EINVAL, "tlk_gau_attention: max_distance beyond the LDS tile");
+    if (fixed + smem > 64 * 1024 && smem > 0) TLK_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), smem, st, a);
     TLK_HIP(hipGetLastError());
     return TLK_OK;
@@ -132,8 +133,11 @@ template <class K> int launch(K kernel, long long blocks, int threads, size_t sm
 template <class T, int KIND, int DK, int MT, int NT, int WM, int WN> int launch_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
 {
     constexpr int KT = 32;
-    const size_t smem = sizeof(T) * KT * (DK + WN * NT * 16) * (a.Lk > KT ? 2 : 1) + (a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * table_width(a.D) : 0);
-    return launch(fwd_kernel<T, KIND, DK, MT, NT, WM, WN, KT>, (long long)a.B * f.heads * f.nsplit * f.nchunk * f.nrow, 64 * WM * WN, smem, a, st);
+    const size_t fixed = sizeof(T) * KT * (DK + WN * NT * 16), smem = a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * table_width(a.D) : 0;
+    const long long blocks = (long long)a.B * f.heads * f.nsplit * f.nchunk * f.nrow;
+    if constexpr (WN > 1)                                           // (one tile of keys: a second buffer would only keep other workgroups off the CU)
+        if (a.Lk <= KT) return launch(fwd_kernel<T, KIND, DK, MT, NT, WM, WN, KT, true>, blocks, 64 * WM * WN, fixed, smem, a, st);
+    return launch(fwd_kernel<T, KIND, DK, MT, NT, WM, WN, KT, false>, blocks, 64 * WM * WN, 2 * fixed, smem, a, st);
 }
 template <class T, int KIND, int DK> int pick_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
 {
@@ -167,19 +171,26 @@ template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
     else rc = a.dk <= 64 ? pick_fwd<T, RELU2, 64>(a, f, st) : pick_fwd<T, RELU2, 128>(a, f, st);
     if (rc != TLK_OK || f.nsplit == 1) return rc;
     const long long blocks = (rows * (a.dv / 4) + 255) / 256;
-    return kind == SOFTMAX ? launch(join_kernel<T, SOFTMAX>, blocks, 256, 0, a, st) : launch(join_kernel<T, RELU2>, blocks, 256, 0, a, st);
+    return kind == SOFTMAX ? launch(join_kernel<T, SOFTMAX>, blocks, 256, 0, 0, a, st) : launch(join_kernel<T, RELU2>, blocks, 256, 0, 0, a, st);
 }
 
 template <class T, int KIND, int DK, int DVC, int W> int launch_dq(const Args &a, const BwdPlan &f, hipStream_t st)
 {
     constexpr int MT = sizeof(T) == 4 ? 1 : 2;
-    const size_t smem = sizeof(T) * 32 * (DK + DVC) * (a.Lk > 32 ? 2 : 1) + (a.table ? sizeof(float) * (table_width(a.D) + W * (2 * a.D + 1) + W * 32 * (MT * 16 + 1)) : 0);
-    return launch(dq_kernel<T, KIND, DK, DVC, MT, W>, (long long)a.B * a.H * f.nchunk * f.nrow_q, 64 * W, smem, a, st);
+    const size_t fixed = sizeof(T) * 32 * (DK + DVC), smem = a.table ? sizeof(float) * (table_width(a.D) + W * (2 * a.D + 1) + W * 32 * (MT * 16 + 1)) : 0;
+    const long long blocks = (long long)a.B * a.H * f.nchunk * f.nrow_q;
+    if constexpr (W < 4)
+        if (a.Lk <= 32) return launch(dq_kernel<T, KIND, DK, DVC, MT, W, true>, blocks, 64 * W, fixed, smem, a, st);
+    return launch(dq_kernel<T, KIND, DK, DVC, MT, W, false>, blocks, 64 * W, 2 * fixed, smem, a, st);
 }
 template <class T, int KIND, int DK, int DVC, int W> int launch_dkv(const Args &a, const BwdPlan &f, hipStream_t st)
 {
-    const size_t smem = sizeof(T) * 32 * (DK + DVC) * (a.Lq > 32 ? 2 : 1) + 128 * sizeof(float) + (a.table ? sizeof(float) * table_width(a.D) : 0);
-    return launch(dkv_kernel<T, KIND, DK, DVC, sizeof(T) == 4 ? 1 : 2, W>, (long long)a.B * a.Hk * f.nchunk * f.nparts * f.nrow_k, 64 * W, smem, a, st);
+    constexpr int MT = sizeof(T) == 4 ? 1 : 2;
+    const size_t fixed = sizeof(T) * 32 * (DK + DVC), smem = a.table ? sizeof(float) * table_width(a.D) : 0;
+    const long long blocks = (long long)a.B * a.Hk * f.nchunk * f.nparts * f.nrow_k;
+    if constexpr (W < 4)
+        if (a.Lq <= 32) return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, true>, blocks, 64 * W, fixed + 512, smem, a, st);
+    return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, false>, blocks, 64 * W, 2 * fixed + 512, smem, a, st);
 }
 template <class T, int KIND, int DK, int DVC> int pick_bwd(Args a, const BwdPlan &f, hipStream_t st)
 {
