@@ -42,7 +42,7 @@ struct Args {
     void *out, *o;
     float *lse;                                 // (B, Lq, H): log2 of the row's sum of 2^(S log2 e), +inf for a row without keys
     float *part, *ml;                           // split keys: (split, B, Lq, H, dv) sums and (split, B, Lq, H, 2) maximum and sum
-    int nsplit, split_keys, nchunk, nrow, fold, nparts;
+    int nsplit, split_keys, nchunk, nrow, fold, nparts, snake;
     // backward
     const void *dO;                             // (B, Lq, H, dv) contiguous: the gradient behind the gate
     const float *delta;                         // (B, Lq, H): sum_d dO o (softmax)
@@ -248,6 +248,8 @@ template <class T, int KIND> __device__ __forceinline__ void expand_bias(const A
     }
 }
 
+// the row tile of the n-th place: the longest causal walks first, from place `snake` on the shortest first
+__device__ __forceinline__ int row_tile(const Args &p, int n) { return n < p.snake ? p.nrow - 1 - n : n - p.snake; }
 __device__ __forceinline__ int key_end(const Args &p, int b) { const int n = p.lens ? p.lens[b] : p.Lk; return n < 0 ? 0 : (n > p.Lk ? p.Lk : n); }
 __device__ __forceinline__ int row_start(const Args &p, int b)
 {
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
     const int hk = id % p.Hk; id /= p.Hk;
     const int ch = id % p.nchunk; id /= p.nchunk;
     const int sp = id % p.nsplit; id /= p.nsplit;
-    const int hg = id % (HB / p.Hk), rt = p.nrow - 1 - id / (HB / p.Hk), h0 = hk * G + hg;
+    const int hg = id % (HB / p.Hk), rt = row_tile(p, id / (HB / p.Hk)), h0 = hk * G + hg;
     const int kend_all = key_end(p, b), q0 = row_start(p, b);
     const int c0 = ch * DVB, cend = p.dv - c0;
     const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0];
@@ -607,7 +609,7 @@ template <class T, int KIND> __global__ void __launch_bounds__(256) join_kernel(
 }
 
 // ----------------------------------------------------------------------------------------------------------------------------------- backward
-// behind the gate: dO = dout * gate, dgate = dout * O, delta = sum_d dO * O.  One wave per row.
+// behind the gate: dO = dout * gate, dgate = dout * O, delta = sum_d dO * O.  LANES lanes a row; bound by HBM.
 template <class T> struct GateArgs {
     const T *dout, *gate, *o;
     long long gs[3];
@@ -616,16 +618,16 @@ template <class T> struct GateArgs {
     long long rows;
     int Lq, H, dv;
 };
-template <class T> __global__ void __launch_bounds__(256) gate_bwd_kernel(const GateArgs<T> p)
+template <class T, int LANES> __global__ void __launch_bounds__(256) gate_bwd_kernel(const GateArgs<T> p)
 {
     using V4 = typename Ty<T>::V4;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+    const long long row = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES;
     if (row >= p.rows) return;
     const long long bi = row / p.H;
     const T *gp = p.gate ? p.gate + (bi / p.Lq) * p.gs[0] + (bi % p.Lq) * p.gs[1] + (row % p.H) * p.gs[2] : nullptr;
     float d = 0.f;
-    for (int c = lane * 4; c < p.dv; c += 256) {
+    for (int c = lane * 4; c < p.dv; c += LANES * 4) {
         const V4 du = *reinterpret_cast<const V4 *>(p.dout + row * p.dv + c), o = *reinterpret_cast<const V4 *>(p.o + row * p.dv + c);
         V4 a, b;
         if (gp) {
@@ -644,7 +646,7 @@ template <class T> __global__ void __launch_bounds__(256) gate_bwd_kernel(const 
         }
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) d += __shfl_xor(d, o);
+    for (int o = LANES / 2; o > 0; o >>= 1) d += __shfl_xor(d, o);
     if (p.delta && lane == 0) p.delta[row] = d;
 }
 
@@ -699,7 +701,7 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
     const int b = id % p.B; id /= p.B;
     const int hk = id % p.Hk; id /= p.Hk;
     const int ch = id % p.nchunk; id /= p.nchunk;
-    const int G = p.H / p.Hk, h = hk * G + id % G, rt = p.nrow - 1 - id / G;
+    const int G = p.H / p.Hk, h = hk * G + id % G, rt = row_tile(p, id / G);
     const int q0 = row_start(p, b), c0 = ch * DVC, cend = p.dv - c0;
     int ke = key_end(p, b);
     if (p.causal) ke = min(ke, min(p.Lq, rt * BM + BM) - 1 + q0 + 1);

@@ -95,26 +95,38 @@ static __global__ void __launch_bounds__(256) db_rows_kernel(const float *part, 
         out[(long long)blockIdx.x * TW + t] = x;
     }
 }
-template <class T> __global__ void __launch_bounds__(256) db_buckets_kernel(const float *part, const int *bucket_of, void *dtable, int H, int TW, int nb, int f32)
+template <class T> __global__ void __launch_bounds__(1024) db_buckets_kernel(const float *part, const int *bucket_of, void *dtable, int H, int TW, int nb, int f32)
 {
     extern __shared__ float sums[];
+    __shared__ float quarter[4][256];
     int *bk = reinterpret_cast<int *>(sums + TW);
-    const int h = blockIdx.x;
-    for (int t = threadIdx.x; t < TW; t += 256) {
+    const int h = blockIdx.x, lane = threadIdx.x & 255, q = threadIdx.x >> 8;
+    for (int t0 = 0; t0 < TW; t0 += 256) {
+        const int t = t0 + lane;
         float x = 0.f;
-#pragma unroll 16
-        for (int s = 0; s < DB_SPLITS; ++s) x += part[((long long)h * DB_SPLITS + s) * TW + t];
-        sums[t] = x;
-        const int b = bucket_of[t];
-        bk[t] = b < 0 ? 0 : (b >= nb ? nb - 1 : b);
+        if (t < TW)
+#pragma unroll
+            for (int s = 0; s < DB_SPLITS / 4; ++s) x += part[((long long)h * DB_SPLITS + q * (DB_SPLITS / 4) + s) * TW + t];
+        quarter[q][lane] = x;
+        __syncthreads();
+        if (q == 0 && t < TW) {
+            sums[t] = quarter[0][lane] + quarter[1][lane] + quarter[2][lane] + quarter[3][lane];
+            const int b = bucket_of[t];
+            bk[t] = b < 0 ? 0 : (b >= nb ? nb - 1 : b);
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    for (int b = threadIdx.x; b < nb; b += 256) {
+    for (int b0 = 0; b0 < nb; b0 += 64) {                             // 16 lanes a bucket
+        const int b = b0 + (threadIdx.x >> 4);
         float x = 0.f;
-#pragma unroll 16
-        for (int t = 0; t < TW; ++t) x += bk[t] == b ? sums[t] : 0.f;
-        if (f32) reinterpret_cast<float *>(dtable)[(long long)b * H + h] = x;
-        else reinterpret_cast<T *>(dtable)[(long long)b * H + h] = (T)x;
+#pragma unroll 4
+        for (int t = threadIdx.x & 15; t < TW; t += 16) x += bk[t] == b ? sums[t] : 0.f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) x += __shfl_xor(x, o);
+        if (b < nb && (threadIdx.x & 15) == 0) {
+            if (f32) reinterpret_cast<float *>(dtable)[(long long)b * H + h] = x;
+            else reinterpret_cast<T *>(dtable)[(long long)b * H + h] = (T)x;
+        }
     }
 }
 
@@ -138,6 +150,12 @@ template <class T, int KIND, int DK, int MT, int NT, int WM, int WN> int launch_
     if constexpr (WN > 1)                                           // (one tile of keys: a second buffer would only keep other workgroups off the CU)
         if (a.Lk <= KT) return launch(fwd_kernel<T, KIND, DK, MT, NT, WM, WN, KT, true>, blocks, 64 * WM * WN, fixed, smem, a, st);
     return launch(fwd_kernel<T, KIND, DK, MT, NT, WM, WN, KT, false>, blocks, 64 * WM * WN, 2 * fixed, smem, a, st);
+}
+// Causal walks differ in length.  Between one and two workgroups a CU, all are resident at once, and the CU that holds the i-th of the first 256 is taken to
+// hold the i-th behind them: those come shortest first, so that the longest walk shares its CU with the shortest.
+inline int snake_from(const Args &a, long long walks, int nrow)
+{
+    return a.causal && walks * nrow > 256 && walks * nrow <= 512 && 256 % walks == 0 ? (int)(256 / walks) : nrow;
 }
 template <class T, int KIND, int DK> int pick_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
 {
@@ -163,6 +181,7 @@ template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
 {
     const FwdPlan f = plan_forward(a, sizeof(T));
     a.fold = f.fold; a.nrow = f.nrow; a.nchunk = f.nchunk; a.nsplit = f.nsplit; a.split_keys = f.split_keys;
+    a.snake = snake_from(a, (long long)a.B * f.heads * f.nchunk * f.nsplit, f.nrow);
     const long long rows = (long long)a.B * a.Lq * a.H;
     a.part = reinterpret_cast<float *>(ws);
     a.ml = a.part + (f.nsplit > 1 ? rows * a.dv * f.nsplit : 0);
@@ -197,6 +216,7 @@ template <class T, int KIND, int DK, int DVC> int pick_bwd(Args a, const BwdPlan
     a.nchunk = f.nchunk;
     a.nparts = f.nparts;
     a.nrow = f.nrow_q;
+    a.snake = snake_from(a, (long long)a.B * a.H * f.nchunk, f.nrow_q);
     int rc = f.w_q == 1 ? launch_dq<T, KIND, DK, DVC, 1>(a, f, st) : (f.w_q == 2 ? launch_dq<T, KIND, DK, DVC, 2>(a, f, st) : launch_dq<T, KIND, DK, DVC, 4>(a, f, st));
     if (rc != TLK_OK) return rc;
     a.nrow = f.nrow_k;
@@ -224,8 +244,11 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
         ga.dgate = reinterpret_cast<T *>(io.dgate);
         ga.delta = kind == SOFTMAX ? reinterpret_cast<float *>(ws + w.delta) : nullptr;
         ga.rows = rows; ga.Lq = a.Lq; ga.H = a.H; ga.dv = a.dv;
-        if ((rows + 3) / 4 > 0x7fffffffLL) return fail(TLK_EINVAL, "tlk_gau_attention: more than 2^31 - 1 workgroups");
-        hipLaunchKernelGGL(gate_bwd_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, ga);
+        const int lanes = a.dv <= 64 ? 16 : (a.dv <= 128 ? 32 : 64);
+        const long long blocks = (rows + 256 / lanes - 1) / (256 / lanes);
+        if (blocks > 0x7fffffffLL) return fail(TLK_EINVAL, "tlk_gau_attention: more than 2^31 - 1 workgroups");
+        const auto kernel = lanes == 16 ? gate_bwd_kernel<T, 16> : (lanes == 32 ? gate_bwd_kernel<T, 32> : gate_bwd_kernel<T, 64>);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, ga);
         TLK_HIP(hipGetLastError());
         if (a.gate) a.dO = ws + w.dO;
         a.delta = ga.delta;
@@ -251,7 +274,7 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
         const int TW = 2 * a.D + 1;
         float *p2 = reinterpret_cast<float *>(ws + w.db2);
         hipLaunchKernelGGL(db_rows_kernel, dim3((unsigned)(a.H * DB_SPLITS)), dim3(256), 0, st, a.db_part, p2, f.nr, TW);
-        hipLaunchKernelGGL(db_buckets_kernel<T>, dim3((unsigned)a.H), dim3(256), (size_t)TW * 8, st, p2, a.bucket_of, io.dtable, a.H, TW, a.nb, a.table_f32);
+        hipLaunchKernelGGL(db_buckets_kernel<T>, dim3((unsigned)a.H), dim3(1024), (size_t)TW * 8, st, p2, a.bucket_of, io.dtable, a.H, TW, a.nb, a.table_f32);
         TLK_HIP(hipGetLastError());
     }
     return TLK_OK;

@@ -19,7 +19,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
 
 enum { NONE = TLK_NORM_NONE, SCALE = TLK_NORM_SCALE, RMS = TLK_NORM_RMS, LAYER = TLK_NORM_LAYER };
-enum { A_RS, A_GATE, A_W1, A_B1, A_W2, A_B2, N_ACC };
+enum { A_RS, A_W1, A_W2, A_GATE, A_B1, A_B2, N_ACC };        // (the first three: every kind of norm)
 
 struct NormArgs {
     const void *h, *x, *gate, *rs, *w1, *b1, *w2, *b2, *dy, *dz;
@@ -31,31 +31,42 @@ struct NormArgs {
     float *part;                     // (workgroup, array, d)
     int groups, per_group;           // workgroups: `per_group` for each of `groups` runs of rows_in_group rows
     long long rows_in_group;
-    int slot[N_ACC], nacc;           // which arrays are kept, and where
+    int slot[N_ACC], scalar[N_ACC], nacc;           // which arrays are kept, and where; which are one sum over all columns
 };
 
 // E = NV * V values a lane; value e of lane t sits in column (e / V * LPR + t) * V + e % V
 template <class T, int LPR, int NV, int V> struct Row {
     static constexpr int E = NV * V;
     static __device__ __forceinline__ int col(int e, int t) { return ((e / V) * LPR + t) * V + e % V; }
-    static __device__ __forceinline__ void load(const void *base, long long off, int d, int t, float (&r)[E], float pad = 0.f)
+    // as it stands in memory (zero behind the row), and widened
+    struct Raw {
+        struct __attribute__((aligned(V == 1 ? sizeof(T) : 16))) { T el[V]; } v[NV];
+    };
+    static __device__ __forceinline__ void fetch(const void *base, long long off, int d, int t, Raw &r)
     {
         const T *p = reinterpret_cast<const T *>(base) + off;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = (v * LPR + t) * V;
             if constexpr (V == 1) {
-                r[v] = c < d ? (float)p[c] : pad;
+                r.v[v].el[0] = c < d ? p[c] : (T)0.f;
             } else {
                 u4 raw = {0, 0, 0, 0};
-                const bool in = c < d;
-                if (in) raw = *reinterpret_cast<const u4 *>(p + c);
-                T el[V];
-                __builtin_memcpy(el, &raw, 16);
-#pragma unroll
-                for (int i = 0; i < V; ++i) r[v * V + i] = in ? (float)el[i] : pad;
+                if (c < d) raw = *reinterpret_cast<const u4 *>(p + c);
+                __builtin_memcpy(&r.v[v], &raw, 16);
             }
         }
+    }
+    static __device__ __forceinline__ void widen(const Raw &r, float (&x)[E])
+    {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = (float)r.v[e / V].el[e % V];
+    }
+    static __device__ __forceinline__ void load(const void *base, long long off, int d, int t, float (&x)[E])
+    {
+        Raw r;
+        fetch(base, off, d, t, r);
+        widen(r, x);
     }
     static __device__ __forceinline__ void store(void *base, long long off, int d, int t, const float (&r)[E])
     {
@@ -230,9 +241,13 @@ template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(256
     if (live_row) R::store(p.z, row * p.d, p.d, t, v);
 }
 
-constexpr int BT = 512;                                                  // threads of a backward workgroup: one per CU, rows in turn
+// One backward workgroup of 512 threads per CU walks rows in turn, 512 / LPR of them at a time.  The next rows' five tensors are fetched while the present
+// ones pass their four reductions: a lane holds 8 values of a row (16 of the widest), so that its sums and two rows' data fit the registers.
+constexpr int BT = 512;
 
-template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(BT) joint_bwd_kernel(const NormArgs p)
+// LEAN: no layer norm and no shared gate, so only res_scale and the two weights have column sums -- half the registers of a lane's sums, which is what
+// lets the rows' loads stay in flight (4096 columns bf16: with all six arrays the sums spilled, 674 us; lean 0 bytes spilled)
+template <class T, int LPR, int NV, int V, bool LEAN> __global__ void __attribute__((amdgpu_flat_work_group_size(BT, BT), amdgpu_waves_per_eu(2, 2))) joint_bwd_kernel(const NormArgs p)
 {
     using R = Row<T, LPR, NV, V>;
     constexpr int E = R::E, SLOTS = BT / LPR;
@@ -244,24 +259,36 @@ template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(BT)
     bool in[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) in[e] = R::col(e, t) < p.d;
-    float acc[N_ACC][E];
+    constexpr int NA = LEAN ? 3 : N_ACC;
+    float acc[NA][E];
 #pragma unroll
-    for (int a = 0; a < N_ACC; ++a)
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[a][e] = 0.f;
     const long long step = (long long)p.per_group * SLOTS;
+    typename R::Raw fh, fx, fg, fy, fz;
+    const auto fetch = [&](long long r0) __attribute__((always_inline)) {
+        const long long row = first + (r0 + slot < p.rows_in_group ? r0 + slot : r0);
+        R::fetch(p.h, row * p.hs, p.d, t, fh);
+        if (p.x) R::fetch(p.x, row * p.xs, p.d, t, fx);
+        if (p.gate) R::fetch(p.gate, row / p.per_gate * p.gs, p.d, t, fg);
+        if (p.dy) R::fetch(p.dy, row * p.d, p.d, t, fy);
+        if (p.dz) R::fetch(p.dz, row * p.d, p.d, t, fz);
+    };
+    if (in_grp * SLOTS < p.rows_in_group) fetch(in_grp * SLOTS);
     for (long long r0 = in_grp * SLOTS; r0 < p.rows_in_group; r0 += step) {            // (uniform over the workgroup: the reductions hold barriers)
         const bool live = r0 + slot < p.rows_in_group;
         const long long row = first + (live ? r0 + slot : r0);
         float h[E], x[E], gt[E], dy[E], dz[E], w[E];
-        R::load(p.h, row * p.hs, p.d, t, h);
-        if (p.x) R::load(p.x, row * p.xs, p.d, t, x);
-        if (p.gate) R::load(p.gate, row / p.per_gate * p.gs, p.d, t, gt);
-        if (p.dy) R::load(p.dy, row * p.d, p.d, t, dy);
+        R::widen(fh, h);
+        if (p.x) R::widen(fx, x);
+        if (p.gate) R::widen(fg, gt);
+        if (p.dy) R::widen(fy, dy);
         else
 #pragma unroll
             for (int e = 0; e < E; ++e) dy[e] = 0.f;
-        if (p.dz) R::load(p.dz, row * p.d, p.d, t, dz);
+        if (p.dz) R::widen(fz, dz);
+        if (r0 + step < p.rows_in_group) fetch(r0 + step);
         float hat1[E], n1[E], live1, live2, inv2 = 1.f;
         const float inv1 = normalise<E>(p.n1, h, hat1, in, p.d, p.eps1, sum, live1);
         load_weight<R, T>(p.n1, p.w1, p.d, t, w);
@@ -290,7 +317,7 @@ template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(BT)
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     acc[A_W2][e] = __builtin_fmaf(dz[e], hat2[e], acc[A_W2][e]);
-                    acc[A_B2][e] += dz[e];
+                    if constexpr (!LEAN) acc[A_B2][e] += dz[e];
                 }
             }
             float w2[E];
@@ -320,7 +347,8 @@ template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(BT)
                 if (live && p.dgate) R::store(p.dgate, row * p.d, p.d, t, dg);
             } else if (live) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) acc[A_GATE][e] += dg[e];
+                for (int e = 0; e < E; ++e)
+                    if constexpr (!LEAN) acc[A_GATE][e] += dg[e];
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) dy[e] *= gt[e];
@@ -329,7 +357,7 @@ template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(BT)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 acc[A_W1][e] = __builtin_fmaf(dy[e], hat1[e], acc[A_W1][e]);
-                acc[A_B1][e] += dy[e];
+                if constexpr (!LEAN) acc[A_B1][e] += dy[e];
             }
         }
 #pragma unroll
@@ -340,10 +368,25 @@ template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(BT)
     // the workgroup's column sums: its row slots joined in LDS, one array after the other
     const int CW = LPR * E;
 #pragma unroll
-    for (int a = 0; a < N_ACC; ++a) {
+    for (int a = 0; a < NA; ++a) {
         if (p.slot[a] < 0) continue;
         float *dst = p.part + ((long long)blockIdx.x * p.nacc + p.slot[a]) * p.d;
         __syncthreads();
+        if (p.scalar[a]) {                                               // ScaleNorm's one weight: over the columns as well
+            float v = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v += acc[a][e];
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+            if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                v = 0.f;
+                for (int i = 0; i < BT / 64; ++i) v += lds[i];
+                dst[0] = v;
+            }
+            continue;
+        }
 #pragma unroll
         for (int e = 0; e < E; ++e) lds[slot * CW + R::col(e, t)] = acc[a][e];
         __syncthreads();
@@ -360,38 +403,31 @@ struct ColArgs {
     void *out[N_ACC];
     int slot[N_ACC], scalar[N_ACC], d, nacc, groups, per_group;
 };
-// adds the workgroups' column sums: 64 columns x 4 runs of workgroups a block; ScaleNorm's one weight is summed over the columns as well
-template <class T> __global__ void __launch_bounds__(256) joint_cols_kernel(const ColArgs p)
+// adds the workgroups' column sums in a fixed order: 64 columns x 16 runs of workgroups a block
+constexpr int CR = 16;
+template <class T> __global__ void __launch_bounds__(64 * CR) joint_cols_kernel(const ColArgs p)
 {
-    __shared__ float s[4][64];
+    __shared__ float s[CR][64];
     const int a = blockIdx.y, cg = threadIdx.x & 63, rg = threadIdx.x >> 6;
-    if (p.slot[a] < 0) return;
+    if (p.slot[a] < 0 || (p.scalar[a] && blockIdx.x > 0)) return;
     const bool per_gate = a == A_GATE;
     const int ng = per_gate ? p.groups : 1, nb = per_gate ? p.per_group : p.groups * p.per_group;
     if ((int)blockIdx.z >= ng) return;
-    const int first = blockIdx.z * nb, share = (nb + 3) / 4, b0 = rg * share, b1 = min(nb, b0 + share);
-    float total = 0.f;
-    for (int c0 = p.scalar[a] ? 0 : (int)blockIdx.x * 64; c0 < p.d; c0 += 64) {
-        const int c = c0 + cg;
-        float v = 0.f;
-        if (c < p.d)
-            for (int b = b0; b < b1; ++b) v += p.part[((long long)(first + b) * p.nacc + p.slot[a]) * p.d + c];
-        total += v;
-        if (!p.scalar[a]) break;
+    const int first = blockIdx.z * nb, share = (nb + CR - 1) / CR, b0 = rg * share, b1 = min(nb, b0 + share), c = blockIdx.x * 64 + cg, cols = p.scalar[a] ? 1 : p.d;
+    float v = 0.f;
+    if (c < cols) {
+        const float *src = p.part + ((long long)first * p.nacc + p.slot[a]) * p.d + c;
+        const long long bs = (long long)p.nacc * p.d;
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) v += src[b * bs];
     }
-    if (p.scalar[a] && blockIdx.x > 0) return;                             // (uniform over the block)
-    s[rg][cg] = total;
+    s[rg][cg] = v;
     __syncthreads();
-    if (rg) return;
-    float v = s[0][cg] + s[1][cg] + s[2][cg] + s[3][cg];
-    if (p.scalar[a]) {
+    if (rg || c >= cols) return;
+    v = 0.f;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-        if (cg == 0) *reinterpret_cast<T *>(p.out[a]) = (T)v;
-        return;
-    }
-    const int c = blockIdx.x * 64 + cg;
-    if (c < p.d) reinterpret_cast<T *>(p.out[a])[(long long)blockIdx.z * p.d + c] = (T)v;
+    for (int i = 0; i < CR; ++i) v += s[i][cg];
+    reinterpret_cast<T *>(p.out[a])[(long long)blockIdx.z * p.d + c] = (T)v;
 }
 
 template <class T, int LPR, int NV, int V> int fwd_launch(const NormArgs &a, hipStream_t st)
@@ -405,33 +441,52 @@ template <class T, int LPR, int NV, int V> int fwd_launch(const NormArgs &a, hip
 template <class T, int LPR, int NV, int V> int bwd_launch(const NormArgs &a, hipStream_t st)
 {
     const size_t smem = (size_t)BT * NV * V * sizeof(float);
-    if (smem > 48 * 1024) TLK_HIP(hipFuncSetAttribute((const void *)joint_bwd_kernel<T, LPR, NV, V>, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
-    hipLaunchKernelGGL((joint_bwd_kernel<T, LPR, NV, V>), dim3((unsigned)(a.groups * a.per_group)), dim3(BT), smem, st, a);
+    const bool lean = a.slot[A_GATE] < 0 && a.slot[A_B1] < 0 && a.slot[A_B2] < 0;
+    const auto kernel = lean ? joint_bwd_kernel<T, LPR, NV, V, true> : joint_bwd_kernel<T, LPR, NV, V, false>;
+    if (smem > 48 * 1024) TLK_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.groups * a.per_group)), dim3(BT), smem, st, a);
     TLK_HIP(hipGetLastError());
     return TLK_OK;
 }
 
-// lanes a row: enough that a lane holds at most 16 values (8192 columns in float32: 32)
-template <class T> int pick(const NormArgs &a, bool vec, bool bwd, hipStream_t st)
+// lanes a row: forward at most 16 values a lane (8192 columns of float32: 32), backward 8 (16)
+template <class T> int pick_fwd(const NormArgs &a, bool vec, hipStream_t st)
 {
     constexpr int V = 16 / sizeof(T);
-#define GO(L, N, W) (bwd ? bwd_launch<T, L, N, W>(a, st) : fwd_launch<T, L, N, W>(a, st))
     if (vec) {
         const int v = (a.d + V - 1) / V;                                   // 16-byte vectors of a row
-        if (v <= 32) return GO(32, 1, V);
-        if (v <= 64) return GO(64, 1, V);
-        if (v <= 128) return GO(64, 2, V);
-        if (v <= 256) return GO(256, 1, V);
-        if (v <= 512) return GO(256, 2, V);
-        if (v <= 1024) return GO(256, 4, V);
-        if constexpr (V == 4) return GO(256, 8, V);
+        if (v <= 32) return fwd_launch<T, 32, 1, V>(a, st);
+        if (v <= 64) return fwd_launch<T, 64, 1, V>(a, st);
+        if (v <= 128) return fwd_launch<T, 64, 2, V>(a, st);
+        if (v <= 256) return fwd_launch<T, 256, 1, V>(a, st);
+        if (v <= 512) return fwd_launch<T, 256, 2, V>(a, st);
+        if (v <= 1024) return fwd_launch<T, 256, 4, V>(a, st);
+        if constexpr (V == 4) return fwd_launch<T, 256, 8, V>(a, st);
         return fail(TLK_EINVAL, "tlk_norm_gate_residual: more than 8192 columns");
     }
-    if (a.d <= 256) return GO(64, 4, 1);
-    if (a.d <= 1024) return GO(64, 16, 1);
-    if (a.d <= 4096) return GO(256, 16, 1);
-    return GO(256, 32, 1);
-#undef GO
+    if (a.d <= 256) return fwd_launch<T, 64, 4, 1>(a, st);
+    if (a.d <= 1024) return fwd_launch<T, 64, 16, 1>(a, st);
+    if (a.d <= 4096) return fwd_launch<T, 256, 16, 1>(a, st);
+    return fwd_launch<T, 256, 32, 1>(a, st);
+}
+template <class T> int pick_bwd(const NormArgs &a, bool vec, hipStream_t st)
+{
+    constexpr int V = 16 / sizeof(T);
+    if (vec) {
+        const int v = (a.d + V - 1) / V;
+        if (v <= 32) return bwd_launch<T, 32, 1, V>(a, st);
+        if (v <= 64) return bwd_launch<T, 64, 1, V>(a, st);
+        if (v <= 128) return bwd_launch<T, 128, 1, V>(a, st);
+        if (v <= 256) return bwd_launch<T, 256, 1, V>(a, st);
+        if (v <= 512) return bwd_launch<T, 512, 1, V>(a, st);
+        if (v <= 1024) return bwd_launch<T, 512, 2, V>(a, st);
+        if constexpr (V == 4) return bwd_launch<T, 512, 4, V>(a, st);
+        return fail(TLK_EINVAL, "tlk_norm_gate_residual: more than 8192 columns");
+    }
+    if (a.d <= 256) return bwd_launch<T, 64, 4, 1>(a, st);
+    if (a.d <= 1024) return bwd_launch<T, 128, 8, 1>(a, st);
+    if (a.d <= 4096) return bwd_launch<T, 512, 8, 1>(a, st);
+    return bwd_launch<T, 512, 16, 1>(a, st);
 }
 
 // 256 workgroups walk the rows (one per CU); a shared gate's gradient is kept per run of rows, so every run gets workgroups of its own
@@ -440,7 +495,7 @@ void cut(const tlk_norm_args *a, NormArgs &n)
     const long long groups = a->gate && a->gate_rows > 1 ? (a->rows + a->gate_rows - 1) / a->gate_rows : 1;
     n.groups = (int)(groups < 1 ? 1 : groups);
     n.rows_in_group = a->rows / n.groups;
-    const int slots = a->dim <= 256 ? 16 : 2;
+    const int slots = a->dim <= 512 ? 8 : (a->dim <= 2048 ? 2 : 1);
     long long per = (256 + n.groups - 1) / n.groups, most = (n.rows_in_group + slots - 1) / slots;
     n.per_group = (int)(per < most ? per : (most < 1 ? 1 : most));
 }
@@ -509,8 +564,8 @@ extern "C" int tlk_norm_gate_residual_fwd(const tlk_norm_args *a, void *y_dev, v
     n.y = y_dev; n.z = z_dev;
     const bool vec = vector_rows(a, {y_dev, z_dev});
     hipStream_t st = (hipStream_t)hip_stream;
-    if (a->dtype == TLK_F32) return pick<float>(n, vec, false, st);
-    return a->dtype == TLK_F16 ? pick<_Float16>(n, vec, false, st) : pick<__bf16>(n, vec, false, st);
+    if (a->dtype == TLK_F32) return pick_fwd<float>(n, vec, st);
+    return a->dtype == TLK_F16 ? pick_fwd<_Float16>(n, vec, st) : pick_fwd<__bf16>(n, vec, st);
 }
 
 extern "C" long long tlk_norm_gate_residual_workspace(const tlk_norm_args *a)
@@ -533,7 +588,8 @@ extern "C" int tlk_norm_gate_residual_bwd(const tlk_norm_args *a, const void *dy
     if (dz_dev && a->next_norm == TLK_NORM_NONE) return fail(TLK_EINVAL, "tlk_norm_gate_residual_bwd: a gradient of z without the next norm");
     int slot[N_ACC];
     const int nacc = arrays(a, slot);
-    void *out[N_ACC] = {g->dres_scale, g->dgate, g->dweight, g->dbias, g->dnext_weight, g->dnext_bias};
+    void *out[N_ACC];
+    out[A_RS] = g->dres_scale; out[A_GATE] = g->dgate; out[A_W1] = g->dweight; out[A_B1] = g->dbias; out[A_W2] = g->dnext_weight; out[A_B2] = g->dnext_bias;
     for (int i = 0; i < N_ACC; ++i)
         if (slot[i] >= 0 && !out[i]) return fail(TLK_EINVAL, "tlk_norm_gate_residual_bwd: a parameter's gradient has no place");
     if (a->rows > 0 && (!g->dh || (a->x && !g->dx) || (a->gate && !g->dgate))) return fail(TLK_EINVAL, "tlk_norm_gate_residual_bwd: a gradient has no place");
@@ -546,17 +602,19 @@ extern "C" int tlk_norm_gate_residual_bwd(const tlk_norm_args *a, const void *dy
     n.part = reinterpret_cast<float *>(workspace_dev);
     n.nacc = nacc;
     memcpy(n.slot, slot, sizeof(slot));
+    n.scalar[A_W1] = a->norm == TLK_NORM_SCALE;
+    n.scalar[A_W2] = a->next_norm == TLK_NORM_SCALE;
     const bool vec = vector_rows(a, {dy_dev, dz_dev, g->dh, g->dx, n.dgate});
     hipStream_t st = (hipStream_t)hip_stream;
-    const int rb = a->dtype == TLK_F32 ? pick<float>(n, vec, true, st) : (a->dtype == TLK_F16 ? pick<_Float16>(n, vec, true, st) : pick<__bf16>(n, vec, true, st));
+    const int rb = a->dtype == TLK_F32 ? pick_bwd<float>(n, vec, st) : (a->dtype == TLK_F16 ? pick_bwd<_Float16>(n, vec, st) : pick_bwd<__bf16>(n, vec, st));
     if (rb != TLK_OK || !nacc) return rb;
     ColArgs c;
     c.part = n.part; c.d = n.d; c.nacc = nacc; c.groups = n.groups; c.per_group = n.per_group;
-    for (int i = 0; i < N_ACC; ++i) { c.out[i] = out[i]; c.slot[i] = slot[i]; c.scalar[i] = (i == A_W1 && a->norm == TLK_NORM_SCALE) || (i == A_W2 && a->next_norm == TLK_NORM_SCALE); }
+    for (int i = 0; i < N_ACC; ++i) { c.out[i] = out[i]; c.slot[i] = slot[i]; c.scalar[i] = n.scalar[i]; }
     const dim3 grid((unsigned)((n.d + 63) / 64), N_ACC, (unsigned)(slot[A_GATE] >= 0 ? n.groups : 1));
-    if (a->dtype == TLK_F32) hipLaunchKernelGGL(joint_cols_kernel<float>, grid, dim3(256), 0, st, c);
-    else if (a->dtype == TLK_F16) hipLaunchKernelGGL(joint_cols_kernel<_Float16>, grid, dim3(256), 0, st, c);
-    else hipLaunchKernelGGL(joint_cols_kernel<__bf16>, grid, dim3(256), 0, st, c);
+    if (a->dtype == TLK_F32) hipLaunchKernelGGL(joint_cols_kernel<float>, grid, dim3(64 * CR), 0, st, c);
+    else if (a->dtype == TLK_F16) hipLaunchKernelGGL(joint_cols_kernel<_Float16>, grid, dim3(64 * CR), 0, st, c);
+    else hipLaunchKernelGGL(joint_cols_kernel<__bf16>, grid, dim3(64 * CR), 0, st, c);
     TLK_HIP(hipGetLastError());
     return TLK_OK;
 }
