@@ -12,7 +12,7 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
-#include "tlk_common.hpp"
+#include "tlk_lanes.hpp"
 
 namespace tlk {
 namespace gau {
@@ -257,8 +257,8 @@ __device__ __forceinline__ int row_start(const Args &p, int b)
     return s < -lim ? -lim : (s > lim ? lim : s);
 }
 
-__device__ __forceinline__ float over_groups_max(float x) { x = fmaxf(x, __shfl_xor(x, 16)); return fmaxf(x, __shfl_xor(x, 32)); }
-__device__ __forceinline__ float over_groups_sum(float x) { x += __shfl_xor(x, 16); return x + __shfl_xor(x, 32); }
+__device__ __forceinline__ float over_groups_max(float x) { return lanes_32<LaneMax>(lanes_16<LaneMax>(x)); }
+__device__ __forceinline__ float over_groups_sum(float x) { return lanes_32<LaneAdd>(lanes_16<LaneAdd>(x)); }
 __device__ __forceinline__ int wave_min_i(int x)
 {
 #pragma unroll
@@ -645,8 +645,7 @@ template <class T, int LANES> __global__ void __launch_bounds__(256) gate_bwd_ke
             for (int r = 0; r < 4; ++r) d += (float)du[r] * (float)o[r];
         }
     }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) d += __shfl_xor(d, o);
+    d = lanes_all<LaneAdd, LANES>(d);
     if (p.delta && lane == 0) p.delta[row] = d;
 }
 
@@ -867,8 +866,8 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         }
     }
     if (p.table) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) { lo += __shfl_xor(lo, o); hi += __shfl_xor(hi, o); }
+        lo = lanes_all<LaneAdd, 64>(lo);
+        hi = lanes_all<LaneAdd, 64>(hi);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");

@@ -9,7 +9,7 @@
 // launch adds the workgroups' sums in a fixed order: no atomics, equal bits on every run.
 #include <initializer_list>
 
-#include "tlk_common.hpp"
+#include "tlk_lanes.hpp"
 
 using namespace tlk;
 
@@ -36,7 +36,7 @@ struct NormArgs {
 
 // E = NV * V values a lane; value e of lane t sits in column (e / V * LPR + t) * V + e % V
 template <class T, int LPR, int NV, int V> struct Row {
-    static constexpr int E = NV * V;
+    static constexpr int E = NV * V, W = V;
     static __device__ __forceinline__ int col(int e, int t) { return ((e / V) * LPR + t) * V + e % V; }
     // as it stands in memory (zero behind the row), and widened
     struct Raw {
@@ -95,12 +95,11 @@ template <int LPR> struct Sum {
     int flip = 0;
     __device__ __forceinline__ float operator()(float v)
     {
-#pragma unroll
-        for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        v = lanes_all<LaneAdd, (LPR < 64 ? LPR : 64)>(v);
         if constexpr (LPR > 64) {
             const int w = threadIdx.x >> 6, n = blockDim.x >> 6, first = w / (LPR / 64) * (LPR / 64);
             if ((threadIdx.x & 63) == 0) s[flip * n + w] = v;
-            __syncthreads();
+            lds_barrier();
             v = 0.f;
 #pragma unroll
             for (int i = 0; i < LPR / 64; ++i) v += s[flip * n + first + i];
@@ -162,6 +161,17 @@ template <int E, class S> __device__ __forceinline__ void normalise_bwd(int kind
     for (int e = 0; e < E; ++e) t[e] = in[e] ? (t[e] - m) * inv - hat[e] * live * a : 0.f;
 }
 
+// a weight as it stands in memory (ScaleNorm: its one value everywhere; none: ones), for use row after row
+template <class R, class T> __device__ __forceinline__ void fetch_weight(int kind, const void *w, int d, int t, typename R::Raw &r)
+{
+    if (kind == RMS || kind == LAYER) {
+        R::fetch(w, 0, d, t, r);
+        return;
+    }
+    const T g = kind == SCALE ? *reinterpret_cast<const T *>(w) : (T)1.f;
+#pragma unroll
+    for (int e = 0; e < R::E; ++e) r.v[e / R::W].el[e % R::W] = g;
+}
 template <class R, class T> __device__ __forceinline__ void load_weight(int kind, const void *w, int d, int t, float (&r)[R::E])
 {
     if (kind == NONE || !w) {
@@ -275,6 +285,12 @@ template <class T, int LPR, int NV, int V, bool LEAN> __global__ void __attribut
         if (p.dy) R::fetch(p.dy, row * p.d, p.d, t, fy);
         if (p.dz) R::fetch(p.dz, row * p.d, p.d, t, fz);
     };
+    // weights first: loads return in order, and one behind the next rows' would wait for them
+    typename R::Raw rw1, rw2, rb1, rrs;
+    fetch_weight<R, T>(p.n1, p.w1, p.d, t, rw1);
+    fetch_weight<R, T>(p.n2, p.w2, p.d, t, rw2);
+    fetch_weight<R, T>(p.x && p.rs ? RMS : NONE, p.rs, p.d, t, rrs);
+    if (p.b1) R::fetch(p.b1, 0, p.d, t, rb1);
     if (in_grp * SLOTS < p.rows_in_group) fetch(in_grp * SLOTS);
     for (long long r0 = in_grp * SLOTS; r0 < p.rows_in_group; r0 += step) {            // (uniform over the workgroup: the reductions hold barriers)
         const bool live = r0 + slot < p.rows_in_group;
@@ -291,20 +307,17 @@ template <class T, int LPR, int NV, int V, bool LEAN> __global__ void __attribut
         if (r0 + step < p.rows_in_group) fetch(r0 + step);
         float hat1[E], n1[E], live1, live2, inv2 = 1.f;
         const float inv1 = normalise<E>(p.n1, h, hat1, in, p.d, p.eps1, sum, live1);
-        load_weight<R, T>(p.n1, p.w1, p.d, t, w);
+        R::widen(rw1, w);
 #pragma unroll
         for (int e = 0; e < E; ++e) n1[e] = hat1[e] * w[e];
         if (p.b1) {
             float b[E];
-            R::load(p.b1, 0, p.d, t, b);
+            R::widen(rb1, b);
 #pragma unroll
             for (int e = 0; e < E; ++e) n1[e] += b[e];
         }
         float rs[E];
-        if (p.x && p.rs) R::load(p.rs, 0, p.d, t, rs);
-        else
-#pragma unroll
-            for (int e = 0; e < E; ++e) rs[e] = 1.f;
+        R::widen(rrs, rs);
         if (p.dz) {
             float hat2[E], y[E];
 #pragma unroll
@@ -321,7 +334,7 @@ template <class T, int LPR, int NV, int V, bool LEAN> __global__ void __attribut
                 }
             }
             float w2[E];
-            load_weight<R, T>(p.n2, p.w2, p.d, t, w2);
+            R::widen(rw2, w2);
 #pragma unroll
             for (int e = 0; e < E; ++e) dz[e] *= w2[e];
             normalise_bwd<E>(p.n2, dz, hat2, in, p.d, inv2, live2, sum);
@@ -376,8 +389,7 @@ template <class T, int LPR, int NV, int V, bool LEAN> __global__ void __attribut
             float v = 0.f;
 #pragma unroll
             for (int e = 0; e < E; ++e) v += acc[a][e];
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+            v = lanes_all<LaneAdd, 64>(v);
             if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
             __syncthreads();
             if (threadIdx.x == 0) {
@@ -496,7 +508,7 @@ void cut(const tlk_norm_args *a, NormArgs &n)
     n.groups = (int)(groups < 1 ? 1 : groups);
     n.rows_in_group = a->rows / n.groups;
     const int slots = a->dim <= 512 ? 8 : (a->dim <= 2048 ? 2 : 1);
-    long long per = (256 + n.groups - 1) / n.groups, most = (n.rows_in_group + slots - 1) / slots;
+    long long per = n.groups < 256 ? 256 / n.groups : 1, most = (n.rows_in_group + slots - 1) / slots;
     n.per_group = (int)(per < most ? per : (most < 1 ? 1 : most));
 }
 int arrays(const tlk_norm_args *a, int (&slot)[N_ACC])
