@@ -841,7 +841,7 @@ int tlk_reid_part_head(const void *feat_dev, int feat_pix_stride, int dtype, int
  *   over the keys j < lens[b] (all len_k without lens; lens is clipped to 0..len_k) and, when causal, j <= i + start_b; start_b = q_start_dev[b],
  *   or q_start.  A row that sees no key gives zeros.  Keys at or behind lens[b] are not read.  Head h reads key / value head h / (heads / kv_heads).
  *   q (batch, len_q, heads, dim_k), k (batch, len_k, kv_heads, dim_k), v (.., dim_v), gate (batch, len_q, heads, dim_v): strides in elements for
- *   batch, row and head, the last dimension contiguous; every stride a multiple of 16 bytes, row strides at most 2^22 elements, every pointer 16-byte aligned; dim_k <= 128 and dim_v
+ *   batch, row and head, the last dimension contiguous; every stride a multiple of 16 bytes, row strides of q, k, v between the width and 2^22 elements, every pointer 16-byte aligned; dim_k <= 128 and dim_v
  *   multiples of 16 bytes of elements.  table (num_buckets, heads) of `dtype` or (table_f32) float32, bucket_of (2 * max_distance + 1) int32 (values are clipped to
  *   0..num_buckets - 1); num_buckets 0: no bias.  max_distance <= 2048.  out, o_raw, dq.. are contiguous (batch, len, heads, dim).
  *   o_raw (nullable): o before the gate, lse (nullable, softmax): log2 sum_j 2^(S log2 e) per (batch, len_q, heads), +inf for a row without keys: what

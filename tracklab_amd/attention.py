@@ -113,12 +113,12 @@ def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda
 def _fit(t, vn):
     """the tensor with a contiguous last dimension, 16-byte aligned rows and heads (as it is where it already has them), and its three strides"""
     s = t.stride()
-    if (t.shape[-1] > 1 and s[3] != 1) or t.data_ptr() % 16 or any(t.shape[i] > 1 and s[i] % vn for i in range(3)) or (t.shape[1] > 1 and s[1] > 1 << 22):
+    if (t.shape[-1] > 1 and s[3] != 1) or t.data_ptr() % 16 or any(t.shape[i] > 1 and s[i] % vn for i in range(3)) or (t.shape[1] > 1 and not t.shape[3] <= s[1] <= 1 << 22):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
         s = t.stride()
-    return t, tuple(s[i] if t.shape[i] > 1 else 0 for i in range(3))
+    return t, tuple(s[i] if t.shape[i] > 1 else (t.shape[3] if i == 1 else 0) for i in range(3))
 
 
 def _gau_args(q, k, v, gate, table, buckets, lens, q_start, kind, causal, scale):

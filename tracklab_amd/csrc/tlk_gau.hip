@@ -37,6 +37,8 @@ int fill(const tlk_gau_args *a, gau::Args &p, const char *fn)
         if (a->q_stride[i] % vn || a->k_stride[i] % vn || a->v_stride[i] % vn || (a->gate && a->gate_stride[i] % vn))
             return fail(TLK_EINVAL, f + ": strides must be multiples of 16 bytes");
         if (i == 1 && (a->q_stride[i] > 1 << 22 || a->k_stride[i] > 1 << 22 || a->v_stride[i] > 1 << 22)) return fail(TLK_EINVAL, f + ": row strides of q, k and v must not pass 2^22 elements");
+        if (i == 1 && ((a->len_q > 1 && a->q_stride[i] < a->dim_k) || (a->len_k > 1 && (a->k_stride[i] < a->dim_k || a->v_stride[i] < a->dim_v))))
+            return fail(TLK_EINVAL, f + ": row strides of q, k and v must not be below their widths");
         if (a->q_stride[i] < 0 || a->k_stride[i] < 0 || a->v_stride[i] < 0 || (a->gate && a->gate_stride[i] < 0)) return fail(TLK_EINVAL, f + ": strides must not be negative");
     }
     memset(&p, 0, sizeof(p));

@@ -106,22 +106,25 @@ template <class T, int ROWS, int COLS, int NW> struct Tile {
             off[i] = c * VN < cend ? (unsigned)(row * (int)rs * (int)sizeof(T) + c * 16) : OOB;
         }
     }
-    // `rows`: how many of the tile's rows there are (uniform); `base`: its first row (uniform)
-    __device__ __forceinline__ void load(const T *base, int rows, char *lds, int lane, const bool whole) const
+    // the buffer descriptor of the tile whose first row `base` is, with `rows` rows left (uniform): it ends with the last of them, so that the loads of the
+    // rows behind it return zeros by themselves (row strides are not below the width: host check)
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_at(const T *base, int rows, long long rs)
     {
-        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int inst = i * NW + wave;
-            if (ROWS * C / 64 % NW != 0 && inst >= ROWS * C / 64) break;
-            const unsigned o = whole || (inst * 64 + lane) / C < rows ? off[i] : OOB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + inst * 1024), 16, (int)o, 0, 0, 0);
-        }
+        const int n = rows < 0 ? 0 : (rows < ROWS ? rows : ROWS);
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, n * (int)rs * (int)sizeof(T), 0x00020000);
     }
-    __device__ __forceinline__ void issue(const T *base, int rows, char *lds, int lane) const
+    // the i-th of the wave's N loads
+    __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t &rsrc, char *lds, int i) const
     {
-        if (rows >= ROWS) load(base, rows, lds, lane, true);
-        else load(base, rows, lds, lane, false);
+        const int inst = i * NW + wave;
+        if (ROWS * C / 64 % NW != 0 && inst >= ROWS * C / 64) return;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + inst * 1024), 16, (int)off[i], 0, 0, 0);
+    }
+    __device__ __forceinline__ void issue(const T *base, int rows, long long rs, char *lds) const
+    {
+        const __amdgpu_buffer_rsrc_t rsrc = tile_at(base, rows, rs);
+#pragma unroll
+        for (int i = 0; i < N; ++i) load(rsrc, lds, i);
     }
     // Fragment reads.  A lane's place in the first fragment (row_at, col_at) is made once per tile and hidden from the optimiser; the place in any other is
     // one exclusive or with a constant (rows begin at multiples of the twisted field) plus a constant.  Left visible, all places of a tile are kept in
@@ -226,7 +229,6 @@ template <int N, int B, class V8, class Load, class Use> __device__ __forceinlin
         __builtin_amdgcn_sched_barrier(0);
     }
 }
-
 // The learned table over distances of head h, in LDS: -D .. D with MARGIN more entries of the end values on both sides, so that a tile that reaches
 // across +-D is looked up without clipping (a wave's tile spans fewer than MARGIN distances).  Softmax works in powers of two, so its bias carries
 // log2 e (finite values stay finite).
@@ -345,13 +347,10 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
     K += kb * p.ks[1];
     V += kb * p.vs[1];
     const long long kstep = KT * p.ks[1], vstep = KT * p.vs[1];
-    const auto issue = [&](int j, char *buf) __attribute__((always_inline)) {        // the tiles in turn: K and V move along
-        tk.issue(K, ke - j, buf, lane);
-        tv.issue(V, ke - j, buf + TK::BYTES, lane);
-        K += kstep;
-        V += vstep;
-    };
-    if (kb < ke) issue(kb, buf0);
+    if (kb < ke) {
+        tk.issue(K, ke - kb, p.ks[1], buf0);
+        tv.issue(V, ke - kb, p.vs[1], buf0 + TK::BYTES);
+    }
     if (p.table)
         for (int i = 0; i < GB; ++i) expand_bias<T, KIND>(p, h0 + i, tab + i * TW, NTH);
     int qi[MT], qh[MT], pos[MT];
@@ -406,7 +405,12 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
         fhi[mt] = p.table ? tab[qh[mt] * TW + TW - 1] : 0.f;
     }    const auto step = [&](const char *cur, char *next, int j0) __attribute__((always_inline)) {
         tiles_ready();                                             // this tile has landed, and the other buffer is free
-        if (!ONE && j0 + KT < ke) issue(j0 + KT, next);
+        K += kstep;
+        V += vstep;
+        if (!ONE) {                                                // the next tile's loads (behind the last tile they fetch nothing)
+            tk.issue(K, ke - j0 - KT, p.ks[1], next);
+            tv.issue(V, ke - j0 - KT, p.vs[1], next + TK::BYTES);
+        }
         if (pmin > pmax || (p.causal && j0 > pmax)) return;        // no row of this wave, or none that sees this tile (uniform over the wave)
         f4 s[MT][NS];
         constexpr int KS = DK / 32, BK = NS * KS < 4 ? NS * KS : 4, BV = NT < 4 ? NT : 4;
@@ -517,6 +521,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
             step(buf0, buf1, j0);
             if (j0 + KT < ke) step(buf1, buf0, j0 + KT);
         }
+        __builtin_amdgcn_s_waitcnt(0x0f70);                        // (vmcnt(0): nothing is on its way to LDS when the workgroup ends)
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -712,13 +717,10 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
     tk.init(w, lane, p.ks[1], p.dk);
     tv.init(w, lane, p.vs[1], cend);
     const long long kstep = KT * p.ks[1], vstep = KT * p.vs[1];
-    const auto issue = [&](int j, char *buf) __attribute__((always_inline)) {        // the tiles in turn: K and V move along
-        tk.issue(K, ke - j, buf, lane);
-        tv.issue(V, ke - j, buf + TK::BYTES, lane);
-        K += kstep;
-        V += vstep;
-    };
-    if (0 < ke) issue(0, buf0);
+    if (0 < ke) {
+        tk.issue(K, ke, p.ks[1], buf0);
+        tv.issue(V, ke, p.vs[1], buf0 + TK::BYTES);
+    }
     if (p.table) {
         expand_bias<T, KIND>(p, h, tab, NTH);
         for (int t = lane; t < NB; t += 64) dbw[t] = 0.f;
@@ -755,7 +757,12 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
     const float flo = p.table ? tab[0] : 0.f, fhi = p.table ? tab[TW - 1] : 0.f;          // the bias beyond +-D
     const auto step = [&](const char *cur, char *next, int j0) __attribute__((always_inline)) {
         tiles_ready();
-        if (!ONE && j0 + KT < ke) issue(j0 + KT, next);
+        K += kstep;
+        V += vstep;
+        if (!ONE) {
+            tk.issue(K, ke - j0 - KT, p.ks[1], next);
+            tv.issue(V, ke - j0 - KT, p.vs[1], next + TK::BYTES);
+        }
         if (i0 >= p.Lq || (p.causal && j0 > pmax)) return;
         const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin) && i0 + MT * 16 <= p.Lq;
         const int where = !p.table || j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3);
@@ -864,6 +871,7 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
             step(buf0, buf1, j0);
             if (j0 + KT < ke) step(buf1, buf0, j0 + KT);
         }
+        __builtin_amdgcn_s_waitcnt(0x0f70);                        // (vmcnt(0): nothing is on its way to LDS when the workgroup ends)
     }
     if (p.table) {
         lo = lanes_all<LaneAdd, 64>(lo);
@@ -959,10 +967,10 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         const T *dO = reinterpret_cast<const T *>(p.dO) + (((long long)b * p.Lq + ib) * p.H + h) * p.dv + c0;
         float ls0 = INFINITY, dl0 = 0.f;
         const auto issue = [&](int i, char *buf) __attribute__((always_inline)) {
-            tq.issue(Q, p.Lq - i, buf, lane);
-            to.issue(dO, p.Lq - i, buf + TQ::BYTES, lane);
-            Q += qstep;
-            dO += ostep;
+            if (buf) {
+                tq.issue(Q, p.Lq - i, p.qs[1], buf);
+                to.issue(dO, p.Lq - i, (long long)p.H * p.dv, buf + TQ::BYTES);
+            }
             if (KIND == SOFTMAX && tid < QT) {
                 const long long row = ((long long)b * p.Lq + i + tid) * p.H + h;
                 ls0 = i + tid < p.Lq ? p.lse[row] : INFINITY;
@@ -984,7 +992,13 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         const auto step = [&](const char *cur, float *st, char *next, int i0) __attribute__((always_inline)) {
             keep(st);
             tiles_ready();
-            if (!ONE && i0 + QT < p.Lq) issue(i0 + QT, next);
+            if (!ONE) issue(i0 + QT, nullptr);                     // (the statistics of the next tile)
+            Q += qstep;
+            dO += ostep;
+            if (!ONE) {
+                tq.issue(Q, p.Lq - i0 - QT, p.qs[1], next);
+                to.issue(dO, p.Lq - i0 - QT, (long long)p.H * p.dv, next + TQ::BYTES);
+            }
             const int pmin = i0 + q0, pmax = min(p.Lq, i0 + QT) - 1 + q0;
             if (jmax < jmin || (p.causal && jmin > pmax)) return;
             const bool full = i0 + QT <= p.Lq && j0 + MT * 16 <= ke && (!p.causal || j0 + MT * 16 - 1 <= pmin);
@@ -1083,6 +1097,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
                 step(buf0, stats0, buf1, i0);
                 if (i0 + QT < p.Lq) step(buf1, stats1, buf0, i0 + QT);
             }
+            __builtin_amdgcn_s_waitcnt(0x0f70);
         }
     }
 #pragma unroll
