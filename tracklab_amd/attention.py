@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import torch
 import torch.nn.functional as F
@@ -24,6 +25,7 @@ from torch.autograd.function import once_differentiable
 from ._lib import TlkError, _dtype_code, check, lib
 
 KINDS = {"relu2": 0, "softmax": 1}
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 NORMS = {None: 0, "none": 0, "scale": 1, "rms": 2, "layer": 3}
 
 
@@ -41,6 +43,13 @@ class NormArgs(C.Structure):
 
 class NormGrads(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("dh", "dx", "dgate", "dres_scale", "dweight", "dbias", "dnext_weight", "dnext_bias")]
+
+
+# the same structures as one pack each: a call is mostly this module's own time on small inputs, and a ctypes field costs as much as a torch query
+_GAU = struct.Struct("=14if4x12q8Q")
+_NORM = struct.Struct("=4i5q2f8Q")
+_GRADS = struct.Struct("=8Q")
+assert _GAU.size == C.sizeof(GauArgs) and _NORM.size == C.sizeof(NormArgs) and _GRADS.size == C.sizeof(NormGrads)
 
 
 def _bound():
@@ -63,7 +72,7 @@ def _need(ok, what):
 
 
 def _ptr(t):
-    return t.data_ptr() if t is not None else None
+    return t.data_ptr() if t is not None else 0
 
 
 def _bytes(n, dev):
@@ -112,54 +121,46 @@ def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda
 
 def _fit(t, vn):
     """the tensor with a contiguous last dimension, 16-byte aligned rows and heads (as it is where it already has them), and its three strides"""
-    s = t.stride()
-    if (t.shape[-1] > 1 and s[3] != 1) or t.data_ptr() % 16 or any(t.shape[i] > 1 and s[i] % vn for i in range(3)) or (t.shape[1] > 1 and not t.shape[3] <= s[1] <= 1 << 22):
+    n0, n1, n2, n3 = t.shape
+    s0, s1, s2, s3 = t.stride()
+    if (s3 != 1 and n3 > 1) or t.data_ptr() % 16 or (n0 > 1 and s0 % vn) or (n2 > 1 and s2 % vn) or (n1 > 1 and (s1 % vn or not n3 <= s1 <= 1 << 22)):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-        s = t.stride()
-    return t, tuple(s[i] if t.shape[i] > 1 else (t.shape[3] if i == 1 else 0) for i in range(3))
+        s0, s1, s2, s3 = t.stride()
+    return t, (s0 if n0 > 1 else 0, s1 if n1 > 1 else n3, s2 if n2 > 1 else 0)
 
 
 def _gau_args(q, k, v, gate, table, buckets, lens, q_start, kind, causal, scale):
-    """the filled argument structure and the tensors it points to"""
-    a = GauArgs()
+    """the packed argument structure and the tensors it points to"""
     vn = 4 if q.dtype == torch.float32 else 8
-    a.dtype, a.kind, a.causal = _dtype_code(q.dtype), kind, causal
-    a.batch, a.len_q, a.heads, a.dim_k = q.shape
-    a.len_k, a.kv_heads, a.dim_v = k.shape[1], k.shape[2], v.shape[3]
-    a.scale = scale
-    q, a.q_stride[:] = _fit(q, vn)
-    k, a.k_stride[:] = _fit(k, vn)
-    v, a.v_stride[:] = _fit(v, vn)
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    q, qs = _fit(q, vn)
+    k, ks = _fit(k, vn)
+    v, vs = _fit(v, vn)
+    gs = (0, 0, 0)
     if gate is not None:
-        gate, a.gate_stride[:] = _fit(gate, vn)
-        a.gate = gate.data_ptr()
-    if table is not None:
-        a.num_buckets, a.max_distance, a.table_f32 = table.shape[0], buckets.numel() // 2, table.dtype == torch.float32
-        a.table, a.bucket_of = table.data_ptr(), buckets.data_ptr()
-    if lens is not None:
-        a.lens = lens.data_ptr()
-    if isinstance(q_start, torch.Tensor):
-        a.q_start_dev = q_start.data_ptr()
-    else:
-        a.q_start = q_start
-    return a, (q, k, v, gate, table)
+        gate, gs = _fit(gate, vn)
+    B, Lq, H, dk = q.shape
+    _, Lk, Hk, dv = v.shape
+    start = isinstance(q_start, torch.Tensor)
+    a = _GAU.pack(_dtype_code(q.dtype), kind, causal, table is not None and table.dtype == torch.float32, B, Lq, Lk, H, Hk, dk, dv,
+                  table.shape[0] if table is not None else 0, buckets.numel() // 2 if table is not None else 0, 0 if start else q_start, scale, *qs, *ks, *vs, *gs,
+                  q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(gate), _ptr(table), _ptr(buckets), _ptr(lens), q_start.data_ptr() if start else 0)
+    return a, (q, k, v, gate)
 
 
 def _gau_forward(q, k, v, gate, table, buckets, lens, q_start, kind, causal, scale, keep):
     """out, and for the backward pass what it needs of (o before the gate, log-sum-exp)"""
     L, dev = _bound(), q.device
     a, held = _gau_args(q, k, v, gate, table, buckets, lens, q_start, kind, causal, scale)
-    shape = (a.batch, a.len_q, a.heads, a.dim_v)
+    shape = (*q.shape[:3], v.shape[3])
     out = torch.empty(shape, dtype=q.dtype, device=dev)
     o = torch.empty_like(out) if keep and gate is not None else None
     lse = torch.empty(shape[:3], dtype=torch.float32, device=dev) if keep and kind == 1 else None
     with _on(dev):
-        n = L.tlk_gau_attention_workspace(C.byref(a), 0)
+        n = L.tlk_gau_attention_workspace(a, 0) if k.shape[1] > 512 else 0            # (up to 512 keys a forward call needs none)
         ws = _bytes(n, dev)
-        check(L.tlk_gau_attention_fwd(C.byref(a), out.data_ptr(), _ptr(o), _ptr(lse), _ptr(ws), n, _stream(dev)))
+        check(L.tlk_gau_attention_fwd(a, out.data_ptr(), _ptr(o), _ptr(lse), _ptr(ws), n, _stream(dev)))
     return out, (o if gate is not None else (out if kind == 1 else None)), lse
 
 
@@ -184,9 +185,9 @@ class _GatedAttention(torch.autograd.Function):
         new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev) if t is not None else None      # noqa: E731
         dq, dk, dv, dgate, dtable = new(q), new(k), new(v), new(gate), new(table)
         with _on(dev):
-            n = L.tlk_gau_attention_workspace(C.byref(a), 1)
+            n = L.tlk_gau_attention_workspace(a, 1)
             ws = _bytes(n, dev)
-            check(L.tlk_gau_attention_bwd(C.byref(a), _ptr(dout), _ptr(o), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dgate), _ptr(dtable), _ptr(ws), n, _stream(dev)))
+            check(L.tlk_gau_attention_bwd(a, _ptr(dout), _ptr(o), _ptr(lse), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dgate), _ptr(dtable), _ptr(ws), n, _stream(dev)))
         return dq, dk, dv, dgate, dtable, None, None, None, None, None, None
 
 
@@ -206,36 +207,42 @@ def gated_attention(q, k, v, gate=None, *, kind="relu2", scale=None, bias=None, 
         _need(k.dim() == 3 and v.dim() == 3 and (gate is None or gate.dim() == 3), "gated_attention: q, k, v and gate must all have a head dimension, or none of them")
         q, k, v, gate = q.unsqueeze(2), k.unsqueeze(2), v.unsqueeze(2), gate.unsqueeze(2) if gate is not None else None
     _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "gated_attention: q, k and v must be (B, L, heads, d) or (B, L, d)")
-    _need(kind in KINDS, f"gated_attention: kind must be one of {sorted(KINDS)}")
+    _need(kind in KINDS, "gated_attention: kind must be 'relu2' or 'softmax'")
     B, Lq, H, dk = q.shape
-    Lk, Hk, dv = k.shape[1], k.shape[2], v.shape[3]
-    _need(q.is_cuda and q.dtype in (torch.float32, torch.float16, torch.bfloat16), "gated_attention: cuda tensors of float32, float16 or bfloat16 (no CPU fallback)")
-    _need(tuple(k.shape) == (B, Lk, Hk, dk) and tuple(v.shape) == (B, Lk, Hk, dv), "gated_attention: shapes of q, k and v do not go together")
+    _, Lk, Hk, dv = v.shape
+    dt, dev = q.dtype, q.device
+    _need(q.is_cuda and dt in _TYPES, "gated_attention: cuda tensors of float32, float16 or bfloat16 (no CPU fallback)")
+    _need(k.shape == (B, Lk, Hk, dk) and v.shape[0] == B, "gated_attention: shapes of q, k and v do not go together")
     _need(Hk > 0 and H > 0 and H % Hk == 0, "gated_attention: q's heads must be a multiple of k's")
     _need(1 <= dk <= 128 and dv >= 1, "gated_attention: 1 <= dk <= 128 and dv >= 1")
-    _need(gate is None or tuple(gate.shape) == (B, Lq, H, dv), "gated_attention: gate must have the result's shape")
+    _need(k.dtype == dt and v.dtype == dt and k.device == dev and v.device == dev, "gated_attention: q, k, v and gate must share type and device")
+    if gate is not None:
+        _need(gate.shape == (B, Lq, H, dv), "gated_attention: gate must have the result's shape")
+        _need(gate.dtype == dt and gate.device == dev, "gated_attention: q, k, v and gate must share type and device")
     _need((bias is None) == (buckets is None), "gated_attention: a bias needs its buckets")
-    for t in (k, v, gate):
-        _need(t is None or (t.dtype == q.dtype and t.device == q.device), "gated_attention: q, k, v and gate must share type and device")
     if bias is not None:
-        _need(bias.dim() == 2 and bias.shape[1] == H and bias.shape[0] > 0 and bias.dtype in (q.dtype, torch.float32) and bias.device == q.device,
+        _need(bias.dim() == 2 and bias.shape[1] == H and bias.shape[0] > 0 and (bias.dtype == dt or bias.dtype == torch.float32) and bias.device == dev,
               "gated_attention: bias must be (num_buckets, heads) of q's type or float32")
-        _need(buckets.dim() == 1 and buckets.numel() % 2 == 1 and buckets.numel() <= 4097 and buckets.dtype == torch.int32 and buckets.device == q.device,
+        _need(buckets.dim() == 1 and buckets.shape[0] % 2 == 1 and buckets.shape[0] <= 4097 and buckets.dtype == torch.int32 and buckets.device == dev,
               "gated_attention: buckets must be (2 * max_distance + 1,) int32, max_distance <= 2048")
         bias, buckets = bias.contiguous(), buckets.contiguous()
-    for n, t in (("lens", lens), ("q_start", q_start)):
-        if isinstance(t, torch.Tensor):
-            _need(tuple(t.shape) == (B,) and t.dtype == torch.int32 and t.device == q.device, f"gated_attention: {n} must be (B,) int32 on q's device")
-    lens = lens.contiguous() if lens is not None else None
-    q_start = q_start.contiguous() if isinstance(q_start, torch.Tensor) else int(q_start or 0)
+    if lens is not None:
+        _need(lens.shape == (B,) and lens.dtype == torch.int32 and lens.device == dev, "gated_attention: lens must be (B,) int32 on q's device")
+        lens = lens.contiguous()
+    if isinstance(q_start, torch.Tensor):
+        _need(q_start.shape == (B,) and q_start.dtype == torch.int32 and q_start.device == dev, "gated_attention: q_start must be (B,) int32 on q's device")
+        q_start = q_start.contiguous()
+    else:
+        q_start = int(q_start or 0)
+        _need(-(1 << 29) <= q_start <= 1 << 29, "gated_attention: q_start must lie within 2^29")
     scale = dk ** -0.5 if scale is None else float(scale)
-    vn = 4 if q.dtype == torch.float32 else 8
+    vn = 4 if dt == torch.float32 else 8
     if dk % vn:                                            # widths that are no multiple of 16 bytes: zero columns change no product
         q, k = F.pad(q, (0, -dk % vn)), F.pad(k, (0, -dk % vn))
     if dv % vn:
         v, gate = F.pad(v, (0, -dv % vn)), F.pad(gate, (0, -dv % vn)) if gate is not None else None
     args = (q, k, v, gate, bias, buckets, lens, q_start, KINDS[kind], bool(causal), scale)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, gate, bias)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (gate is not None and gate.requires_grad) or (bias is not None and bias.requires_grad)):
         out = _GatedAttention.apply(*args)
     else:
         out = _gau_forward(*args, False)[0]
@@ -248,6 +255,8 @@ def gated_attention(q, k, v, gate=None, *, kind="relu2", scale=None, bias=None, 
 
 def _row_view(t, d):
     """(tensor, stride of its rows) with every row's values contiguous and the rows evenly spaced"""
+    if t.is_contiguous():
+        return t, d
     s, n = t.stride(), t.dim()
     if d == 1 or s[-1] == 1:
         step, want = None, None
@@ -267,19 +276,13 @@ def _row_view(t, d):
 
 
 def _norm_args(h, x, gate, rs, w, b, w2, b2, norm, next_norm, eps, next_eps, gate_rows):
-    a = NormArgs()
+    """the packed argument structure and the tensors it points to"""
     d = h.shape[-1]
-    a.dtype, a.norm, a.next_norm, a.dim = _dtype_code(h.dtype), norm, next_norm, d
-    a.rows, a.gate_rows, a.eps, a.next_eps = h.numel() // d, gate_rows, eps, next_eps
-    h, a.h_stride = _row_view(h, d)
-    a.h = h.data_ptr()
-    if x is not None:
-        x, a.x_stride = _row_view(x, d)
-        a.x = x.data_ptr()
-    if gate is not None:
-        gate, a.gate_stride = _row_view(gate, d)
-        a.gate = gate.data_ptr()
-    a.res_scale, a.weight, a.bias, a.next_weight, a.next_bias = _ptr(rs), _ptr(w), _ptr(b), _ptr(w2), _ptr(b2)
+    h, hs = _row_view(h, d)
+    x, xs = _row_view(x, d) if x is not None else (None, 0)
+    gate, gs = _row_view(gate, d) if gate is not None else (None, 0)
+    a = _NORM.pack(_dtype_code(h.dtype), norm, next_norm, d, h.numel() // d, gate_rows, hs, xs, gs, eps, next_eps, h.data_ptr(), _ptr(x), _ptr(gate), _ptr(rs), _ptr(w),
+                   _ptr(b), _ptr(w2), _ptr(b2))
     return a, (h, x, gate)
 
 
@@ -289,7 +292,7 @@ def _joint_forward(h, x, gate, rs, w, b, w2, b2, *plain):
     y = torch.empty(h.shape, dtype=h.dtype, device=dev)
     z = torch.empty(h.shape, dtype=h.dtype, device=dev) if plain[1] else None
     with _on(dev):
-        check(L.tlk_norm_gate_residual_fwd(C.byref(a), y.data_ptr(), _ptr(z), _stream(dev)))
+        check(L.tlk_norm_gate_residual_fwd(a, y.data_ptr(), _ptr(z), _stream(dev)))
     return (y, z) if z is not None else y
 
 
@@ -312,11 +315,11 @@ class _NormGateResidual(torch.autograd.Function):
             return tuple(g.zero_() if g is not None else None for g in grads) + (None,) * len(ctx.plain)
         a, held = _norm_args(*saved, *ctx.plain)
         dy, dz = (t.contiguous() if t is not None else None for t in (dy, dz))
-        g = NormGrads(*[_ptr(t) for t in grads])
+        g = _GRADS.pack(*[_ptr(t) for t in grads])
         with _on(dev):
-            n = L.tlk_norm_gate_residual_workspace(C.byref(a))
+            n = L.tlk_norm_gate_residual_workspace(a)
             ws = _bytes(n, dev)
-            check(L.tlk_norm_gate_residual_bwd(C.byref(a), _ptr(dy), _ptr(dz), C.byref(g), _ptr(ws), n, _stream(dev)))
+            check(L.tlk_norm_gate_residual_bwd(a, _ptr(dy), _ptr(dz), g, _ptr(ws), n, _stream(dev)))
         return tuple(grads) + (None,) * len(ctx.plain)
 
 
@@ -328,13 +331,14 @@ def norm_gate_residual(h, residual=None, *, norm=None, weight=None, bias=None, e
     "scale" (v * weight / max(|v| / sqrt(d), eps), weight one value), "rms" (v * weight / sqrt(mean v^2 + eps), weight (d,)) or "layer" (weight (d,), bias
     (d,) or None).  gate: None, (d,), h's shape, or h's first dimensions followed by ones and d -- (B, 1, d): one gate for each sequence.
     res_scale: (d,) or None.  Statistics and sums are float32; z is normalised from y before its rounding."""
-    _need(h.is_cuda and h.dtype in (torch.float32, torch.float16, torch.bfloat16), "norm_gate_residual: cuda tensors of float32, float16 or bfloat16 (no CPU fallback)")
+    _need(h.is_cuda and h.dtype in _TYPES, "norm_gate_residual: cuda tensors of float32, float16 or bfloat16 (no CPU fallback)")
     _need(h.dim() >= 1 and 1 <= h.shape[-1] <= 8192, "norm_gate_residual: rows of 1 to 8192 values")
     _need(norm in NORMS and next_norm in NORMS, "norm_gate_residual: a norm is None, 'scale', 'rms' or 'layer'")
     d, rows = h.shape[-1], h.numel() // h.shape[-1]
     n1, n2 = NORMS[norm], NORMS[next_norm]
+    dt, dev = h.dtype, h.device
     for t in (residual, gate, weight, bias, res_scale, next_weight, next_bias):
-        _need(t is None or (t.dtype == h.dtype and t.device == h.device), "norm_gate_residual: tensors must share type and device")
+        _need(t is None or (t.dtype == dt and t.device == dev), "norm_gate_residual: tensors must share type and device")
     _need(residual is None or residual.shape == h.shape, "norm_gate_residual: the residual must have h's shape")
     _need(res_scale is None or (residual is not None and tuple(res_scale.shape) == (d,)), "norm_gate_residual: res_scale is (d,) and goes with a residual")
     for kind, w, b in ((n1, weight, bias), (n2, next_weight, next_bias)):

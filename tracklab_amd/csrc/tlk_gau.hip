@@ -34,12 +34,12 @@ int fill(const tlk_gau_args *a, gau::Args &p, const char *fn)
     if (keys > 0 && (!a->k || !a->v)) return fail(TLK_EINVAL, f + ": null k or v");
     if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->gate) & 15) return fail(TLK_EINVAL, f + ": q, k, v and gate must be 16-byte aligned");
     for (int i = 0; i < 3; ++i) {
+        if (a->q_stride[i] < 0 || a->k_stride[i] < 0 || a->v_stride[i] < 0 || (a->gate && a->gate_stride[i] < 0)) return fail(TLK_EINVAL, f + ": strides must not be negative");
         if (a->q_stride[i] % vn || a->k_stride[i] % vn || a->v_stride[i] % vn || (a->gate && a->gate_stride[i] % vn))
             return fail(TLK_EINVAL, f + ": strides must be multiples of 16 bytes");
         if (i == 1 && (a->q_stride[i] > 1 << 22 || a->k_stride[i] > 1 << 22 || a->v_stride[i] > 1 << 22)) return fail(TLK_EINVAL, f + ": row strides of q, k and v must not pass 2^22 elements");
         if (i == 1 && ((a->len_q > 1 && a->q_stride[i] < a->dim_k) || (a->len_k > 1 && (a->k_stride[i] < a->dim_k || a->v_stride[i] < a->dim_v))))
             return fail(TLK_EINVAL, f + ": row strides of q, k and v must not be below their widths");
-        if (a->q_stride[i] < 0 || a->k_stride[i] < 0 || a->v_stride[i] < 0 || (a->gate && a->gate_stride[i] < 0)) return fail(TLK_EINVAL, f + ": strides must not be negative");
     }
     memset(&p, 0, sizeof(p));
     p.q = a->q; p.k = a->k; p.v = a->v; p.gate = a->gate;
