@@ -206,6 +206,10 @@ template <class T> __device__ __forceinline__ typename Ty<T>::V8 pack8(f4 a, f4 
     return r;
 }
 
+// widths come in steps of 32 (64, 96, 128 for q and k), rows of a tile in powers of two
+constexpr int tile_width(int dk) { return dk == 96 ? 128 : dk; }
+// fragments in flight: 4, or the 3 that divide a count of 6
+constexpr int batch(int n) { return n % 4 == 0 ? 4 : (n % 3 == 0 ? 3 : (n % 2 == 0 ? 2 : 1)); }
 // N fragments from LDS, each used by a few matrix instructions: B of them are read while the B before are multiplied.  (An LDS read takes longer than
 // the two instructions that one fragment feeds; left to itself the compiler keeps one or two reads in flight and every fragment waits.)
 // `first`: the first B fragments, read by fragments() earlier, behind other work.
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
 {
     using V8 = typename Ty<T>::V8;
     constexpr int NTH = 64 * WM * WN, BM = WM * MT * 16, DVB = WN * NT * 16, NS = KT / 16;
-    using TK = Tile<T, KT, DK, WM * WN>;
+    using TK = Tile<T, KT, tile_width(DK), WM * WN>;
     using TV = Tile<T, KT, DVB, WM * WN>;
     constexpr int BUF = TK::BYTES + TV::BYTES;
     // (two objects and a loop that names them in turn, not one with an offset: the compiler then knows that a transposing read of one cannot see the loads
@@ -413,7 +417,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
         }
         if (pmin > pmax || (p.causal && j0 > pmax)) return;        // no row of this wave, or none that sees this tile (uniform over the wave)
         f4 s[MT][NS];
-        constexpr int KS = DK / 32, BK = NS * KS < 4 ? NS * KS : 4, BV = NT < 4 ? NT : 4;
+        constexpr int KS = DK / 32, BK = batch(NS * KS), BV = batch(NT);
         const int krow = TK::row_at(0, g, l);
         const typename TV::Col vcol = TV::col_at(TK::BYTES, g, l);
         const auto key = [&](int i) __attribute__((always_inline)) { return TK::row8(cur, krow, i / KS, i % KS); };
@@ -686,14 +690,14 @@ template <class T> __device__ __forceinline__ float unhold(int e) { return !Ty<T
 
 // dQ and the bias gradient: W waves, MT x 16 queries each; walks the keys.  dS^T has a query in the column: its registers are the B operand of
 // dQ^T = K^T dS^T.  The bias gradient needs sums along diagonals: a tile that lies beyond +-D of all its queries is one sum in registers, one near
-// the diagonal goes through a wave's own (KT x BM) LDS tile and each lane sums one diagonal -- no atomics, the order is fixed.
+// the diagonal goes through a wave's own (KT x BM) LDS tile and each lane sums two diagonals -- no atomics, the order is fixed.
 template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
 __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
     constexpr int KT = 32, NTH = 64 * W, BM = W * MT * 16, NS = 2, LT = MT * 16 + 1;
-    static_assert(KT + MT * 16 <= 64, "one diagonal of a wave's tile per lane");
-    using TK = Tile<T, KT, DK, W>;
+    static_assert(KT == 32 && MT <= 2, "the 32 + 31 diagonals of a wave's tile are two per lane of a half wave");
+    using TK = Tile<T, KT, tile_width(DK), W>;
     using TV = Tile<T, KT, DVC, W>;
     constexpr int BUF = TK::BYTES + TV::BYTES;
     __shared__ __attribute__((aligned(1024))) char buf0[BUF], buf1[ONE ? 16 : BUF];     // (two objects: see fwd_kernel)
@@ -769,7 +773,7 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         const float far = where == 1 ? fhi : flo;
         float all = 0.f;
         f4 s[MT][NS], dp[MT][NS];
-        constexpr int KS = DK / 32, VS = DVC / 32, B = DK + DVC > 256 ? 2 : 4;           // (fragments in flight: what the registers leave)
+        constexpr int KS = DK / 32, VS = DVC / 32, BK = DK + DVC > 256 ? 2 : batch(NS * KS), B = DK + DVC > 256 ? 2 : 4, BC = DK + DVC > 256 ? 2 : batch(DK / 16);      // (fragments in flight: what the registers leave)
         const int krow = TK::row_at(0, g, l), vrow = TV::row_at(TK::BYTES, g, l);
         const typename TK::Col kplace = TK::col_at(0, g, l);
         const auto key = [&](int i) __attribute__((always_inline)) { return TK::row8(cur, krow, i / KS, i % KS); };
@@ -779,9 +783,9 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int n = 0; n < NS; ++n) { s[mt][n] = f4{0, 0, 0, 0}; dp[mt][n] = f4{0, 0, 0, 0}; }
-        V8 kf[B], vf[B], cf[B];
+        V8 kf[BK], vf[B], cf[BC];
         fragments(kf, 0, key);
-        stream<NS * KS, B>(kf, key, [&](int i, V8 a) __attribute__((always_inline)) {
+        stream<NS * KS, BK>(kf, key, [&](int i, V8 a) __attribute__((always_inline)) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) s[mt][i / KS] = Ty<T>::mma(a, qf[mt][i % KS], s[mt][i / KS]);
         });
@@ -836,16 +840,24 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            const int e = lane - (MT * 16 - 1);                                       // key - query within the tile
-            float sum = 0.f;
-            for (int c = 0; c < MT * 16; ++c)
-                if (c + e >= 0 && c + e < KT) sum += tile[(c + e) * LT + c];
-            const int d = e + j0 - i0 - q0;
-            if (lane < KT + MT * 16 - 1) {
-                if (d >= p.D) hi += sum;
-                else if (d <= -p.D) lo += sum;
-                else dbw[d + p.D] += sum;
+            // lane n of each half walks half of the queries down the diagonal that begins n keys ahead; past the last key it goes on at the first, on the
+            // diagonal 32 keys behind: all lanes read at every step, and the 63 diagonals are two sums a lane
+            const int n = lane & 31, h0 = lane >> 5;
+            float ahead = 0.f, behind = 0.f;
+#pragma unroll 8
+            for (int i = 0; i < MT * 8; ++i) {
+                const int c = h0 * MT * 8 + i, r = c + n;
+                const float x = tile[(r & 31) * LT + c];
+                ahead += r < KT ? x : 0.f;
+                behind += r < KT ? 0.f : x;
             }
+            ahead = lanes_32<LaneAdd>(ahead);
+            behind = lanes_32<LaneAdd>(behind);
+            const int e = h0 ? n - KT : n, d = e + j0 - i0 - q0;                        // key - query within the tile, and between positions
+            const float sum = h0 ? behind : ahead;
+            if (d >= p.D) hi += sum;
+            else if (d <= -p.D) lo += sum;
+            else dbw[d + p.D] += sum;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
@@ -859,7 +871,7 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         V8 pb[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) pb[mt] = pack8<T>(s[mt][0], s[mt][1]);
-        stream<DK / 16, B>(cf, kcol, [&](int n, V8 a) __attribute__((always_inline)) {
+        stream<DK / 16, BC>(cf, kcol, [&](int n, V8 a) __attribute__((always_inline)) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) acc[n][mt] = Ty<T>::mma(a, pb[mt], acc[n][mt]);
         });
@@ -913,7 +925,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
 {
     using V8 = typename Ty<T>::V8;
     constexpr int QT = 32, NTH = 64 * W, BN = W * MT * 16, NS = 2;
-    using TQ = Tile<T, QT, DK, W>;
+    using TQ = Tile<T, QT, tile_width(DK), W>;
     using TO = Tile<T, QT, DVC, W>;
     constexpr int BUF = TQ::BYTES + TO::BYTES;
     __shared__ __attribute__((aligned(1024))) char buf0[BUF], buf1[ONE ? 16 : BUF];     // (two objects: see fwd_kernel)
@@ -1005,7 +1017,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
             const int where = !p.table || jmin - pmax >= p.D ? 1 : (jmax - pmin <= -p.D ? 2 : 3);
             const float far = where == 1 ? fhi : flo;
             f4 s[MT][NS], wt[MT][NS];                              // (wt: dW first, then the weights)
-            constexpr int KS = DK / 32, VS = DVC / 32, BK = NS * KS < 4 ? NS * KS : 4;
+            constexpr int KS = DK / 32, VS = DVC / 32, BK = batch(NS * KS), BQ = batch(DK / 16);
             const int qplace = TQ::row_at(0, g, l), oplace = TO::row_at(TQ::BYTES, g, l);
             const typename TQ::Col qcplace = TQ::col_at(0, g, l);
             const typename TO::Col ocplace = TO::col_at(TQ::BYTES, g, l);
@@ -1084,8 +1096,9 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) av[n][mt] = Ty<T>::mma(a, wb[mt], av[n][mt]);
             });
-            fragments(ob, 0, qcol);
-            stream<DK / 16, 4>(ob, qcol, [&](int n, V8 a) __attribute__((always_inline)) {
+            V8 cb[BQ];
+            fragments(cb, 0, qcol);
+            stream<DK / 16, BQ>(cb, qcol, [&](int n, V8 a) __attribute__((always_inline)) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) ak[n][mt] = Ty<T>::mma(a, db[mt], ak[n][mt]);
             });

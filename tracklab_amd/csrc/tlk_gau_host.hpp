@@ -1,6 +1,11 @@
 // tlk_gau_host.hpp -- launches of the gated attention unit's kernels for one element type (included by tlk_gau_{f16,bf16,f32}.hip).
 #pragma once
+#include <type_traits>
+
 #include "tlk_gau.hpp"
+#ifndef TLK_KT64
+#define TLK_KT64 8
+#endif
 
 namespace tlk {
 namespace gau {
@@ -144,8 +149,8 @@ template <class K> int launch(K kernel, long long blocks, int threads, size_t fi
 
 template <class T, int KIND, int DK, int MT, int NT, int WM, int WN> int launch_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
 {
-    constexpr int KT = 32;
-    const size_t fixed = sizeof(T) * KT * (DK + WN * NT * 16), smem = a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * table_width(a.D) : 0;
+    constexpr int KT = WN == 1 && sizeof(T) == 2 && NT <= TLK_KT64 ? 64 : 32;
+    const size_t fixed = sizeof(T) * KT * (tile_width(DK) + WN * NT * 16), smem = a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * table_width(a.D) : 0;
     const long long blocks = (long long)a.B * f.heads * f.nsplit * f.nchunk * f.nrow;
     if constexpr (WN > 1)                                           // (one tile of keys: a second buffer would only keep other workgroups off the CU)
         if (a.Lk <= KT) return launch(fwd_kernel<T, KIND, DK, MT, NT, WM, WN, KT, true>, blocks, 64 * WM * WN, fixed, smem, a, st);
@@ -186,8 +191,8 @@ template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
     a.part = reinterpret_cast<float *>(ws);
     a.ml = a.part + (f.nsplit > 1 ? rows * a.dv * f.nsplit : 0);
     int rc;
-    if (kind == SOFTMAX) rc = a.dk <= 64 ? pick_fwd<T, SOFTMAX, 64>(a, f, st) : pick_fwd<T, SOFTMAX, 128>(a, f, st);
-    else rc = a.dk <= 64 ? pick_fwd<T, RELU2, 64>(a, f, st) : pick_fwd<T, RELU2, 128>(a, f, st);
+    if (kind == SOFTMAX) rc = a.dk <= 64 ? pick_fwd<T, SOFTMAX, 64>(a, f, st) : (a.dk <= 96 ? pick_fwd<T, SOFTMAX, 96>(a, f, st) : pick_fwd<T, SOFTMAX, 128>(a, f, st));
+    else rc = a.dk <= 64 ? pick_fwd<T, RELU2, 64>(a, f, st) : (a.dk <= 96 ? pick_fwd<T, RELU2, 96>(a, f, st) : pick_fwd<T, RELU2, 128>(a, f, st));
     if (rc != TLK_OK || f.nsplit == 1) return rc;
     const long long blocks = (rows * (a.dv / 4) + 255) / 256;
     return kind == SOFTMAX ? launch(join_kernel<T, SOFTMAX>, blocks, 256, 0, 0, a, st) : launch(join_kernel<T, RELU2>, blocks, 256, 0, 0, a, st);
@@ -196,7 +201,7 @@ template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
 template <class T, int KIND, int DK, int DVC, int W> int launch_dq(const Args &a, const BwdPlan &f, hipStream_t st)
 {
     constexpr int MT = sizeof(T) == 4 ? 1 : 2;
-    const size_t fixed = sizeof(T) * 32 * (DK + DVC), smem = a.table ? sizeof(float) * (table_width(a.D) + W * (2 * a.D + 1) + W * 32 * (MT * 16 + 1)) : 0;
+    const size_t fixed = sizeof(T) * 32 * (tile_width(DK) + DVC), smem = a.table ? sizeof(float) * (table_width(a.D) + W * (2 * a.D + 1) + W * 32 * (MT * 16 + 1)) : 0;
     const long long blocks = (long long)a.B * a.H * f.nchunk * f.nrow_q;
     if constexpr (W < 4)
         if (a.Lk <= 32) return launch(dq_kernel<T, KIND, DK, DVC, MT, W, true>, blocks, 64 * W, fixed, smem, a, st);
@@ -205,7 +210,7 @@ template <class T, int KIND, int DK, int DVC, int W> int launch_dq(const Args &a
 template <class T, int KIND, int DK, int DVC, int W> int launch_dkv(const Args &a, const BwdPlan &f, hipStream_t st)
 {
     constexpr int MT = sizeof(T) == 4 ? 1 : 2;
-    const size_t fixed = sizeof(T) * 32 * (DK + DVC), smem = a.table ? sizeof(float) * table_width(a.D) : 0;
+    const size_t fixed = sizeof(T) * 32 * (tile_width(DK) + DVC), smem = a.table ? sizeof(float) * table_width(a.D) : 0;
     const long long blocks = (long long)a.B * a.Hk * f.nchunk * f.nparts * f.nrow_k;
     if constexpr (W < 4)
         if (a.Lq <= 32) return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, true>, blocks, 64 * W, fixed + 512, smem, a, st);
@@ -226,8 +231,12 @@ template <class T, int KIND, int DK, int DVC> int pick_bwd(Args a, const BwdPlan
 }
 template <class T, int KIND> int pick_bwd_sizes(const Args &a, const BwdPlan &f, hipStream_t st)
 {
-    if (a.dk <= 64) return f.dvc == 64 ? pick_bwd<T, KIND, 64, 64>(a, f, st) : (f.dvc == 128 ? pick_bwd<T, KIND, 64, 128>(a, f, st) : pick_bwd<T, KIND, 64, 256>(a, f, st));
-    return f.dvc == 64 ? pick_bwd<T, KIND, 128, 64>(a, f, st) : (f.dvc == 128 ? pick_bwd<T, KIND, 128, 128>(a, f, st) : pick_bwd<T, KIND, 128, 256>(a, f, st));
+    const auto widths = [&](auto dk) {
+        constexpr int DK = decltype(dk)::value;
+        return f.dvc == 64 ? pick_bwd<T, KIND, DK, 64>(a, f, st) : (f.dvc == 128 ? pick_bwd<T, KIND, DK, 128>(a, f, st) : pick_bwd<T, KIND, DK, 256>(a, f, st));
+    };
+    if (a.dk <= 64) return widths(std::integral_constant<int, 64>());
+    return a.dk <= 96 ? widths(std::integral_constant<int, 96>()) : widths(std::integral_constant<int, 128>());
 }
 template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t st)
 {
