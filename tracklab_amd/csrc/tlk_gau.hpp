@@ -374,17 +374,30 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
 #pragma unroll
         for (int ks = 0; ks < DK / 32; ++ks) qf[mt][ks] = (ok[mt] && ks * 32 + g * 8 < p.dk) ? ld8(src + ks * 32) : zero8<T>();
     }
-    // few rows: the gate is fetched along with everything else (a block has one or two tiles to walk; behind them its latency would show)
+    // Few rows: a block has one or two tiles to walk, and what surrounds them is what it costs.  The results go through LDS, 16 rows at a time, so that
+    // gate, o and out move as whole rows, 16 bytes a lane (from the accumulators a lane has 8 bytes of each of 16 rows: eight times as many lines to
+    // touch; 2400 crops of 17 x 512 f16: 45 -> 40 us), and the gate is fetched along with everything else.
     constexpr bool EARLY = WN > 1;
-    typename Ty<T>::V4 early[EARLY ? NT : 1][MT];
+    constexpr int VN = 16 / sizeof(T), RC = DVB / VN, CH = (16 * RC + NTH - 1) / NTH, LDE = DVB + 4;
+    static_assert(!EARLY || 16 * LDE * 4 <= BUF, "16 rows of results fit a tile's buffer");
+    u4 early[EARLY ? MT * CH : 1];
+    const auto piece = [&](int mt, int i, int &er, int &ec, int &eq, int &eh) __attribute__((always_inline)) {       // this lane's i-th 16 bytes of 16 rows
+        const int at = i * NTH + tid, r = (er = at / RC, rt * BM + mt * 16 + er);
+        ec = (at - er * RC) * VN;
+        if (at >= 16 * RC || r >= rows || ec >= cend) return false;
+        eh = r / p.Lq;
+        eq = r - eh * p.Lq;
+        return true;
+    };
     if (EARLY && p.gate && p.nsplit == 1) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const T *gp = reinterpret_cast<const T *>(p.gate) + b * p.gs[0] + (long long)qi[mt] * p.gs[1] + (h0 + qh[mt]) * p.gs[2] + c0 + wn * NT * 16 + g * 4;
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                if (ok[mt] && wn * NT * 16 + n * 16 + g * 4 < cend) early[n][mt] = *reinterpret_cast<const typename Ty<T>::V4 *>(gp + n * 16);
-        }
+            for (int i = 0; i < CH; ++i) {
+                int er, ec, eq, eh;
+                if (piece(mt, i, er, ec, eq, eh))
+                    early[mt * CH + i] = *reinterpret_cast<const u4 *>(reinterpret_cast<const T *>(p.gate) + b * p.gs[0] + (long long)eq * p.gs[1] + (h0 + eh) * p.gs[2] + c0 + ec);
+            }
     }
     pmin = __builtin_amdgcn_readfirstlane(wave_min_i(pmin));
     pmax = __builtin_amdgcn_readfirstlane(wave_max_i(pmax));
@@ -527,6 +540,52 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
         }
         __builtin_amdgcn_s_waitcnt(0x0f70);                        // (vmcnt(0): nothing is on its way to LDS when the workgroup ends)
     }
+    if (EARLY && p.nsplit == 1) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float fin = 1.f;
+            if (KIND == SOFTMAX) {
+                lsum[mt] = over_groups_sum(lsum[mt]);
+                fin = lsum[mt] == 0.f ? 0.f : 1.f / lsum[mt];
+                if (p.lse && ok[mt] && c0 == 0 && wn == 0 && g == 0)
+                    p.lse[((long long)b * p.Lq + qi[mt]) * p.H + h0 + qh[mt]] = lsum[mt] == 0.f ? INFINITY : m[mt] + log2f(lsum[mt]);
+            } else if (Ty<T>::scaled) {
+                fin = ex[mt] == E_NONE ? 0.f : ldexpf(1.f, ex[mt]);
+            }
+            float *res = reinterpret_cast<float *>(buf0);
+            __syncthreads();                                        // the tiles, or the 16 rows before, are no longer read
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                f4 x = acc[n][mt] * fin;
+                if (KIND == RELU2 && Ty<T>::scaled) x *= fin;       // (twice: see below)
+                *reinterpret_cast<f4 *>(res + l * LDE + (wn * NT + n) * 16 + g * 4) = x;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                int er, ec, eq, eh;
+                if (!piece(mt, i, er, ec, eq, eh)) continue;
+                const long long at = (((long long)b * p.Lq + eq) * p.H + h0 + eh) * p.dv + c0 + ec;
+                T y[VN], u[VN];
+                __builtin_memcpy(u, &early[mt * CH + i], 16);
+                float x[VN];
+#pragma unroll
+                for (int e = 0; e < VN; e += 4) *reinterpret_cast<f4 *>(x + e) = *reinterpret_cast<const f4 *>(res + er * LDE + ec + e);
+                u4 raw;
+                if (p.o) {
+#pragma unroll
+                    for (int e = 0; e < VN; ++e) y[e] = (T)x[e];
+                    __builtin_memcpy(&raw, y, 16);
+                    *reinterpret_cast<u4 *>(reinterpret_cast<T *>(p.o) + at) = raw;
+                }
+#pragma unroll
+                for (int e = 0; e < VN; ++e) y[e] = (T)(p.gate ? x[e] * (float)u[e] : x[e]);
+                __builtin_memcpy(&raw, y, 16);
+                *reinterpret_cast<u4 *>(reinterpret_cast<T *>(p.out) + at) = raw;
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         if (KIND == SOFTMAX) lsum[mt] = over_groups_sum(lsum[mt]);
@@ -564,9 +623,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
                 *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.o) + row * p.dv + c) = y;
             }
             if (gp) {
-                typename Ty<T>::V4 u;
-                if constexpr (EARLY) u = early[n][mt];
-                else u = *reinterpret_cast<const typename Ty<T>::V4 *>(gp + c);
+                const typename Ty<T>::V4 u = *reinterpret_cast<const typename Ty<T>::V4 *>(gp + c);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[r] *= (float)u[r];
             }
@@ -577,18 +634,20 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
     }
 }
 
-// joins the key splits of few-row calls: one lane per four output values
-template <class T, int KIND> __global__ void __launch_bounds__(256) join_kernel(const Args p)
+// joins the key splits of few-row calls: one lane per four output values, a wave a workgroup (few rows: the CUs' number counts)
+template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(const Args p)
 {
     const int cv = p.dv / 4;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x, nrow = (long long)p.B * p.Lq * p.H;
+    const long long idx = (long long)blockIdx.x * 64 + threadIdx.x, nrow = (long long)p.B * p.Lq * p.H;
     if (idx >= nrow * cv) return;
     const long long row = idx / cv;
     const int c = (int)(idx - row * cv) * 4;
     f4 x = {0, 0, 0, 0};
     if (KIND == SOFTMAX) {
         float m = NEG, s = 0.f;
+#pragma unroll 8
         for (int i = 0; i < p.nsplit; ++i) m = fmaxf(m, p.ml[2 * (i * nrow + row)]);
+#pragma unroll 8
         for (int i = 0; i < p.nsplit; ++i) {
             const float f = pow2_(p.ml[2 * (i * nrow + row)] - m);
             s += f * p.ml[2 * (i * nrow + row) + 1];
@@ -597,6 +656,7 @@ template <class T, int KIND> __global__ void __launch_bounds__(256) join_kernel(
         x *= s == 0.f ? 0.f : 1.f / s;
         if (p.lse && c == 0) p.lse[row] = s == 0.f ? INFINITY : m + log2f(s);
     } else {
+#pragma unroll 8
         for (int i = 0; i < p.nsplit; ++i) x += *reinterpret_cast<const f4 *>(p.part + (i * nrow + row) * p.dv + c);
     }
     const int h = (int)(row % p.H);
@@ -1161,7 +1221,7 @@ template <class T> __global__ void __launch_bounds__(256) sum_parts_kernel(const
     *reinterpret_cast<typename Ty<T>::V4 *>(y + i) = v;
 }
 
-// host side, one instantiation per element type (tlk_gau_f16.hip, tlk_gau_bf16.hip, tlk_gau_f32.hip)
+// host side, one instantiation per element type and direction (tlk_gau_{f16,bf16,f32}{,_bwd}.hip)
 struct BwdIo {
     const void *dout, *o;
     void *dq, *dk, *dv, *dgate, *dtable;

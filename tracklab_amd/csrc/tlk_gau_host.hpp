@@ -1,11 +1,8 @@
-// tlk_gau_host.hpp -- launches of the gated attention unit's kernels for one element type (included by tlk_gau_{f16,bf16,f32}.hip).
+// tlk_gau_host.hpp -- launches of the gated attention unit's kernels for one element type (included by tlk_gau_{f16,bf16,f32}{,_bwd}.hip).
 #pragma once
 #include <type_traits>
 
 #include "tlk_gau.hpp"
-#ifndef TLK_KT64
-#define TLK_KT64 8
-#endif
 
 namespace tlk {
 namespace gau {
@@ -149,7 +146,7 @@ template <class K> int launch(K kernel, long long blocks, int threads, size_t fi
 
 template <class T, int KIND, int DK, int MT, int NT, int WM, int WN> int launch_fwd(const Args &a, const FwdPlan &f, hipStream_t st)
 {
-    constexpr int KT = WN == 1 && sizeof(T) == 2 && NT <= TLK_KT64 ? 64 : 32;
+    constexpr int KT = WN == 1 && sizeof(T) == 2 && NT <= 8 ? 64 : 32;          // (two buffers of 64 keys leave two workgroups a CU up to 128 columns)
     const size_t fixed = sizeof(T) * KT * (tile_width(DK) + WN * NT * 16), smem = a.table ? sizeof(float) * (f.fold ? a.H / a.Hk : 1) * table_width(a.D) : 0;
     const long long blocks = (long long)a.B * f.heads * f.nsplit * f.nchunk * f.nrow;
     if constexpr (WN > 1)                                           // (one tile of keys: a second buffer would only keep other workgroups off the CU)
@@ -194,8 +191,8 @@ template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
     if (kind == SOFTMAX) rc = a.dk <= 64 ? pick_fwd<T, SOFTMAX, 64>(a, f, st) : (a.dk <= 96 ? pick_fwd<T, SOFTMAX, 96>(a, f, st) : pick_fwd<T, SOFTMAX, 128>(a, f, st));
     else rc = a.dk <= 64 ? pick_fwd<T, RELU2, 64>(a, f, st) : (a.dk <= 96 ? pick_fwd<T, RELU2, 96>(a, f, st) : pick_fwd<T, RELU2, 128>(a, f, st));
     if (rc != TLK_OK || f.nsplit == 1) return rc;
-    const long long blocks = (rows * (a.dv / 4) + 255) / 256;
-    return kind == SOFTMAX ? launch(join_kernel<T, SOFTMAX>, blocks, 256, 0, 0, a, st) : launch(join_kernel<T, RELU2>, blocks, 256, 0, 0, a, st);
+    const long long blocks = (rows * (a.dv / 4) + 63) / 64;
+    return kind == SOFTMAX ? launch(join_kernel<T, SOFTMAX>, blocks, 64, 0, 0, a, st) : launch(join_kernel<T, RELU2>, blocks, 64, 0, 0, a, st);
 }
 
 template <class T, int KIND, int DK, int DVC, int W> int launch_dq(const Args &a, const BwdPlan &f, hipStream_t st)
