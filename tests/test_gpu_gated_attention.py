@@ -111,6 +111,18 @@ def test_widths_that_are_no_multiple_of_16_bytes(dk, dv):
         _check(_inputs(7, dtype, 2, 19, 23, 2, 1, dk, dv), "softmax")
 
 
+def test_what_stands_beside_float32_rows_of_half_a_fragment():
+    """12 and 20 columns of float32, which 32-byte reads would pass: the columns next to them hold NaN"""
+    for dk, dv, Lq, Lk in ((12, 20, 19, 23), (20, 12, 3, 40), (4, 4, 70, 1)):
+        t = _inputs(30, F32, 2, Lq, Lk, 2, 1, dk, dv)
+        for n, d in (("q", dk), ("k", dk), ("v", dv), ("gate", dv)):
+            wide = torch.full((*t[n].shape[:3], d + 4), float("nan"), device="cuda")
+            wide[..., :d] = t[n]
+            t[n] = wide[..., :d]
+        for kind in ("relu2", "softmax"):
+            _check(t, kind)
+
+
 @pytest.mark.parametrize("kind", ["relu2", "softmax"])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 def test_few_rows_over_many_keys(dtype, kind):

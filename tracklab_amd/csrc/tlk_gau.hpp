@@ -84,8 +84,20 @@ template <class T> __device__ __forceinline__ typename Ty<T>::V8 zero8()
     return r;
 }
 
-// eight consecutive values of a row in global memory
-template <class T> __device__ __forceinline__ typename Ty<T>::V8 ld8(const T *p) { return *reinterpret_cast<const typename Ty<T>::V8 *>(p); }
+// eight consecutive values of a row in global memory, `left` of them within its width (which is a multiple of 16 bytes); the others zero and not read
+template <class T> __device__ __forceinline__ typename Ty<T>::V8 ld8(const T *p, int left)
+{
+    typename Ty<T>::V8 r = zero8<T>();
+    if constexpr (sizeof(T) == 2) {
+        if (left > 0) r = *reinterpret_cast<const typename Ty<T>::V8 *>(p);
+    } else {
+        f4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+        if (left > 0) a = *reinterpret_cast<const f4 *>(p);
+        if (left > 4) b = *reinterpret_cast<const f4 *>(p + 4);
+        r = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return r;
+}
 
 // A ROWS x COLS tile in LDS, filled by direct-to-LDS loads: 64 lanes x 16 bytes land in 1024 consecutive bytes, so the tile has no padding; instead the
 // 16-byte chunk c of row r stands at c ^ twist(r), which spreads the 16 rows of a fragment read and of a transposing read over all banks.  The loads go
@@ -372,7 +384,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
         if (ok[mt]) { pmin = min(pmin, pos[mt]); pmax = max(pmax, pos[mt]); }
         const T *src = Q + (long long)qi[mt] * p.qs[1] + (h0 + hi) * p.qs[2] + g * 8;
 #pragma unroll
-        for (int ks = 0; ks < DK / 32; ++ks) qf[mt][ks] = (ok[mt] && ks * 32 + g * 8 < p.dk) ? ld8(src + ks * 32) : zero8<T>();
+        for (int ks = 0; ks < DK / 32; ++ks) qf[mt][ks] = ld8(src + ks * 32, ok[mt] ? p.dk - ks * 32 - g * 8 : 0);
     }
     // Few rows: a block has one or two tiles to walk, and what surrounds them is what it costs.  The results go through LDS, 16 rows at a time, so that
     // gate, o and out move as whole rows, 16 bytes a lane (from the accumulators a lane has 8 bytes of each of 16 rows: eight times as many lines to
@@ -799,10 +811,10 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         const long long row = ((long long)b * p.Lq + (ok ? i : 0)) * p.H + h;
         const T *src = Q + (long long)(ok ? i : 0) * p.qs[1] + g * 8;
 #pragma unroll
-        for (int ks = 0; ks < DK / 32; ++ks) qf[mt][ks] = (ok && ks * 32 + g * 8 < p.dk) ? ld8(src + ks * 32) : zero8<T>();
+        for (int ks = 0; ks < DK / 32; ++ks) qf[mt][ks] = ld8(src + ks * 32, ok ? p.dk - ks * 32 - g * 8 : 0);
         const T *dsrc = reinterpret_cast<const T *>(p.dO) + row * p.dv + c0 + g * 8;
 #pragma unroll
-        for (int ks = 0; ks < DVC / 32; ++ks) df[mt][ks] = (ok && ks * 32 + g * 8 < cend) ? ld8(dsrc + ks * 32) : zero8<T>();
+        for (int ks = 0; ks < DVC / 32; ++ks) df[mt][ks] = ld8(dsrc + ks * 32, ok ? cend - ks * 32 - g * 8 : 0);
         lse[mt] = KIND == SOFTMAX ? (ok ? p.lse[row] : INFINITY) : 0.f;
         del[mt] = KIND == SOFTMAX && ok && ch == 0 ? p.delta[row] : 0.f;              // (dW comes in chunks of dv: the subtraction belongs to one of them)
     }
@@ -1007,9 +1019,9 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         const T *kp = reinterpret_cast<const T *>(p.k) + b * p.ks[0] + (long long)(ok ? j : 0) * p.ks[1] + hk * p.ks[2] + g * 8;
         const T *vp = reinterpret_cast<const T *>(p.v) + b * p.vs[0] + (long long)(ok ? j : 0) * p.vs[1] + hk * p.vs[2] + c0 + g * 8;
 #pragma unroll
-        for (int ks = 0; ks < DK / 32; ++ks) kf[mt][ks] = (ok && ks * 32 + g * 8 < p.dk) ? ld8(kp + ks * 32) : zero8<T>();
+        for (int ks = 0; ks < DK / 32; ++ks) kf[mt][ks] = ld8(kp + ks * 32, ok ? p.dk - ks * 32 - g * 8 : 0);
 #pragma unroll
-        for (int ks = 0; ks < DVC / 32; ++ks) vf[mt][ks] = (ok && ks * 32 + g * 8 < cend) ? ld8(vp + ks * 32) : zero8<T>();
+        for (int ks = 0; ks < DVC / 32; ++ks) vf[mt][ks] = ld8(vp + ks * 32, ok ? cend - ks * 32 - g * 8 : 0);
     }
     f4 av[DVC / 16][MT], ak[DK / 16][MT];
 #pragma unroll
