@@ -190,3 +190,13 @@ def test_workspace_sizes_are_those_of_the_plan():
     n = L.tlk_gau_attention_workspace(C.byref(a), 0)
     assert n % (3 * 4 * (128 + 2) * 4) == 0                    # (splits, batch x heads rows, dim_v sums + maximum and sum)
     assert L.tlk_gau_attention_workspace(C.byref(_gau()), 0) == 0
+
+
+def test_workspaces_must_be_aligned():
+    L, err = A._bound(), A._bound().tlk_last_error
+    one = _gau(len_q=1, len_k=20000)
+    need = L.tlk_gau_attention_workspace(C.byref(one), 0)
+    assert need > 0 and L.tlk_gau_attention_fwd(C.byref(one), PTR, None, None, PTR + 8, need, None) == -1 and b"aligned" in err()
+    soft = _gau(kind=1)
+    need = L.tlk_gau_attention_workspace(C.byref(soft), 1)
+    assert L.tlk_gau_attention_bwd(C.byref(soft), *[PTR] * 8, PTR + 8, need, None) == -1 and b"aligned" in err()

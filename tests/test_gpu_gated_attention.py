@@ -123,6 +123,21 @@ def test_what_stands_beside_float32_rows_of_half_a_fragment():
             _check(t, kind)
 
 
+def test_the_c_entry_ignores_the_row_strides_of_one_row():
+    import ctypes as C
+    A = _A()
+    L = A._bound()
+    t = _inputs(31, BF16, 2, 1, 1, 2, 1, 64, 72, True, 0)
+    want = A.gated_attention(t["q"], t["k"], t["v"], t["gate"])
+    a = A.GauArgs()
+    a.dtype, a.kind, a.batch, a.len_q, a.len_k, a.heads, a.kv_heads, a.dim_k, a.dim_v, a.scale = 2, 0, 2, 1, 1, 2, 1, 64, 72, 0.125
+    a.q_stride[:], a.k_stride[:], a.v_stride[:], a.gate_stride[:] = (128, 0, 64), (64, 0, 64), (72, 0, 72), (144, 0, 72)
+    a.q, a.k, a.v, a.gate = (t[n].data_ptr() for n in ("q", "k", "v", "gate"))
+    out = torch.zeros_like(want)
+    assert L.tlk_gau_attention_fwd(C.byref(a), out.data_ptr(), None, None, None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    assert want.any() and torch.equal(out, want)
+
+
 @pytest.mark.parametrize("kind", ["relu2", "softmax"])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 def test_few_rows_over_many_keys(dtype, kind):

@@ -46,6 +46,8 @@ int fill(const tlk_gau_args *a, gau::Args &p, const char *fn)
     p.table = a->num_buckets > 0 ? a->table : nullptr;
     p.bucket_of = a->bucket_of; p.lens = a->lens; p.q_start = a->q_start_dev;
     for (int i = 0; i < 3; ++i) { p.qs[i] = a->q_stride[i]; p.ks[i] = a->k_stride[i]; p.vs[i] = a->v_stride[i]; p.gs[i] = a->gate_stride[i]; }
+    if (a->len_q == 1) p.qs[1] = a->dim_k;                          // (the stride of a single row says nothing)
+    if (a->len_k == 1) { p.ks[1] = a->dim_k; p.vs[1] = a->dim_v; }
     p.B = a->batch; p.Lq = a->len_q; p.Lk = a->len_k; p.H = a->heads; p.Hk = a->kv_heads; p.dk = a->dim_k; p.dv = a->dim_v;
     p.nb = a->num_buckets; p.D = a->num_buckets > 0 ? a->max_distance : 0; p.q0 = a->q_start; p.causal = a->causal != 0; p.table_f32 = a->table_f32 || a->dtype == TLK_F32;
     p.scale = a->scale;
@@ -81,7 +83,8 @@ extern "C" int tlk_gau_attention_fwd(const tlk_gau_args *args, void *out_dev, vo
     if ((long long)p.B * p.Lq == 0) return TLK_OK;
     if (!out_dev || (((uintptr_t)out_dev | (uintptr_t)o_raw_dev) & 15)) return fail(TLK_EINVAL, "tlk_gau_attention_fwd: out must be given, out and o_raw 16-byte aligned");
     const long long need = workspace(p, kind_of(args), elem(args->dtype), false);
-    if (need > 0 && (!workspace_dev || workspace_bytes < need)) return fail(TLK_EINVAL, "tlk_gau_attention_fwd: workspace too small (tlk_gau_attention_workspace)");
+    if (need > 0 && (!workspace_dev || workspace_bytes < need || ((uintptr_t)workspace_dev & 15)))
+        return fail(TLK_EINVAL, "tlk_gau_attention_fwd: workspace too small or not 16-byte aligned (tlk_gau_attention_workspace)");
     p.out = out_dev; p.o = o_raw_dev; p.lse = args->kind == TLK_GAU_SOFTMAX ? lse_dev : nullptr;
     hipStream_t st = (hipStream_t)hip_stream;
     if (args->dtype == TLK_F32) return gau::forward<float>(p, kind_of(args), workspace_dev, st);
