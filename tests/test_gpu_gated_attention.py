@@ -138,6 +138,13 @@ def test_the_c_entry_ignores_the_row_strides_of_one_row():
     assert want.any() and torch.equal(out, want)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16], ids=["f32", "f16"])
+def test_the_widest_bias_with_the_widest_values(dtype):
+    """2048 distances a side beside 256 and 300 columns of dv: float32 tiles leave less LDS for the waves' sums"""
+    for dv in (256, 300):
+        _check(_inputs(32, dtype, 1, 70, 150, 2, 2, 128, dv, True, 7, 2048), "softmax")
+
+
 @pytest.mark.parametrize("kind", ["relu2", "softmax"])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 def test_few_rows_over_many_keys(dtype, kind):

@@ -52,6 +52,9 @@ inline BwdPlan plan_backward(const Args &a, int elem)
     const int per = elem == 4 ? 16 : 32;                            // rows (keys) of a wave: float32 operands take twice the registers
     f.w_q = a.Lq <= 2 * per ? (a.Lq <= per ? 1 : 2) : 4;
     f.w_k = a.Lk <= 2 * per ? (a.Lk <= per ? 1 : 2) : 4;
+    // (a wide table leaves less LDS for the waves' own sums)
+    const auto lds = [&](int w) { return 2LL * elem * 32 * ((a.dk <= 64 ? 64 : 128) + f.dvc) + 4LL * (table_width(a.D) + w * (2 * a.D + 1 + 32 * (per + 1))); };
+    while (a.table && f.w_q > 1 && lds(f.w_q) + 1024 > 160 * 1024) f.w_q /= 2;
     f.rows_q = per * f.w_q;
     f.rows_k = per * f.w_k;
     f.nrow_q = div_up(a.Lq, f.rows_q);
