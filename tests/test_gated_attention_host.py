@@ -200,3 +200,11 @@ def test_workspaces_must_be_aligned():
     soft = _gau(kind=1)
     need = L.tlk_gau_attention_workspace(C.byref(soft), 1)
     assert L.tlk_gau_attention_bwd(C.byref(soft), *[PTR] * 8, PTR + 8, need, None) == -1 and b"aligned" in err()
+
+
+def test_few_workgroups_over_many_keys_are_split():
+    L = A._bound()
+    size = lambda **over: L.tlk_gau_attention_workspace(C.byref(_gau(heads=1, kv_heads=1, batch=1, **over)), 0)      # noqa: E731
+    assert size(len_q=128, len_k=512) == 0 and size(len_q=128, len_k=1024) == 2 * 128 * (64 + 2) * 4          # 512 keys a workgroup at least
+    assert size(len_q=128 * 128, len_k=4096) > 0 and size(len_q=128 * 129, len_k=4096) == 0                   # a workgroup for every other CU
+    assert size(len_q=128 * 128, len_k=2047) == 0 and size(len_q=128 * 128, len_k=2048) > 0                   # what the split saves against what its sums move

@@ -147,6 +147,18 @@ def test_the_widest_bias_with_the_widest_values(dtype):
 
 @pytest.mark.parametrize("kind", ["relu2", "softmax"])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_few_tiles_of_rows_over_many_keys(dtype, kind):
+    """more rows than one tile, too few to fill the card: the keys are split; lengths that end inside a split, on its border and at zero"""
+    lens = torch.tensor([1500, 512, 0, 257], dtype=torch.int32).cuda()
+    for Lq, H, Hk, dv in ((40, 2, 1, 64), (130, 1, 1, 72)):
+        t = _inputs(33, dtype, 4, Lq, 1500, H, Hk, 64, dv, True, 16, 64)
+        _check(t, kind, causal=True, lens=lens, start=lens - Lq, train=False)
+        _check(t, kind, lens=lens)
+    _check(_inputs(34, dtype, 1, 150, 1300, 1, 1, 128, 264, True, 16, 64), kind, causal=True, start=1150)
+
+
+@pytest.mark.parametrize("kind", ["relu2", "softmax"])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 def test_few_rows_over_many_keys(dtype, kind):
     """a cache that is split over workgroups, heads sharing keys answered together; lengths that end inside a split, on its border, and at zero"""
     lens = torch.tensor([3001, 2048, 0, 1, 257, 4096], dtype=torch.int32).cuda()

@@ -646,31 +646,40 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
     }
 }
 
-// joins the key splits of few-row calls: one lane per four output values, a wave a workgroup (few rows: the CUs' number counts)
+// joins the key splits of few-row calls: a wave per row and 64 columns; 16 lanes hold the columns, four groups of lanes every fourth split each
 template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(const Args p)
 {
-    const int cv = p.dv / 4;
-    const long long idx = (long long)blockIdx.x * 64 + threadIdx.x, nrow = (long long)p.B * p.Lq * p.H;
-    if (idx >= nrow * cv) return;
-    const long long row = idx / cv;
-    const int c = (int)(idx - row * cv) * 4;
+    const int cg = (p.dv + 63) / 64, lane = threadIdx.x, g = lane >> 4;
+    const long long row = blockIdx.x / cg, nrow = (long long)p.B * p.Lq * p.H;
+    const int c = (int)(blockIdx.x % cg) * 64 + (lane & 15) * 4;
+    const bool in = c < p.dv;
     f4 x = {0, 0, 0, 0};
+    float m = NEG, s = 0.f;
     if (KIND == SOFTMAX) {
-        float m = NEG, s = 0.f;
 #pragma unroll 8
-        for (int i = 0; i < p.nsplit; ++i) m = fmaxf(m, p.ml[2 * (i * nrow + row)]);
+        for (int i = g; i < p.nsplit; i += 4) m = fmaxf(m, p.ml[2 * (i * nrow + row)]);
+        m = over_groups_max(m);
+    }
 #pragma unroll 8
-        for (int i = 0; i < p.nsplit; ++i) {
+    for (int i = g; i < p.nsplit; i += 4) {
+        f4 y = {0, 0, 0, 0};
+        if (in) y = *reinterpret_cast<const f4 *>(p.part + (i * nrow + row) * p.dv + c);
+        if (KIND == SOFTMAX) {
             const float f = pow2_(p.ml[2 * (i * nrow + row)] - m);
             s += f * p.ml[2 * (i * nrow + row) + 1];
-            x += *reinterpret_cast<const f4 *>(p.part + (i * nrow + row) * p.dv + c) * f;
+            x += y * f;
+        } else {
+            x += y;
         }
-        x *= s == 0.f ? 0.f : 1.f / s;
-        if (p.lse && c == 0) p.lse[row] = s == 0.f ? INFINITY : m + log2f(s);
-    } else {
-#pragma unroll 8
-        for (int i = 0; i < p.nsplit; ++i) x += *reinterpret_cast<const f4 *>(p.part + (i * nrow + row) * p.dv + c);
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = over_groups_sum(x[r]);
+    if (KIND == SOFTMAX) {
+        s = over_groups_sum(s);
+        x *= s == 0.f ? 0.f : 1.f / s;
+        if (p.lse && c == 0 && lane == 0) p.lse[row] = s == 0.f ? INFINITY : m + log2f(s);
+    }
+    if (!in || g) return;
     const int h = (int)(row % p.H);
     const long long bi = row / p.H;
     typename Ty<T>::V4 y;

@@ -31,8 +31,13 @@ inline FwdPlan plan_forward(const Args &a, int elem)
     const long long blocks = (long long)a.B * f.heads * f.nchunk * f.nrow;
     f.nsplit = 1;
     f.split_keys = a.Lk;
-    if (f.few && a.Lk > 512 && blocks < 2048) {
-        const int want = (int)((2048 + blocks - 1) / blocks), most = div_up(a.Lk, 256);
+    // Few workgroups over many keys: the keys are split.  One tile of rows is read at the rate of HBM, which takes many workgroups: 2048, of 256 keys at least.
+    // More rows are matrix products: two workgroups a CU, of 512 keys at least, and no split from half a workgroup a CU on or where the sums of the splits
+    // move more than they save (bf16, dv 128, one head: 128 rows x 4096 keys 97 -> 21 us, 4 x 1024 x 4096 98 -> 32; 16 x 1024 rows x 1024 keys would go
+    // 32 -> 37, x 4096 keys 100 -> 61; 192 workgroups 55 -> 70).
+    const int full = f.few ? 2048 : 512, least = f.few ? 256 : 512;
+    if (a.Lk > 512 && blocks > 0 && (f.few ? blocks < 2048 : blocks <= 128 && a.Lk >= 16 * blocks)) {
+        const int want = (int)(f.few ? (full + blocks - 1) / blocks : full / blocks), most = div_up(a.Lk, least);
         f.nsplit = want < most ? want : most;
         f.split_keys = div_up(div_up(a.Lk, f.nsplit), 64) * 64;
         f.nsplit = div_up(a.Lk, f.split_keys);
@@ -194,7 +199,7 @@ template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
     if (kind == SOFTMAX) rc = a.dk <= 64 ? pick_fwd<T, SOFTMAX, 64>(a, f, st) : (a.dk <= 96 ? pick_fwd<T, SOFTMAX, 96>(a, f, st) : pick_fwd<T, SOFTMAX, 128>(a, f, st));
     else rc = a.dk <= 64 ? pick_fwd<T, RELU2, 64>(a, f, st) : (a.dk <= 96 ? pick_fwd<T, RELU2, 96>(a, f, st) : pick_fwd<T, RELU2, 128>(a, f, st));
     if (rc != TLK_OK || f.nsplit == 1) return rc;
-    const long long blocks = (rows * (a.dv / 4) + 63) / 64;
+    const long long blocks = rows * ((a.dv + 63) / 64);
     return kind == SOFTMAX ? launch(join_kernel<T, SOFTMAX>, blocks, 64, 0, 0, a, st) : launch(join_kernel<T, RELU2>, blocks, 64, 0, 0, a, st);
 }
 
