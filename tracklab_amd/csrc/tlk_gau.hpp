@@ -14,6 +14,9 @@
 
 #include "tlk_lanes.hpp"
 
+// the launch bounds below are meant for the registers; workgroups of one or two waves, and wide tiles, reach fewer waves for their LDS
+#pragma clang diagnostic ignored "-Wpass-failed"
+
 namespace tlk {
 namespace gau {
 
@@ -1005,6 +1008,10 @@ template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
 __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK + DVC == 256) ? 1 : 2) dkv_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
+    // float16 softmax: weights are at most 1, so one fixed power of two does for them: 2^14 higher no weight above 2^-28 is subnormal.  It comes with the
+    // log-sum-exp, for nothing; the score gradients carry it too.  (An exponent of their own, as the squares have: 6 x 1021 tokens, 8 heads, 72 and 104
+    // columns 124 us, so 100.)
+    constexpr float UP = KIND == SOFTMAX && Ty<T>::scaled ? 14.f : 0.f;
     constexpr int QT = 32, NTH = 64 * W, BN = W * MT * 16, NS = 2;
     using TQ = Tile<T, QT, tile_width(DK), W>;
     using TO = Tile<T, QT, DVC, W>;
@@ -1071,7 +1078,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
             }
         };
         const auto keep = [&](float *st) __attribute__((always_inline)) {
-            if (KIND == SOFTMAX && tid < QT) { st[tid] = ls0; st[QT + tid] = dl0; }
+            if (KIND == SOFTMAX && tid < QT) { st[tid] = ls0 - UP; st[QT + tid] = dl0; }
         };
         __syncthreads();                                                                  // the previous head's tiles and table are no longer read
         if (ib < p.Lq) {
@@ -1098,7 +1105,9 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
             const int where = !p.table || jmin - pmax >= p.D ? 1 : (jmax - pmin <= -p.D ? 2 : 3);
             const float far = where == 1 ? fhi : flo;
             f4 s[MT][NS], wt[MT][NS];                              // (wt: dW first, then the weights)
-            constexpr int KS = DK / 32, VS = DVC / 32, BK = batch(NS * KS), BQ = batch(DK / 16);
+            // (float16 with its exponents passes the registers of two waves at 192 columns and more: shorter batches spill less)
+            constexpr bool TIGHT = Ty<T>::scaled && DK + DVC > 160 && DK + DVC < 256;
+            constexpr int KS = DK / 32, VS = DVC / 32, BK = TIGHT ? 2 : batch(NS * KS), BQ = TIGHT ? 2 : batch(DK / 16), BO = TIGHT ? 2 : 4;
             const int qplace = TQ::row_at(0, g, l), oplace = TO::row_at(TQ::BYTES, g, l);
             const typename TQ::Col qcplace = TQ::col_at(0, g, l);
             const typename TO::Col ocplace = TO::col_at(TQ::BYTES, g, l);
@@ -1110,14 +1119,14 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int n = 0; n < NS; ++n) { s[mt][n] = f4{0, 0, 0, 0}; wt[mt][n] = f4{0, 0, 0, 0}; }
-            V8 qb[BK], ob[4];
+            V8 qb[BK], ob[BO];
             fragments(qb, 0, qrow);
             stream<NS * KS, BK>(qb, qrow, [&](int i, V8 a) __attribute__((always_inline)) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) s[mt][i / KS] = Ty<T>::mma(a, kf[mt][i % KS], s[mt][i / KS]);
             });
             fragments(ob, 0, orow);
-            stream<NS * VS, 4>(ob, orow, [&](int i, V8 a) __attribute__((always_inline)) {
+            stream<NS * VS, BO>(ob, orow, [&](int i, V8 a) __attribute__((always_inline)) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) wt[mt][i / VS] = Ty<T>::mma(a, vf[mt][i % VS], wt[mt][i / VS]);
             });
@@ -1163,7 +1172,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
             V8 wb[MT], db[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const float fv = hold<T, NS>(wt[mt], ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
+                const float fv = UP != 0.f ? 1.f : hold<T, NS>(wt[mt], ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
                 if (Ty<T>::scaled && __any(fv != 1.f))
 #pragma unroll
                     for (int n = 0; n < DVC / 16; ++n) av[n][mt] *= fv;
@@ -1173,7 +1182,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
                 wb[mt] = pack8<T>(wt[mt][0], wt[mt][1]);
                 db[mt] = pack8<T>(s[mt][0], s[mt][1]);
             }
-            stream<DVC / 16, 4>(ob, ocol, [&](int n, V8 a) __attribute__((always_inline)) {
+            stream<DVC / 16, BO>(ob, ocol, [&](int n, V8 a) __attribute__((always_inline)) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) av[n][mt] = Ty<T>::mma(a, wb[mt], av[n][mt]);
             });
@@ -1199,7 +1208,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         const int j = j0 + mt * 16 + l;
         if (j >= p.Lk) continue;
         const long long row = ((long long)b * p.Lk + j) * p.Hk + hk;
-        const float finv = unhold<T>(ev[mt]), fink = p.scale * unhold<T>(ek[mt]);
+        const float down = ldexpf(1.f, -(int)UP), finv = UP != 0.f ? down : unhold<T>(ev[mt]), fink = p.scale * unhold<T>(ek[mt]) * down;
         typename Ty<T>::V4 y;
 #pragma unroll
         for (int n = 0; n < DVC / 16; ++n) {
