@@ -105,6 +105,34 @@ def test_distances_of_the_bias(D, buckets):
     _check(t, "relu2", causal=True, start=80)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("dv, causal", [(64, False), (64, True), (320, False)])
+def test_shared_distances_of_a_softmax_take_up_no_rounding(dtype, dv, causal):
+    """A row's score gradients sum to zero.  With values between two neighbours of the type o is rounded the same way in every row, by up to half a step: a
+    delta from that o would leave eps / 4 of sum W |dW| in the entries beyond +-D.  Bound: dW and S are float32 sums of dv and dk products (relative error
+    below (dv + dk) 2^-24 < 2^-15), a weight's exponent of a few units takes S's error a few times, and sums over 700 keys add 2^-17: 2^-13 of sum W (|dW| +
+    |delta|), which is below eps / 4 for both types' eps / 4 (2^-12 and 2^-9)."""
+    L, D = 700, 16
+    t = _inputs(35, dtype, 2, L, L, 1, 1, 64, dv, False, 2 * D + 1, D, F32)
+    t["buckets"] = torch.arange(2 * D + 1, dtype=torch.int32).cuda()
+    g = torch.Generator().manual_seed(36)
+    t["v"] = (1 + torch.finfo(dtype).eps * (torch.rand(t["v"].shape, generator=g) < 0.75)).to(dtype).cuda()
+    t["dout"] = torch.ones_like(t["dout"])
+    got = _run(t, "softmax", causal)["dtable"].double().cpu()[:, 0]
+    q, k, v, tab = (t[n].double().cpu() for n in ("q", "k", "v", "table"))
+    away = torch.arange(L) - torch.arange(L)[:, None]
+    want, size = torch.zeros(2 * D + 1, dtype=torch.float64), torch.zeros(2 * D + 1, dtype=torch.float64)
+    for b in range(2):
+        s = q[b, :, 0] @ k[b, :, 0].T / 8 + tab[:, 0][away.clamp(-D, D) + D]
+        w = torch.softmax(torch.where(away > 0, -math.inf, s) if causal else s, -1)
+        dw = v[b, :, 0].sum(-1).expand(L, L)
+        delta = (w * dw).sum(-1, keepdim=True)
+        want.index_add_(0, (away.clamp(-D, D) + D).reshape(-1), (w * (dw - delta)).reshape(-1))
+        size.index_add_(0, (away.clamp(-D, D) + D).reshape(-1), (w * (dw + delta)).reshape(-1))
+    for e in (0, 2 * D):
+        assert float((got - want)[e].abs()) <= float(size[e]) * 2.0 ** -13, (e, float(got[e]), float(want[e]), float(size[e]))
+
+
 @pytest.mark.parametrize("dk, dv", [(20, 13), (5, 3), (100, 33), (127, 257)])
 def test_widths_that_are_no_multiple_of_16_bytes(dk, dv):
     for dtype in (F32, F16):

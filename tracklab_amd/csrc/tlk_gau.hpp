@@ -12,6 +12,8 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 #include "tlk_lanes.hpp"
 
 // the launch bounds below are meant for the registers; workgroups of one or two waves, and wide tiles, reach fewer waves for their LDS
@@ -775,6 +777,9 @@ template <class T> __device__ __forceinline__ float unhold(int e) { return !Ty<T
 // dQ and the bias gradient: W waves, MT x 16 queries each; walks the keys.  dS^T has a query in the column: its registers are the B operand of
 // dQ^T = K^T dS^T.  The bias gradient needs sums along diagonals: a tile that lies beyond +-D of all its queries is one sum in registers, one near
 // the diagonal goes through a wave's own (KT x BM) LDS tile and each lane sums two diagonals -- no atomics, the order is fixed.
+// Softmax: the score gradients of a row sum to zero, but with delta = dO . o from the rounded o they sum to eta = dO . (W v - o), and the two entries beyond
+// +-D, into which most pairs fall, take it up over all rows: against entries that cancel by nature it was 1e-2 of the gradient (1137 bf16 tokens, D 16).
+// What the row really sums to is known at the end of its walk; eta times the row's weight beyond +-D goes off those entries.  (Of one diagonal it is nothing.)
 template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
 __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
 {
@@ -839,7 +844,9 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
     int ex[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) ex[mt] = E_NONE;
-    float lo = 0.f, hi = 0.f;
+    float lo = 0.f, hi = 0.f, eta[MT], mlo[MT], mhi[MT];                              // (eta, and the weight beyond -D and +D, of the lane's query)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) eta[mt] = mlo[mt] = mhi[mt] = 0.f;
     const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
     if (p.table) __syncthreads();
     const float flo = p.table ? tab[0] : 0.f, fhi = p.table ? tab[TW - 1] : 0.f;          // the bias beyond +-D
@@ -855,7 +862,6 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin) && i0 + MT * 16 <= p.Lq;
         const int where = !p.table || j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3);
         const float far = where == 1 ? fhi : flo;
-        float all = 0.f;
         f4 s[MT][NS], dp[MT][NS];
         constexpr int KS = DK / 32, VS = DVC / 32, BK = DK + DVC > 256 ? 2 : batch(NS * KS), B = DK + DVC > 256 ? 2 : 4, BC = DK + DVC > 256 ? 2 : batch(DK / 16);      // (fragments in flight: what the registers leave)
         const int krow = TK::row_at(0, g, l), vrow = TV::row_at(TK::BYTES, g, l);
@@ -901,25 +907,37 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
                 }
             }
         }
+        const auto gradients = [&](auto near) __attribute__((always_inline)) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float wgt;
-                    s[mt][n][r] = dscore<KIND>(s[mt][n][r], dp[mt][n][r], lse[mt], del[mt], wgt);
-                    all += s[mt][n][r];
-                }
-        if (where == 3)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt) {
+                float all = 0.f, mass = 0.f;
 #pragma unroll
                 for (int n = 0; n < NS; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = s[mt][n][r];
-        if (where == 1) hi += all;
-        if (where == 2) lo += all;
+                    for (int r = 0; r < 4; ++r) {
+                        float wgt;
+                        const float x = s[mt][n][r] = dscore<KIND>(s[mt][n][r], dp[mt][n][r], lse[mt], del[mt], wgt);
+                        all += x;
+                        if constexpr (decltype(near)::value) {
+                            tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = x;
+                            if (KIND == SOFTMAX) {
+                                const int away = j0 + n * 16 + g * 4 + r - (i0 + mt * 16 + l + q0);
+                                mhi[mt] += away >= p.D ? wgt : 0.f;
+                                mlo[mt] += away < p.D && away <= -p.D ? wgt : 0.f;
+                            }
+                        } else {
+                            mass += wgt;
+                        }
+                    }
+                if (KIND == SOFTMAX) eta[mt] += all;
+                if constexpr (!decltype(near)::value) {
+                    if (where == 1) { hi += all; mhi[mt] += mass; }
+                    else { lo += all; mlo[mt] += mass; }
+                }
+            }
+        };
+        if (where == 3) gradients(std::true_type());
+        else gradients(std::false_type());
         if (where == 3) {
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -970,6 +988,13 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         __builtin_amdgcn_s_waitcnt(0x0f70);                        // (vmcnt(0): nothing is on its way to LDS when the workgroup ends)
     }
     if (p.table) {
+        if (KIND == SOFTMAX)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float e = over_groups_sum(eta[mt]);          // (a chunk of dv has its part of eta: the parts' corrections add up as the entries do)
+                lo -= e * mlo[mt];
+                hi -= e * mhi[mt];
+            }
         lo = lanes_all<LaneAdd, 64>(lo);
         hi = lanes_all<LaneAdd, 64>(hi);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
