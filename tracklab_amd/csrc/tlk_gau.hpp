@@ -931,8 +931,12 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
                     }
                 if (KIND == SOFTMAX) eta[mt] += all;
                 if constexpr (!decltype(near)::value) {
-                    if (where == 1) { hi += all; mhi[mt] += mass; }
-                    else { lo += all; mlo[mt] += mass; }
+                    hi += where == 1 ? all : 0.f;                  // (selected values: of selected sums the compiler makes an address, and memory of the registers)
+                    lo += where == 1 ? 0.f : all;
+                    if (KIND == SOFTMAX) {
+                        mhi[mt] += where == 1 ? mass : 0.f;
+                        mlo[mt] += where == 1 ? 0.f : mass;
+                    }
                 }
             }
         };
