@@ -907,6 +907,9 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
                 }
             }
         }
+        int right = where == 1 ? -1 : 0;                           // (opaque: of a choice between two sums the compiler makes an address, and memory of the registers)
+        asm volatile("" : "+v"(right));
+        const auto masked = [](float x, int m) __attribute__((always_inline)) { return __builtin_bit_cast(float, __builtin_bit_cast(int, x) & m); };
         const auto gradients = [&](auto near) __attribute__((always_inline)) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -931,11 +934,11 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
                     }
                 if (KIND == SOFTMAX) eta[mt] += all;
                 if constexpr (!decltype(near)::value) {
-                    hi += where == 1 ? all : 0.f;                  // (selected values: of selected sums the compiler makes an address, and memory of the registers)
-                    lo += where == 1 ? 0.f : all;
+                    hi += masked(all, right);
+                    lo += masked(all, ~right);
                     if (KIND == SOFTMAX) {
-                        mhi[mt] += where == 1 ? mass : 0.f;
-                        mlo[mt] += where == 1 ? 0.f : mass;
+                        mhi[mt] += masked(mass, right);
+                        mlo[mt] += masked(mass, ~right);
                     }
                 }
             }
@@ -961,9 +964,9 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
             behind = lanes_32<LaneAdd>(behind);
             const int e = h0 ? n - KT : n, d = e + j0 - i0 - q0;                        // key - query within the tile, and between positions
             const float sum = h0 ? behind : ahead;
-            if (d >= p.D) hi += sum;
-            else if (d <= -p.D) lo += sum;
-            else dbw[d + p.D] += sum;
+            hi += d >= p.D ? sum : 0.f;
+            lo += d < p.D && d <= -p.D ? sum : 0.f;
+            if (d < p.D && d > -p.D) dbw[d + p.D] += sum;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
