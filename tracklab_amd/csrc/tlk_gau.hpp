@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
     }
 }
 
-// joins the key splits of few-row calls: a wave per row and 64 columns; 16 lanes hold the columns, four groups of lanes every fourth split each
+// joins the key splits: a wave per row and 64 columns; 16 lanes hold the columns, four groups of lanes every fourth split each
 // (512 rows of 128 in 16 splits: 6 us, a launch's own time; a lane for four columns and all splits took 14)
 template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(const Args p)
 {
