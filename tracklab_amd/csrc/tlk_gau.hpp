@@ -50,6 +50,7 @@ struct Args {
     int nsplit, split_keys, nchunk, nrow, fold, nparts, snake;
     // backward
     const void *dO;                             // (B, Lq, H, dv) contiguous: the gradient behind the gate
+    const void *dO_low;                         // the same shape: what dO's rounding left (16-bit types with a gate and a table)
     const float *delta;                         // (B, Lq, H): sum_d dO o (softmax)
     void *dq, *dk_, *dv_;
     float *dq_part, *dk_part, *dv_part;         // (chunk, B, Lq, H, dk); (chunk x part, B, Lk, Hk, dk), (part, B, Lk, Hk, dv): sums of several blocks, joined afterwards
@@ -708,10 +709,11 @@ template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(c
 
 // ----------------------------------------------------------------------------------------------------------------------------------- backward
 // behind the gate: dO = dout * gate, dgate = dout * O, delta = sum_d dO * O.  LANES lanes a row; bound by HBM (4 x 4096 rows of 1024 bf16: 28 us, 5 tensors of 34 MB, which the caches hold in part).
+// low: what rounding dO left; the product of two 16-bit values is dO + low exactly (16 bits of bfloat16, 22 of float16), and delta is formed from it.
 template <class T> struct GateArgs {
     const T *dout, *gate, *o;
     long long gs[3];
-    T *dO, *dgate;
+    T *dO, *low, *dgate;
     float *delta;
     long long rows;
     int Lq, H, dv;
@@ -727,16 +729,19 @@ template <class T, int LANES> __global__ void __launch_bounds__(256) gate_bwd_ke
     float d = 0.f;
     for (int c = lane * 4; c < p.dv; c += LANES * 4) {
         const V4 du = *reinterpret_cast<const V4 *>(p.dout + row * p.dv + c), o = *reinterpret_cast<const V4 *>(p.o + row * p.dv + c);
-        V4 a, b;
+        V4 a, b, rest;
         if (gp) {
             const V4 u = *reinterpret_cast<const V4 *>(gp + c);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                a[r] = (T)((float)du[r] * (float)u[r]);
+                const float x = (float)du[r] * (float)u[r];
+                a[r] = (T)x;
+                rest[r] = (T)(x - (float)a[r]);
                 b[r] = (T)((float)du[r] * (float)o[r]);
-                d += (float)a[r] * (float)o[r];
+                d += (p.low ? x : (float)a[r]) * (float)o[r];
             }
             *reinterpret_cast<V4 *>(p.dO + row * p.dv + c) = a;
+            if (p.low) *reinterpret_cast<V4 *>(p.low + row * p.dv + c) = rest;
             *reinterpret_cast<V4 *>(p.dgate + row * p.dv + c) = b;
         } else {
 #pragma unroll
@@ -783,10 +788,12 @@ template <class T> __device__ __forceinline__ float unhold(int e) { return !Ty<T
 // Softmax: the score gradients of a row sum to zero, but with delta = dO . o from the rounded o they sum to eta = dO . (W v - o), and the two entries beyond
 // +-D, into which most pairs fall, take it up over all rows: against entries that cancel by nature it was 1e-2 of the gradient (1137 bf16 tokens, D 16).
 // What the row really sums to is known at the end of its walk; eta times the row's weight beyond +-D goes off those entries.  (Of one diagonal it is nothing.)
-// Bound by the vector work between three products per score tile: 4 x 4096 causal bf16 tokens, dk 128, dv 1024, relu^2: 176 us; 4 x 2048 tokens, 16 heads of 64,
+// Bound by the vector work between three products per score tile: 4 x 4096 causal bf16 tokens, dk 128, dv 1024, relu^2: 250 us with two parts of dO, 176 with one; 4 x 2048 tokens, 16 heads of 64,
 // softmax, causal: 114 us (91 without eta).
-template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
-__global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
+// LOW: dO comes in two parts.  Rounded once, dO is off by the same amounts for all keys of its row; a bucket's sum over many pairs, which cancel, keeps that (bf16, 4 x 1024
+// tokens, relu^2: up to 1e-2 of the bias gradient).  One more product a tile, and its fragments: at 256 columns one wave a SIMD has the registers for them.
+template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE, bool LOW>
+__global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
     constexpr int KT = 32, NTH = 64 * W, BM = W * MT * 16, NS = 2, LT = MT * 16 + 1;
@@ -824,7 +831,7 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         for (int t = lane; t < NB; t += 64) dbw[t] = 0.f;
     }
     const int i0 = rt * BM + w * MT * 16;                                             // the wave's first query
-    V8 qf[MT][DK / 32], df[MT][DVC / 32];
+    V8 qf[MT][DK / 32], df[MT][DVC / 32], dl[LOW ? MT : 1][LOW ? DVC / 32 : 1];
     float lse[MT], del[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -837,6 +844,11 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         const T *dsrc = reinterpret_cast<const T *>(p.dO) + row * p.dv + c0 + g * 8;
 #pragma unroll
         for (int ks = 0; ks < DVC / 32; ++ks) df[mt][ks] = ld8(dsrc + ks * 32, ok ? cend - ks * 32 - g * 8 : 0);
+        if constexpr (LOW) {
+            const T *lsrc = reinterpret_cast<const T *>(p.dO_low) + row * p.dv + c0 + g * 8;
+#pragma unroll
+            for (int ks = 0; ks < DVC / 32; ++ks) dl[mt][ks] = ld8(lsrc + ks * 32, ok ? cend - ks * 32 - g * 8 : 0);
+        }
         lse[mt] = KIND == SOFTMAX ? (ok ? p.lse[row] : INFINITY) : 0.f;
         del[mt] = KIND == SOFTMAX && ok && ch == 0 ? p.delta[row] : 0.f;              // (dW comes in chunks of dv: the subtraction belongs to one of them)
     }
@@ -868,7 +880,8 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         const int where = !p.table || j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3);
         const float far = where == 1 ? fhi : flo;
         f4 s[MT][NS], dp[MT][NS];
-        constexpr int KS = DK / 32, VS = DVC / 32, BK = DK + DVC > 256 ? 2 : batch(NS * KS), B = DK + DVC > 256 ? 2 : 4, BC = DK + DVC > 256 ? 2 : batch(DK / 16);      // (fragments in flight: what the registers leave)
+        constexpr bool TIGHT = LOW ? DK > 64 && DVC == 128 : DK + DVC > 256;            // (fragments in flight: what the registers leave)
+        constexpr int KS = DK / 32, VS = DVC / 32, BK = TIGHT ? 2 : batch(NS * KS), B = TIGHT ? 2 : 4, BC = TIGHT ? 2 : batch(DK / 16);
         const int krow = TK::row_at(0, g, l), vrow = TV::row_at(TK::BYTES, g, l);
         const typename TK::Col kplace = TK::col_at(0, g, l);
         const auto key = [&](int i) __attribute__((always_inline)) { return TK::row8(cur, krow, i / KS, i % KS); };
@@ -887,7 +900,10 @@ __global__ void __launch_bounds__(64 * W, 2) dq_kernel(const Args p)
         fragments(vf, 0, val);
         stream<NS * VS, B>(vf, val, [&](int i, V8 a) __attribute__((always_inline)) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) dp[mt][i / VS] = Ty<T>::mma(a, df[mt][i % VS], dp[mt][i / VS]);
+            for (int mt = 0; mt < MT; ++mt) {
+                dp[mt][i / VS] = Ty<T>::mma(a, df[mt][i % VS], dp[mt][i / VS]);
+                if constexpr (LOW) dp[mt][i / VS] = Ty<T>::mma(a, dl[mt][i % VS], dp[mt][i / VS]);
+            }
         });
         fragments(cf, 0, kcol);
         __builtin_amdgcn_sched_barrier(0);

@@ -74,7 +74,7 @@ inline BwdPlan plan_backward(const Args &a, int elem)
 constexpr int DB_SPLITS = 64;
 
 struct BwdWs {
-    long long dO, delta, dq, dk, dv, db, db2, total;
+    long long dO, low, delta, dq, dk, dv, db, db2, total;
 };
 inline BwdWs layout_backward(const Args &a, int kind, int elem, const BwdPlan &f)
 {
@@ -83,6 +83,7 @@ inline BwdWs layout_backward(const Args &a, int kind, int elem, const BwdPlan &f
     const long long rows = (long long)a.B * a.Lq * a.H, keys = (long long)a.B * a.Lk * a.Hk;
     const auto take = [&](long long bytes) { const long long r = at; at += align_up(bytes); return r; };
     w.dO = take(a.gate ? rows * a.dv * elem : 0);
+    w.low = take(a.gate && a.table && elem == 2 ? rows * a.dv * elem : 0);
     w.delta = take(kind == SOFTMAX ? rows * 4 : 0);
     w.dq = take(f.nchunk > 1 ? rows * a.dk * f.nchunk * 4 : 0);
     w.dk = take(f.nchunk * f.nparts > 1 ? keys * a.dk * f.nchunk * f.nparts * 4 : 0);
@@ -203,14 +204,19 @@ template <class T> int forward(Args a, int kind, void *ws, hipStream_t st)
     return kind == SOFTMAX ? launch(join_kernel<T, SOFTMAX>, blocks, 64, 0, 0, a, st) : launch(join_kernel<T, RELU2>, blocks, 64, 0, 0, a, st);
 }
 
-template <class T, int KIND, int DK, int DVC, int W> int launch_dq(const Args &a, const BwdPlan &f, hipStream_t st)
+template <class T, int KIND, int DK, int DVC, int W, bool LOW> int launch_dq(const Args &a, const BwdPlan &f, hipStream_t st)
 {
     constexpr int MT = sizeof(T) == 4 ? 1 : 2;
     const size_t fixed = sizeof(T) * 32 * (tile_width(DK) + DVC), smem = a.table ? sizeof(float) * (table_width(a.D) + W * (2 * a.D + 1) + W * 32 * (MT * 16 + 1)) : 0;
     const long long blocks = (long long)a.B * a.H * f.nchunk * f.nrow_q;
     if constexpr (W < 4)
-        if (a.Lk <= 32) return launch(dq_kernel<T, KIND, DK, DVC, MT, W, true>, blocks, 64 * W, fixed, smem, a, st);
-    return launch(dq_kernel<T, KIND, DK, DVC, MT, W, false>, blocks, 64 * W, 2 * fixed, smem, a, st);
+        if (a.Lk <= 32) return launch(dq_kernel<T, KIND, DK, DVC, MT, W, true, LOW>, blocks, 64 * W, fixed, smem, a, st);
+    return launch(dq_kernel<T, KIND, DK, DVC, MT, W, false, LOW>, blocks, 64 * W, 2 * fixed, smem, a, st);
+}
+template <class T, int KIND, int DK, int DVC, bool LOW> int pick_dq(const Args &a, const BwdPlan &f, hipStream_t st)
+{
+    if (f.w_q == 1) return launch_dq<T, KIND, DK, DVC, 1, LOW>(a, f, st);
+    return f.w_q == 2 ? launch_dq<T, KIND, DK, DVC, 2, LOW>(a, f, st) : launch_dq<T, KIND, DK, DVC, 4, LOW>(a, f, st);
 }
 template <class T, int KIND, int DK, int DVC, int W> int launch_dkv(const Args &a, const BwdPlan &f, hipStream_t st)
 {
@@ -226,8 +232,11 @@ template <class T, int KIND, int DK, int DVC> int pick_bwd(Args a, const BwdPlan
     a.nchunk = f.nchunk;
     a.nparts = f.nparts;
     a.nrow = f.nrow_q;
-    a.snake = snake_from(a, (long long)a.B * a.H * f.nchunk, f.nrow_q);
-    int rc = f.w_q == 1 ? launch_dq<T, KIND, DK, DVC, 1>(a, f, st) : (f.w_q == 2 ? launch_dq<T, KIND, DK, DVC, 2>(a, f, st) : launch_dq<T, KIND, DK, DVC, 4>(a, f, st));
+    // (two parts of dO at 256 columns: one workgroup a CU, so the longest walks first do by themselves; 4 x 4096 causal tokens, dv 1024: 298 us in the order for two, 250 so)
+    a.snake = a.dO_low && DVC == 256 ? f.nrow_q : snake_from(a, (long long)a.B * a.H * f.nchunk, f.nrow_q);
+    int rc;
+    if constexpr (sizeof(T) == 2) rc = a.dO_low ? pick_dq<T, KIND, DK, DVC, true>(a, f, st) : pick_dq<T, KIND, DK, DVC, false>(a, f, st);
+    else rc = pick_dq<T, KIND, DK, DVC, false>(a, f, st);
     if (rc != TLK_OK) return rc;
     a.nrow = f.nrow_k;
     if (f.w_k == 1) return launch_dkv<T, KIND, DK, DVC, 1>(a, f, st);
@@ -255,6 +264,7 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
         ga.dout = reinterpret_cast<const T *>(io.dout); ga.gate = reinterpret_cast<const T *>(a.gate); ga.o = reinterpret_cast<const T *>(io.o);
         for (int i = 0; i < 3; ++i) ga.gs[i] = a.gs[i];
         ga.dO = a.gate ? reinterpret_cast<T *>(ws + w.dO) : nullptr;
+        ga.low = a.gate && a.table && sizeof(T) == 2 ? reinterpret_cast<T *>(ws + w.low) : nullptr;
         ga.dgate = reinterpret_cast<T *>(io.dgate);
         ga.delta = kind == SOFTMAX ? reinterpret_cast<float *>(ws + w.delta) : nullptr;
         ga.rows = rows; ga.Lq = a.Lq; ga.H = a.H; ga.dv = a.dv;
@@ -266,6 +276,7 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
         TLK_HIP(hipGetLastError());
         if (a.gate) a.dO = ws + w.dO;
         a.delta = ga.delta;
+        a.dO_low = ga.low;
     }
     a.dq = io.dq; a.dk_ = io.dk; a.dv_ = io.dv;
     a.dq_part = reinterpret_cast<float *>(ws + w.dq);
