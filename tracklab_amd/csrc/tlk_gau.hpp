@@ -785,11 +785,12 @@ template <class T> __device__ __forceinline__ float unhold(int e) { return !Ty<T
 // dQ and the bias gradient: W waves, MT x 16 queries each; walks the keys.  dS^T has a query in the column: its registers are the B operand of
 // dQ^T = K^T dS^T.  The bias gradient needs sums along diagonals: a tile that lies beyond +-D of all its queries is one sum in registers, one near
 // the diagonal goes through a wave's own (KT x BM) LDS tile and each lane sums two diagonals -- no atomics, the order is fixed.
-// Softmax: the score gradients of a row sum to zero, but with delta = dO . o from the rounded o they sum to eta = dO . (W v - o), and the two entries beyond
-// +-D, into which most pairs fall, take it up over all rows: against entries that cancel by nature it was 1e-2 of the gradient (1137 bf16 tokens, D 16).
-// What the row really sums to is known at the end of its walk; eta times the row's weight beyond +-D goes off those entries.  (Of one diagonal it is nothing.)
+// Softmax: the score gradients of a row sum to zero, but with delta = dO . o from rounded weights and the rounded o they sum to eta = dO . (W v - o), and an entry
+// that most pairs share takes it up over all rows: against sums that cancel by nature it was 1e-2 of the gradient (1137 bf16 tokens, D 16), and the whole of
+// it where all distances but one share an entry.  What the row really sums to is known at the end of its walk: eta times the row's weights goes off the sums, beyond +-D as
+// one product (the weights are summed on the way), within them in a second walk over the tiles near the diagonal, which forms S and W again and nothing else.
 // Bound by the vector work between three products per score tile: 4 x 4096 causal bf16 tokens, dk 128, dv 1024, relu^2: 250 us with two parts of dO, 176 with one; 4 x 2048 tokens, 16 heads of 64,
-// softmax, causal: 114 us (91 without eta).
+// softmax, causal: 129 us (91 without eta).
 // LOW: dO comes in two parts.  Rounded once, dO is off by the same amounts for all keys of its row; a bucket's sum over many pairs, which cancel, keeps that (bf16, 4 x 1024
 // tokens, relu^2: up to 1e-2 of the bias gradient).  One more product a tile, and its fragments: at 256 columns one wave a SIMD has the registers for them.
 template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE, bool LOW>
@@ -867,6 +868,59 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
     const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
     if (p.table) __syncthreads();
     const float flo = p.table ? tab[0] : 0.f, fhi = p.table ? tab[TW - 1] : 0.f;          // the bias beyond +-D
+    const auto place = [&](int j0) __attribute__((always_inline)) { return !p.table || j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3); };
+    const auto whole = [&](int j0) __attribute__((always_inline)) { return j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin) && i0 + MT * 16 <= p.Lq; };
+    // scale, bias and mask of a tile's scores
+    const auto scores = [&](f4 (&s)[MT][NS], int j0, bool full, int where) __attribute__((always_inline)) {
+        const float far = where == 1 ? fhi : flo;
+        if (full && where != 3) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[mt][n][r] = __builtin_fmaf(s[mt][n][r], sc, far);
+        } else {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const int i = i0 + mt * 16 + l, last = i >= p.Lq ? -1 : (p.causal ? min(ke - 1, i + q0) : ke - 1);
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    add_bias<1>(s[mt][n], sc, where == 3, tab + (p.D + MARGIN + j0 + n * 16 + g * 4 - i - q0), far);
+                    if (!full)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (j0 + n * 16 + g * 4 + r > last) s[mt][n][r] = -INFINITY;
+                }
+            }
+        }
+    };
+    // sums of the wave's tile along its diagonals, into the distance sums
+    const auto diagonals = [&](int j0) __attribute__((always_inline)) {
+                    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                    // lane n of each half walks half of the queries down the diagonal that begins n keys ahead; past the last key it goes on at the first, on the
+                    // diagonal 32 keys behind: all lanes read at every step, and the 63 diagonals are two sums a lane
+                    const int n = lane & 31, h0 = lane >> 5;
+                    float ahead = 0.f, behind = 0.f;
+        #pragma unroll 8
+                    for (int i = 0; i < MT * 8; ++i) {
+                        const int c = h0 * MT * 8 + i, r = c + n;
+                        const float x = tile[(r & 31) * LT + c];
+                        ahead += r < KT ? x : 0.f;
+                        behind += r < KT ? 0.f : x;
+                    }
+                    ahead = lanes_32<LaneAdd>(ahead);
+                    behind = lanes_32<LaneAdd>(behind);
+                    const int e = h0 ? n - KT : n, d = e + j0 - i0 - q0;                        // key - query within the tile, and between positions
+                    const float sum = h0 ? behind : ahead;
+                    hi += d >= p.D ? sum : 0.f;
+                    lo += d < p.D && d <= -p.D ? sum : 0.f;
+                    if (d < p.D && d > -p.D) dbw[d + p.D] += sum;
+                    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+    };
     const auto step = [&](const char *cur, char *next, int j0) __attribute__((always_inline)) {
         tiles_ready();
         K += kstep;
@@ -876,9 +930,8 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
             tv.issue(V, ke - j0 - KT, p.vs[1], next + TK::BYTES);
         }
         if (i0 >= p.Lq || (p.causal && j0 > pmax)) return;
-        const bool full = j0 + KT <= ke && (!p.causal || j0 + KT - 1 <= pmin) && i0 + MT * 16 <= p.Lq;
-        const int where = !p.table || j0 - pmax >= p.D ? 1 : (j0 + KT - 1 - pmin <= -p.D ? 2 : 3);
-        const float far = where == 1 ? fhi : flo;
+        const bool full = whole(j0);
+        const int where = place(j0);
         f4 s[MT][NS], dp[MT][NS];
         constexpr bool TIGHT = LOW ? DK > 64 && DVC == 128 : DK + DVC > 256;            // (fragments in flight: what the registers leave)
         constexpr int KS = DK / 32, VS = DVC / 32, BK = TIGHT ? 2 : batch(NS * KS), B = TIGHT ? 2 : 4, BC = TIGHT ? 2 : batch(DK / 16);
@@ -907,27 +960,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
         });
         fragments(cf, 0, kcol);
         __builtin_amdgcn_sched_barrier(0);
-        if (full && where != 3) {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int n = 0; n < NS; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[mt][n][r] = __builtin_fmaf(s[mt][n][r], sc, far);
-        } else {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const int i = i0 + mt * 16 + l, last = i >= p.Lq ? -1 : (p.causal ? min(ke - 1, i + q0) : ke - 1);
-#pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    add_bias<1>(s[mt][n], sc, where == 3, tab + (p.D + MARGIN + j0 + n * 16 + g * 4 - i - q0), far);
-                    if (!full)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (j0 + n * 16 + g * 4 + r > last) s[mt][n][r] = -INFINITY;
-                }
-            }
-        }
+        scores(s, j0, full, where);
         int right = where == 1 ? -1 : 0;                           // (opaque: of a choice between two sums the compiler makes an address, and memory of the registers)
         asm volatile("" : "+v"(right));
         const auto masked = [](float x, int m) __attribute__((always_inline)) { return __builtin_bit_cast(float, __builtin_bit_cast(int, x) & m); };
@@ -944,11 +977,6 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
                         all += x;
                         if constexpr (decltype(near)::value) {
                             tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = x;
-                            if (KIND == SOFTMAX) {
-                                const int away = j0 + n * 16 + g * 4 + r - (i0 + mt * 16 + l + q0);
-                                mhi[mt] += away >= p.D ? wgt : 0.f;
-                                mlo[mt] += away < p.D && away <= -p.D ? wgt : 0.f;
-                            }
                         } else {
                             mass += wgt;
                         }
@@ -966,31 +994,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
         };
         if (where == 3) gradients(std::true_type());
         else gradients(std::false_type());
-        if (where == 3) {
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            // lane n of each half walks half of the queries down the diagonal that begins n keys ahead; past the last key it goes on at the first, on the
-            // diagonal 32 keys behind: all lanes read at every step, and the 63 diagonals are two sums a lane
-            const int n = lane & 31, h0 = lane >> 5;
-            float ahead = 0.f, behind = 0.f;
-#pragma unroll 8
-            for (int i = 0; i < MT * 8; ++i) {
-                const int c = h0 * MT * 8 + i, r = c + n;
-                const float x = tile[(r & 31) * LT + c];
-                ahead += r < KT ? x : 0.f;
-                behind += r < KT ? 0.f : x;
-            }
-            ahead = lanes_32<LaneAdd>(ahead);
-            behind = lanes_32<LaneAdd>(behind);
-            const int e = h0 ? n - KT : n, d = e + j0 - i0 - q0;                        // key - query within the tile, and between positions
-            const float sum = h0 ? behind : ahead;
-            hi += d >= p.D ? sum : 0.f;
-            lo += d < p.D && d <= -p.D ? sum : 0.f;
-            if (d < p.D && d > -p.D) dbw[d + p.D] += sum;
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
+        if (where == 3) diagonals(j0);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const float f = hold<T, NS>(s[mt], ex[mt]);
@@ -1015,23 +1019,6 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
         }
         __builtin_amdgcn_s_waitcnt(0x0f70);                        // (vmcnt(0): nothing is on its way to LDS when the workgroup ends)
     }
-    if (p.table) {
-        if (KIND == SOFTMAX)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const float e = over_groups_sum(eta[mt]);          // (a chunk of dv has its part of eta: the parts' corrections add up as the entries do)
-                lo -= e * mlo[mt];
-                hi -= e * mhi[mt];
-            }
-        lo = lanes_all<LaneAdd, 64>(lo);
-        hi = lanes_all<LaneAdd, 64>(hi);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        const long long nr = (long long)p.B * p.nchunk * p.nrow * W, at = (((long long)b * p.nchunk + ch) * p.nrow + rt) * W + w;
-        float *dst = p.db_part + ((long long)h * nr + at) * NB;
-        for (int t = lane; t < NB; t += 64) dst[t] = t == 0 ? lo + (p.D == 0 ? hi : 0.f) : (t == NB - 1 ? hi : dbw[t]);
-    }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int i = i0 + mt * 16 + l;
@@ -1052,6 +1039,66 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
                 *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.dq) + row * p.dk + c) = y;
             }
         }
+    }
+    if (p.table) {
+        if constexpr (KIND == SOFTMAX) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                eta[mt] = over_groups_sum(eta[mt]);                // (a chunk of dv has its part of eta: the parts' corrections add up as the entries do)
+                lo -= eta[mt] * mlo[mt];
+                hi -= eta[mt] * mhi[mt];
+            }
+            const auto again = [&](const char *cur, char *next, int j0) __attribute__((always_inline)) {
+                if (!ONE) {
+                    tiles_ready();
+                    K += kstep;
+                    tk.issue(K, ke - j0 - KT, p.ks[1], next);
+                }
+                if (i0 >= p.Lq || (p.causal && j0 > pmax) || place(j0) != 3) return;
+                f4 s[MT][NS];
+                const int krow = TK::row_at(0, g, l);
+#pragma unroll
+                for (int n = 0; n < NS; ++n)
+#pragma unroll
+                    for (int ks = 0; ks < DK / 32; ++ks) {
+                        const V8 a = TK::row8(cur, krow, n, ks);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) s[mt][n] = Ty<T>::mma(a, qf[mt][ks], ks ? s[mt][n] : f4{0, 0, 0, 0});
+                    }
+                scores(s, j0, whole(j0), 3);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int n = 0; n < NS; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = -eta[mt] * pow2_(s[mt][n][r] - lse[mt]);
+                diagonals(j0);
+            };
+            if constexpr (ONE) {
+                if (0 < ke) again(buf0, buf1, 0);                  // (its keys are still there)
+            } else {
+                // the tiles that hold a distance within +-D of any of the workgroup's queries
+                const int first = max(0, rt * BM + q0 - p.D - KT + 2) / KT * KT, end = min(ke, min(p.Lq, rt * BM + BM) - 1 + q0 + p.D);
+                __syncthreads();                                   // the first walk's tiles are no longer read
+                if (first < end) {
+                    K = reinterpret_cast<const T *>(p.k) + b * p.ks[0] + hk * p.ks[2] + first * p.ks[1];
+                    tk.issue(K, ke - first, p.ks[1], buf0);
+                }
+                for (int j0 = first; j0 < end; j0 += 2 * KT) {
+                    again(buf0, buf1, j0);
+                    if (j0 + KT < end) again(buf1, buf0, j0 + KT);
+                }
+                __builtin_amdgcn_s_waitcnt(0x0f70);
+            }
+        }
+        lo = lanes_all<LaneAdd, 64>(lo);
+        hi = lanes_all<LaneAdd, 64>(hi);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const long long nr = (long long)p.B * p.nchunk * p.nrow * W, at = (((long long)b * p.nchunk + ch) * p.nrow + rt) * W + w;
+        float *dst = p.db_part + ((long long)h * nr + at) * NB;
+        for (int t = lane; t < NB; t += 64) dst[t] = t == 0 ? lo + (p.D == 0 ? hi : 0.f) : (t == NB - 1 ? hi : dbw[t]);
     }
 }
 
