@@ -51,7 +51,8 @@ struct Args {
     // backward
     const void *dO;                             // (B, Lq, H, dv) contiguous: the gradient behind the gate
     const void *dO_low;                         // the same shape: what dO's rounding left (16-bit types with a gate and a table)
-    const float *delta;                         // (B, Lq, H): sum_d dO o (softmax)
+    const float *dO_exp;                        // (B, Lq, H): dO stands at 2^-dO_exp of its row (float16 with a gate; null: as it is)
+    const float *delta;                         // (B, Lq, H): sum_d dO o (softmax), at dO's scale
     void *dq, *dk_, *dv_;
     float *dq_part, *dk_part, *dv_part;         // (chunk, B, Lq, H, dk); (chunk x part, B, Lk, Hk, dk), (part, B, Lk, Hk, dv): sums of several blocks, joined afterwards
     float *db_part;                             // (heads, B * chunk * nrow * waves, 2 D + 1)
@@ -709,12 +710,14 @@ template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(c
 
 // ----------------------------------------------------------------------------------------------------------------------------------- backward
 // behind the gate: dO = dout * gate, dgate = dout * O, delta = sum_d dO * O.  LANES lanes a row; bound by HBM (4 x 4096 rows of 1024 bf16: 28 us, 5 tensors of 34 MB, which the caches hold in part).
+// float16: dO stands at a power of two of its row, which puts the largest magnitude at 2^14 .. 2^15 -- the product of two float16 values reaches from 2^-48 to 2^32.
 // low: what rounding dO left; the product of two 16-bit values is dO + low exactly (16 bits of bfloat16, 22 of float16), and delta is formed from it.
+constexpr int NO_ROW = -100;                      // dO_exp of a row of zeros: below every other
 template <class T> struct GateArgs {
     const T *dout, *gate, *o;
     long long gs[3];
     T *dO, *low, *dgate;
-    float *delta;
+    float *delta, *dO_exp;
     long long rows;
     int Lq, H, dv;
 };
@@ -726,7 +729,22 @@ template <class T, int LANES> __global__ void __launch_bounds__(256) gate_bwd_ke
     if (row >= p.rows) return;
     const long long bi = row / p.H;
     const T *gp = p.gate ? p.gate + (bi / p.Lq) * p.gs[0] + (bi % p.Lq) * p.gs[1] + (row % p.H) * p.gs[2] : nullptr;
-    float d = 0.f;
+    float d = 0.f, scale = 1.f;
+    if constexpr (Ty<T>::scaled)
+        if (gp) {
+            float top = 0.f;
+            for (int c = lane * 4; c < p.dv; c += LANES * 4) {
+                const V4 du = *reinterpret_cast<const V4 *>(p.dout + row * p.dv + c), u = *reinterpret_cast<const V4 *>(gp + c);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf((float)du[r] * (float)u[r]));
+            }
+            top = lanes_all<LaneMax, LANES>(top);
+            int e = 0;                                            // (infinite: as it is)
+            if (top < INFINITY) (void)frexpf(top, &e), e -= 15;
+            if (top == 0.f) e = NO_ROW;
+            scale = ldexpf(1.f, -e);
+            if (lane == 0) p.dO_exp[row] = (float)e;
+        }
     for (int c = lane * 4; c < p.dv; c += LANES * 4) {
         const V4 du = *reinterpret_cast<const V4 *>(p.dout + row * p.dv + c), o = *reinterpret_cast<const V4 *>(p.o + row * p.dv + c);
         V4 a, b, rest;
@@ -734,7 +752,7 @@ template <class T, int LANES> __global__ void __launch_bounds__(256) gate_bwd_ke
             const V4 u = *reinterpret_cast<const V4 *>(gp + c);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float x = (float)du[r] * (float)u[r];
+                const float x = (float)du[r] * (float)u[r] * scale;
                 a[r] = (T)x;
                 rest[r] = (T)(x - (float)a[r]);
                 b[r] = (T)((float)du[r] * (float)o[r]);
@@ -752,14 +770,19 @@ template <class T, int LANES> __global__ void __launch_bounds__(256) gate_bwd_ke
     if (p.delta && lane == 0) p.delta[row] = d;
 }
 
-// dS of one pair from its score x (scaled, biased, masked: -inf; softmax in powers of two), dW and the row's statistics; w returns the weight
-template <int KIND> __device__ __forceinline__ float dscore(float x, float dw, float lse, float delta, float &w)
+// dS of one pair from its score x (scaled, biased, masked: -inf; softmax in powers of two), dW and the row's statistics; w returns the weight.  Where dO, and dW
+// with it, stand at 2^-e of their row, the weight takes 2^e: lse is given e lower (and delta as dW), or two = 2 * 2^e -- w is then twice the weight.
+template <int KIND, bool SCALED> __device__ __forceinline__ float dscore(float x, float dw, float lse, float delta, float two, float &w)
 {
     if (KIND == SOFTMAX) {
         w = pow2_(x - lse);
         return w * (dw - delta);
     }
     const float s = relu_(x);
+    if (SCALED) {
+        w = s * (s * two);
+        return s * two * dw;
+    }
     w = s * s;
     return 2.f * s * dw;
 }
@@ -833,7 +856,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
     }
     const int i0 = rt * BM + w * MT * 16;                                             // the wave's first query
     V8 qf[MT][DK / 32], df[MT][DVC / 32], dl[LOW ? MT : 1][LOW ? DVC / 32 : 1];
-    float lse[MT], del[MT];
+    float lse[MT], del[MT], up[Ty<T>::scaled ? MT : 1];                               // (up: what dO is to be multiplied by)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int i = i0 + mt * 16 + l;
@@ -852,6 +875,11 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
         }
         lse[mt] = KIND == SOFTMAX ? (ok ? p.lse[row] : INFINITY) : 0.f;
         del[mt] = KIND == SOFTMAX && ok && ch == 0 ? p.delta[row] : 0.f;              // (dW comes in chunks of dv: the subtraction belongs to one of them)
+        if constexpr (Ty<T>::scaled) {
+            const float e = p.dO_exp && ok ? p.dO_exp[row] : 0.f;
+            up[mt] = ldexpf(1.f, (int)e);
+            lse[mt] -= e;
+        }
     }
     const int pmin = i0 + q0, pmax = min(p.Lq, i0 + MT * 16) - 1 + q0;
     f4 acc[DK / 16][MT];
@@ -973,7 +1001,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float wgt;
-                        const float x = s[mt][n][r] = dscore<KIND>(s[mt][n][r], dp[mt][n][r], lse[mt], del[mt], wgt);
+                        const float x = s[mt][n][r] = dscore<KIND, Ty<T>::scaled>(s[mt][n][r], dp[mt][n][r], lse[mt], del[mt], Ty<T>::scaled ? 2.f * up[mt] : 2.f, wgt);
                         all += x;
                         if constexpr (decltype(near)::value) {
                             tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = x;
@@ -1044,7 +1072,9 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
         if constexpr (KIND == SOFTMAX) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                eta[mt] = over_groups_sum(eta[mt]);                // (a chunk of dv has its part of eta: the parts' corrections add up as the entries do)
+                eta[mt] = over_groups_sum(eta[mt]);
+                if constexpr (Ty<T>::scaled) eta[mt] /= up[mt];    // (the weights carry it)
+                // (a chunk of dv has its part of eta: the parts' corrections add up as the entries do)
                 lo -= eta[mt] * mlo[mt];
                 hi -= eta[mt] * mhi[mt];
             }
@@ -1108,16 +1138,17 @@ template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
 __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK + DVC == 256) ? 1 : 2) dkv_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
-    // float16 softmax: weights are at most 1, so one fixed power of two does for them: 2^14 higher no weight above 2^-28 is subnormal.  It comes with the
-    // log-sum-exp, for nothing; the score gradients carry it too.  (An exponent of their own, as the squares have: 6 x 1021 tokens, 8 heads, 72 and 104
-    // columns 124 us, so 100.)
-    constexpr float UP = KIND == SOFTMAX && Ty<T>::scaled ? 14.f : 0.f;
+    // float16 softmax: weights are at most 1, and 2^14 higher none above 2^-28 is subnormal.  Behind a gate a weight takes 2^e of its row's dO, and the largest e
+    // of the rows walked so far goes off all of them: one power of two, raised with the walk, that comes with the log-sum-exp; the score gradients carry it too.
+    // (An exponent for every key, as the squares have: 6 x 1021 tokens, 8 heads, 72 and 104 columns 124 us; factors of the weights 132; so 119.)
+    constexpr bool SOFT16 = KIND == SOFTMAX && Ty<T>::scaled;
+    constexpr float HIGH = 14.f;
     constexpr int QT = 32, NTH = 64 * W, BN = W * MT * 16, NS = 2;
     using TQ = Tile<T, QT, tile_width(DK), W>;
     using TO = Tile<T, QT, DVC, W>;
     constexpr int BUF = TQ::BYTES + TO::BYTES;
     __shared__ __attribute__((aligned(1024))) char buf0[BUF], buf1[ONE ? 16 : BUF];     // (two objects: see fwd_kernel)
-    __shared__ __attribute__((aligned(16))) float stats0[2 * QT], stats1[2 * QT];       // the tiles' log-sum-exp and delta
+    __shared__ __attribute__((aligned(16))) float stats0[2 * QT + 4], stats1[2 * QT + 4];       // the tiles' log-sum-exp, delta (float16 relu^2: 2 * 2^e), power of two (SOFT16)
     extern __shared__ __attribute__((aligned(16))) float tab[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15, G = p.H / p.Hk, TW = table_width(p.D);
     int id = blockIdx.x;
@@ -1148,6 +1179,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         for (int n = 0; n < DK / 16; ++n) ak[n][mt] = f4{0, 0, 0, 0};
     }
     int ev[MT], ek[MT];
+    float walked = p.dO_exp ? (float)NO_ROW : 0.f, held = walked;                       // SOFT16: the rows' largest e so far (the first wave's), and what the sums stand at
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) ev[mt] = ek[mt] = E_NONE;
     const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
@@ -1165,20 +1197,29 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         const long long qstep = QT * p.qs[1], ostep = (long long)QT * p.H * p.dv;
         const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2] + ib * p.qs[1];              // (the tiles in turn: Q and dO move along)
         const T *dO = reinterpret_cast<const T *>(p.dO) + (((long long)b * p.Lq + ib) * p.H + h) * p.dv + c0;
-        float ls0 = INFINITY, dl0 = 0.f;
+        float ls0 = INFINITY, dl0 = 0.f, e0 = 0.f;
         const auto issue = [&](int i, char *buf) __attribute__((always_inline)) {
             if (buf) {
                 tq.issue(Q, p.Lq - i, p.qs[1], buf);
                 to.issue(dO, p.Lq - i, (long long)p.H * p.dv, buf + TQ::BYTES);
             }
-            if (KIND == SOFTMAX && tid < QT) {
+            if ((KIND == SOFTMAX || Ty<T>::scaled) && tid < QT) {
                 const long long row = ((long long)b * p.Lq + i + tid) * p.H + h;
-                ls0 = i + tid < p.Lq ? p.lse[row] : INFINITY;
-                dl0 = i + tid < p.Lq && ch == 0 ? p.delta[row] : 0.f;
+                const bool ok = i + tid < p.Lq;
+                if (Ty<T>::scaled) e0 = !p.dO_exp ? 0.f : (ok ? p.dO_exp[row] : (float)NO_ROW);
+                if (KIND == SOFTMAX) {
+                    ls0 = ok ? p.lse[row] - e0 : INFINITY;
+                    dl0 = ok && ch == 0 ? p.delta[row] : 0.f;
+                }
             }
         };
         const auto keep = [&](float *st) __attribute__((always_inline)) {
-            if (KIND == SOFTMAX && tid < QT) { st[tid] = ls0 - UP; st[QT + tid] = dl0; }
+            if (SOFT16 && p.dO_exp && w == 0) {
+                walked = fmaxf(walked, lanes_all<LaneMax, 32>(e0));
+                if (tid == 0) st[2 * QT] = walked;
+            }
+            if (KIND == SOFTMAX && tid < QT) { st[tid] = SOFT16 ? ls0 + (walked - HIGH) : ls0; st[QT + tid] = dl0; }
+            if (KIND == RELU2 && Ty<T>::scaled && tid < QT) st[QT + tid] = ldexpf(2.f, (int)e0);
         };
         __syncthreads();                                                                  // the previous head's tiles and table are no longer read
         if (ib < p.Lq) {
@@ -1253,26 +1294,38 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
                     }
                 }
             }
+            if (SOFT16 && p.dO_exp) {
+                const float e = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(st[2 * QT])));
+                if (e > held) {
+                    const float f = ldexpf(1.f, (int)(held - e));
+                    held = e;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                        for (int n = 0; n < DVC / 16; ++n) av[n][mt] *= f;
+#pragma unroll
+                        for (int n = 0; n < DK / 16; ++n) ak[n][mt] *= f;
+                    }
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
                 f4 ls = {0, 0, 0, 0}, dl = {0, 0, 0, 0};
-                if (KIND == SOFTMAX) {
-                    ls = *reinterpret_cast<const f4 *>(st + n * 16 + g * 4);
-                    dl = *reinterpret_cast<const f4 *>(st + QT + n * 16 + g * 4);
-                }
+                if (KIND == SOFTMAX) ls = *reinterpret_cast<const f4 *>(st + n * 16 + g * 4);
+                if (KIND == SOFTMAX || Ty<T>::scaled) dl = *reinterpret_cast<const f4 *>(st + QT + n * 16 + g * 4);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float wgt;
-                        s[mt][n][r] = dscore<KIND>(s[mt][n][r], wt[mt][n][r], ls[r], dl[r], wgt);
+                        s[mt][n][r] = dscore<KIND, Ty<T>::scaled>(s[mt][n][r], wt[mt][n][r], ls[r], dl[r], dl[r], wgt);
                         wt[mt][n][r] = wgt;
                     }
             }
             V8 wb[MT], db[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const float fv = UP != 0.f ? 1.f : hold<T, NS>(wt[mt], ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
+                const float fv = SOFT16 ? 1.f : hold<T, NS>(wt[mt], ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
                 if (Ty<T>::scaled && __any(fv != 1.f))
 #pragma unroll
                     for (int n = 0; n < DVC / 16; ++n) av[n][mt] *= fv;
@@ -1308,7 +1361,8 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         const int j = j0 + mt * 16 + l;
         if (j >= p.Lk) continue;
         const long long row = ((long long)b * p.Lk + j) * p.Hk + hk;
-        const float down = ldexpf(1.f, -(int)UP), finv = UP != 0.f ? down : unhold<T>(ev[mt]), fink = p.scale * unhold<T>(ek[mt]) * down;
+        const float down = SOFT16 ? ldexpf(1.f, (int)(held - HIGH)) : 1.f, finv = SOFT16 ? down : unhold<T>(ev[mt]) * (Ty<T>::scaled ? 0.5f : 1.f),
+                    fink = p.scale * unhold<T>(ek[mt]) * down;
         typename Ty<T>::V4 y;
 #pragma unroll
         for (int n = 0; n < DVC / 16; ++n) {

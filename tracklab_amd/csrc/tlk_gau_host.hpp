@@ -74,7 +74,7 @@ inline BwdPlan plan_backward(const Args &a, int elem)
 constexpr int DB_SPLITS = 64;
 
 struct BwdWs {
-    long long dO, low, delta, dq, dk, dv, db, db2, total;
+    long long dO, low, exp, delta, dq, dk, dv, db, db2, total;
 };
 inline BwdWs layout_backward(const Args &a, int kind, int elem, const BwdPlan &f)
 {
@@ -84,6 +84,7 @@ inline BwdWs layout_backward(const Args &a, int kind, int elem, const BwdPlan &f
     const auto take = [&](long long bytes) { const long long r = at; at += align_up(bytes); return r; };
     w.dO = take(a.gate ? rows * a.dv * elem : 0);
     w.low = take(a.gate && a.table && elem == 2 ? rows * a.dv * elem : 0);
+    w.exp = take(a.gate && elem == 2 ? rows * 4 : 0);
     w.delta = take(kind == SOFTMAX ? rows * 4 : 0);
     w.dq = take(f.nchunk > 1 ? rows * a.dk * f.nchunk * 4 : 0);
     w.dk = take(f.nchunk * f.nparts > 1 ? keys * a.dk * f.nchunk * f.nparts * 4 : 0);
@@ -224,8 +225,8 @@ template <class T, int KIND, int DK, int DVC, int W> int launch_dkv(const Args &
     const size_t fixed = sizeof(T) * 32 * (tile_width(DK) + DVC), smem = a.table ? sizeof(float) * table_width(a.D) : 0;
     const long long blocks = (long long)a.B * a.Hk * f.nchunk * f.nparts * f.nrow_k;
     if constexpr (W < 4)
-        if (a.Lq <= 32) return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, true>, blocks, 64 * W, fixed + 512, smem, a, st);
-    return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, false>, blocks, 64 * W, 2 * fixed + 512, smem, a, st);
+        if (a.Lq <= 32) return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, true>, blocks, 64 * W, fixed + 544, smem, a, st);
+    return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, false>, blocks, 64 * W, 2 * fixed + 544, smem, a, st);
 }
 template <class T, int KIND, int DK, int DVC> int pick_bwd(Args a, const BwdPlan &f, hipStream_t st)
 {
@@ -265,6 +266,7 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
         for (int i = 0; i < 3; ++i) ga.gs[i] = a.gs[i];
         ga.dO = a.gate ? reinterpret_cast<T *>(ws + w.dO) : nullptr;
         ga.low = a.gate && a.table && sizeof(T) == 2 ? reinterpret_cast<T *>(ws + w.low) : nullptr;
+        ga.dO_exp = a.gate && Ty<T>::scaled ? reinterpret_cast<float *>(ws + w.exp) : nullptr;
         ga.dgate = reinterpret_cast<T *>(io.dgate);
         ga.delta = kind == SOFTMAX ? reinterpret_cast<float *>(ws + w.delta) : nullptr;
         ga.rows = rows; ga.Lq = a.Lq; ga.H = a.H; ga.dv = a.dv;
@@ -277,6 +279,7 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
         if (a.gate) a.dO = ws + w.dO;
         a.delta = ga.delta;
         a.dO_low = ga.low;
+        a.dO_exp = ga.dO_exp;
     }
     a.dq = io.dq; a.dk_ = io.dk; a.dv_ = io.dv;
     a.dq_part = reinterpret_cast<float *>(ws + w.dq);
