@@ -74,3 +74,12 @@ def test_rows_of_zeros_and_a_row_that_is_not_a_number():
         bad["dout"][0, 33, 0, 5] = float("inf")
         dq = X.run(bad, kind)["dq"]
         assert not dq[0, 33].isfinite().all() and torch.equal(dq[0, :33], got["dq"][0, :33]) and torch.equal(dq[0, 34:], got["dq"][0, 34:])
+
+
+def test_values_before_the_gate_beyond_the_largest_number():
+    """relu^2 weights of hundreds: o above 65504 behind gates that bring it back; the gate's gradient is dout * o"""
+    for B, Lq, Lk, dv in ((2, 300, 300, 64), (2, 17, 40, 512), (1, 4, 2000, 72)):
+        t = X.inputs(6, F16, B, Lq, Lk, 1, 1, 64, dv, True, 0, std={"q": 8.0, "k": 8.0, "gate": 2.0 ** -9, "dout": 2.0 ** -11, "v": 4.0})
+        got, want = X.run(t, "relu2"), X.attention(t, "relu2")
+        assert float((want["dgate"].abs() / t["dout"].double().abs().clamp(min=1e-30)).max()) > 65504
+        _close(got, want, ("out", "dgate", "dv"))

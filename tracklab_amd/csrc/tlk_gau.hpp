@@ -83,6 +83,16 @@ template <> struct Ty<float> {
     }
 };
 
+// o as it is kept for the backward pass: float16 relu^2 weights are no shares of one, and o may pass 65504 where the gate brings the result back
+template <class T, int KIND> using Kept = std::conditional_t<KIND == RELU2 && Ty<T>::scaled, float, T>;
+template <class O> __device__ __forceinline__ void keep4(void *o, long long at, f4 x)
+{
+    typename Ty<O>::V4 y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = (O)x[r];
+    *reinterpret_cast<typename Ty<O>::V4 *>(reinterpret_cast<O *>(o) + at) = y;
+}
+
 template <class T> __device__ __forceinline__ typename Ty<T>::V8 zero8()
 {
     typename Ty<T>::V8 r;
@@ -594,10 +604,15 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
                 for (int e = 0; e < VN; e += 4) *reinterpret_cast<f4 *>(x + e) = *reinterpret_cast<const f4 *>(res + er * LDE + ec + e);
                 u4 raw;
                 if (p.o) {
+                    if constexpr (std::is_same_v<Kept<T, KIND>, T>) {
 #pragma unroll
-                    for (int e = 0; e < VN; ++e) y[e] = (T)x[e];
-                    __builtin_memcpy(&raw, y, 16);
-                    *reinterpret_cast<u4 *>(reinterpret_cast<T *>(p.o) + at) = raw;
+                        for (int e = 0; e < VN; ++e) y[e] = (T)x[e];
+                        __builtin_memcpy(&raw, y, 16);
+                        *reinterpret_cast<u4 *>(reinterpret_cast<T *>(p.o) + at) = raw;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VN; e += 4) *reinterpret_cast<f4 *>(reinterpret_cast<float *>(p.o) + at + e) = *reinterpret_cast<const f4 *>(x + e);
+                    }
                 }
 #pragma unroll
                 for (int e = 0; e < VN; ++e) y[e] = (T)(p.gate ? x[e] * (float)u[e] : x[e]);
@@ -638,11 +653,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
             f4 x = acc[n][mt] * fin;
             if (TWICE) x *= fin;
             typename Ty<T>::V4 y;
-            if (p.o) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
-                *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.o) + row * p.dv + c) = y;
-            }
+            if (p.o) keep4<Kept<T, KIND>>(p.o, row * p.dv + c, x);
             if (gp) {
                 const typename Ty<T>::V4 u = *reinterpret_cast<const typename Ty<T>::V4 *>(gp + c);
 #pragma unroll
@@ -693,11 +704,7 @@ template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(c
     const int h = (int)(row % p.H);
     const long long bi = row / p.H;
     typename Ty<T>::V4 y;
-    if (p.o) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = (T)x[r];
-        *reinterpret_cast<typename Ty<T>::V4 *>(reinterpret_cast<T *>(p.o) + row * p.dv + c) = y;
-    }
+    if (p.o) keep4<Kept<T, KIND>>(p.o, row * p.dv + c, x);
     if (p.gate) {
         const typename Ty<T>::V4 u = *reinterpret_cast<const typename Ty<T>::V4 *>(reinterpret_cast<const T *>(p.gate) + (bi / p.Lq) * p.gs[0] + (bi % p.Lq) * p.gs[1] + h * p.gs[2] + c);
 #pragma unroll
@@ -714,14 +721,15 @@ template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(c
 // low: what rounding dO left; the product of two 16-bit values is dO + low exactly (16 bits of bfloat16, 22 of float16), and delta is formed from it.
 constexpr int NO_ROW = -100;                      // dO_exp of a row of zeros: below every other
 template <class T> struct GateArgs {
-    const T *dout, *gate, *o;
+    const T *dout, *gate;
+    const void *o;
     long long gs[3];
     T *dO, *low, *dgate;
     float *delta, *dO_exp;
     long long rows;
     int Lq, H, dv;
 };
-template <class T, int LANES> __global__ void __launch_bounds__(256) gate_bwd_kernel(const GateArgs<T> p)
+template <class T, class O, int LANES> __global__ void __launch_bounds__(256) gate_bwd_kernel(const GateArgs<T> p)
 {
     using V4 = typename Ty<T>::V4;
     const long long row = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
@@ -746,7 +754,8 @@ template <class T, int LANES> __global__ void __launch_bounds__(256) gate_bwd_ke
             if (lane == 0) p.dO_exp[row] = (float)e;
         }
     for (int c = lane * 4; c < p.dv; c += LANES * 4) {
-        const V4 du = *reinterpret_cast<const V4 *>(p.dout + row * p.dv + c), o = *reinterpret_cast<const V4 *>(p.o + row * p.dv + c);
+        const V4 du = *reinterpret_cast<const V4 *>(p.dout + row * p.dv + c);
+        const auto o = *reinterpret_cast<const typename Ty<O>::V4 *>(reinterpret_cast<const O *>(p.o) + row * p.dv + c);
         V4 a, b, rest;
         if (gp) {
             const V4 u = *reinterpret_cast<const V4 *>(gp + c);

@@ -262,7 +262,7 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
     a.dO = io.dout;
     if ((a.gate || kind == SOFTMAX) && rows > 0) {
         GateArgs<T> ga;
-        ga.dout = reinterpret_cast<const T *>(io.dout); ga.gate = reinterpret_cast<const T *>(a.gate); ga.o = reinterpret_cast<const T *>(io.o);
+        ga.dout = reinterpret_cast<const T *>(io.dout); ga.gate = reinterpret_cast<const T *>(a.gate); ga.o = io.o;
         for (int i = 0; i < 3; ++i) ga.gs[i] = a.gs[i];
         ga.dO = a.gate ? reinterpret_cast<T *>(ws + w.dO) : nullptr;
         ga.low = a.gate && a.table && sizeof(T) == 2 ? reinterpret_cast<T *>(ws + w.low) : nullptr;
@@ -273,7 +273,8 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
         const int lanes = a.dv <= 64 ? 16 : (a.dv <= 128 ? 32 : 64);
         const long long blocks = (rows + 256 / lanes - 1) / (256 / lanes);
         if (blocks > 0x7fffffffLL) return fail(TLK_EINVAL, "tlk_gau_attention: more than 2^31 - 1 workgroups");
-        const auto kernel = lanes == 16 ? gate_bwd_kernel<T, 16> : (lanes == 32 ? gate_bwd_kernel<T, 32> : gate_bwd_kernel<T, 64>);
+        const auto by_lanes = [&](auto o) { using O = decltype(o); return lanes == 16 ? gate_bwd_kernel<T, O, 16> : (lanes == 32 ? gate_bwd_kernel<T, O, 32> : gate_bwd_kernel<T, O, 64>); };
+        const auto kernel = kind == RELU2 ? by_lanes(Kept<T, RELU2>()) : by_lanes(Kept<T, SOFTMAX>());
         hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, ga);
         TLK_HIP(hipGetLastError());
         if (a.gate) a.dO = ws + w.dO;
