@@ -844,8 +844,8 @@ int tlk_reid_part_head(const void *feat_dev, int feat_pix_stride, int dtype, int
  *   batch, row and head, the last dimension contiguous; every stride a multiple of 16 bytes, row strides of q, k, v between the width and 2^22 elements, every pointer 16-byte aligned; dim_k <= 128 and dim_v
  *   multiples of 16 bytes of elements.  table (num_buckets, heads) of `dtype` or (table_f32) float32, bucket_of (2 * max_distance + 1) int32 (values are clipped to
  *   0..num_buckets - 1); num_buckets 0: no bias.  max_distance <= 2048.  out, o_raw, dq.. are contiguous (batch, len, heads, dim).
- *   o_raw (nullable): o before the gate, of `dtype` (float16 relu^2: float32, since it may pass 65504 where out does not), lse (nullable, softmax): log2 sum_j 2^(S log2 e) per (batch, len_q, heads), +inf for a row without keys: what
- *   the backward call takes.  Products run on the matrix cores in `dtype` and are summed in float32; weights are rounded to `dtype` for the second product
+ *   o_raw (nullable): o before the gate, of `dtype` (float16 relu^2: float32, since it may pass 65504 where out does not), lse (nullable, softmax): float32 (batch, len_q, heads, 2),
+ *   a row's largest x = S log2 e and log2 sum_j 2^(x_j - largest), the latter +inf for a row without keys: what the backward call takes.  Products run on the matrix cores in `dtype` and are summed in float32; weights are rounded to `dtype` for the second product
  *   (float16: with a power of two per row, so weights beyond its range survive), o and out once.
  * tlk_gau_attention_bwd:  dout, o_raw (needed with a gate or softmax), lse (softmax) -> dq, dk, dv, dgate (with a gate), dtable (with a table); weights
  *   are formed again from q and k.  With shared key heads the gradients of the sharing heads are summed in float32.  No atomics: equal bits on every run.

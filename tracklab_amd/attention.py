@@ -150,13 +150,13 @@ def _gau_args(q, k, v, gate, table, buckets, lens, q_start, kind, causal, scale)
 
 
 def _gau_forward(q, k, v, gate, table, buckets, lens, q_start, kind, causal, scale, keep):
-    """out, and for the backward pass what it needs of (o before the gate, log-sum-exp)"""
+    """out, and for the backward pass what it needs of (o before the gate, a softmax row's maximum and sum)"""
     L, dev = _bound(), q.device
     a, held = _gau_args(q, k, v, gate, table, buckets, lens, q_start, kind, causal, scale)
     shape = (*q.shape[:3], v.shape[3])
     out = torch.empty(shape, dtype=q.dtype, device=dev)
     o = torch.empty(shape, dtype=torch.float32 if kind == 0 and q.dtype == torch.float16 else q.dtype, device=dev) if keep and gate is not None else None
-    lse = torch.empty(shape[:3], dtype=torch.float32, device=dev) if keep and kind == 1 else None
+    lse = torch.empty((*shape[:3], 2), dtype=torch.float32, device=dev) if keep and kind == 1 else None
     with _on(dev):
         n = L.tlk_gau_attention_workspace(a, 0) if k.shape[1] > 512 else 0            # (up to 512 keys a forward call needs none)
         ws = _bytes(n, dev)

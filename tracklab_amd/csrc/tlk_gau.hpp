@@ -45,7 +45,7 @@ struct Args {
     float scale;
     // forward
     void *out, *o;
-    float *lse;                                 // (B, Lq, H): log2 of the row's sum of 2^(S log2 e), +inf for a row without keys
+    float *lse;                                 // (B, Lq, H, 2): the row's largest x = S log2 e, and log2 of its sum of 2^(x - largest), +inf for a row without keys
     float *part, *ml;                           // split keys: (split, B, Lq, H, dv) sums and (split, B, Lq, H, 2) maximum and sum
     int nsplit, split_keys, nchunk, nrow, fold, nparts, snake;
     // backward
@@ -336,6 +336,14 @@ template <int STEP> __device__ __forceinline__ void add_bias(f4 &s, float sc, bo
     }
 }
 
+// The statistics of a softmax row.  Two numbers: next to a largest score of 10^4 and more, log2 of the sum is rounded away in one (float32, all keys of a row at a
+// bias of -10^9: every weight 1 in the backward pass where it is one share of n).
+__device__ __forceinline__ void keep_sum(float *lse, long long row, float m, float sum)
+{
+    lse[2 * row] = m;
+    lse[2 * row + 1] = sum == 0.f ? INFINITY : log2f(sum);
+}
+
 // ------------------------------------------------------------------------------------------------------------------------------------ forward
 // WM x WN waves; a wave owns MT x 16 rows and NT x 16 columns of the output.  Rows of a block are (head of the group, query) pairs when p.fold
 // (few queries: the heads that share keys and values are answered in one pass over them).
@@ -578,8 +586,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
             if (KIND == SOFTMAX) {
                 lsum[mt] = over_groups_sum(lsum[mt]);
                 fin = lsum[mt] == 0.f ? 0.f : 1.f / lsum[mt];
-                if (p.lse && ok[mt] && c0 == 0 && wn == 0 && g == 0)
-                    p.lse[((long long)b * p.Lq + qi[mt]) * p.H + h0 + qh[mt]] = lsum[mt] == 0.f ? INFINITY : m[mt] + log2f(lsum[mt]);
+                if (p.lse && ok[mt] && c0 == 0 && wn == 0 && g == 0) keep_sum(p.lse, ((long long)b * p.Lq + qi[mt]) * p.H + h0 + qh[mt], m[mt], lsum[mt]);
             } else if (Ty<T>::scaled) {
                 fin = ex[mt] == E_NONE ? 0.f : ldexpf(1.f, ex[mt]);
             }
@@ -644,7 +651,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WN > 1 && sizeof(T) == 2 ? (MT *
             }
             continue;
         }
-        if (p.lse && c0 == 0 && wn == 0 && g == 0) p.lse[row] = lsum[mt] == 0.f ? INFINITY : m[mt] + log2f(lsum[mt]);
+        if (p.lse && c0 == 0 && wn == 0 && g == 0) keep_sum(p.lse, row, m[mt], lsum[mt]);
         const T *gp = p.gate ? reinterpret_cast<const T *>(p.gate) + b * p.gs[0] + (long long)qi[mt] * p.gs[1] + (h0 + qh[mt]) * p.gs[2] : nullptr;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -698,7 +705,7 @@ template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(c
     if (KIND == SOFTMAX) {
         s = over_groups_sum(s);
         x *= s == 0.f ? 0.f : 1.f / s;
-        if (p.lse && c == 0 && lane == 0) p.lse[row] = s == 0.f ? INFINITY : m + log2f(s);
+        if (p.lse && c == 0 && lane == 0) keep_sum(p.lse, row, m, s);
     }
     if (!in || g) return;
     const int h = (int)(row % p.H);
@@ -780,11 +787,11 @@ template <class T, class O, int LANES> __global__ void __launch_bounds__(256) ga
 }
 
 // dS of one pair from its score x (scaled, biased, masked: -inf; softmax in powers of two), dW and the row's statistics; w returns the weight.  Where dO, and dW
-// with it, stand at 2^-e of their row, the weight takes 2^e: lse is given e lower (and delta as dW), or two = 2 * 2^e -- w is then twice the weight.
-template <int KIND, bool SCALED> __device__ __forceinline__ float dscore(float x, float dw, float lse, float delta, float two, float &w)
+// with it, stand at 2^-e of their row, the weight takes 2^e: lsum is given e lower (and delta as dW), or two = 2 * 2^e -- w is then twice the weight.
+template <int KIND, bool SCALED> __device__ __forceinline__ float dscore(float x, float dw, float top, float lsum, float delta, float two, float &w)
 {
     if (KIND == SOFTMAX) {
-        w = pow2_(x - lse);
+        w = pow2_(x - top - lsum);
         return w * (dw - delta);
     }
     const float s = relu_(x);
@@ -822,7 +829,7 @@ template <class T> __device__ __forceinline__ float unhold(int e) { return !Ty<T
 // it where all distances but one share an entry.  What the row really sums to is known at the end of its walk: eta times the row's weights goes off the sums, beyond +-D as
 // one product (the weights are summed on the way), within them in a second walk over the tiles near the diagonal, which forms S and W again and nothing else.
 // Bound by the vector work between three products per score tile: 4 x 4096 causal bf16 tokens, dk 128, dv 1024, relu^2: 250 us with two parts of dO, 176 with one; 4 x 2048 tokens, 16 heads of 64,
-// softmax, causal: 129 us (91 without eta).
+// softmax, causal: 134 us (of it 38 for eta and 5 for the second statistic of a row).
 // LOW: dO comes in two parts.  Rounded once, dO is off by the same amounts for all keys of its row; a bucket's sum over many pairs, which cancel, keeps that (bf16, 4 x 1024
 // tokens, relu^2: up to 1e-2 of the bias gradient).  One more product a tile, and its fragments: at 256 columns one wave a SIMD has the registers for them.
 template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE, bool LOW>
@@ -865,7 +872,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
     }
     const int i0 = rt * BM + w * MT * 16;                                             // the wave's first query
     V8 qf[MT][DK / 32], df[MT][DVC / 32], dl[LOW ? MT : 1][LOW ? DVC / 32 : 1];
-    float lse[MT], del[MT], up[Ty<T>::scaled ? MT : 1];                               // (up: what dO is to be multiplied by)
+    float top[MT], lsum[MT], del[MT], up[Ty<T>::scaled ? MT : 1];                               // (up: what dO is to be multiplied by)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int i = i0 + mt * 16 + l;
@@ -882,12 +889,13 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
 #pragma unroll
             for (int ks = 0; ks < DVC / 32; ++ks) dl[mt][ks] = ld8(lsrc + ks * 32, ok ? cend - ks * 32 - g * 8 : 0);
         }
-        lse[mt] = KIND == SOFTMAX ? (ok ? p.lse[row] : INFINITY) : 0.f;
+        top[mt] = KIND == SOFTMAX && ok ? p.lse[2 * row] : 0.f;
+        lsum[mt] = KIND == SOFTMAX ? (ok ? p.lse[2 * row + 1] : INFINITY) : 0.f;
         del[mt] = KIND == SOFTMAX && ok && ch == 0 ? p.delta[row] : 0.f;              // (dW comes in chunks of dv: the subtraction belongs to one of them)
         if constexpr (Ty<T>::scaled) {
             const float e = p.dO_exp && ok ? p.dO_exp[row] : 0.f;
             up[mt] = ldexpf(1.f, (int)e);
-            lse[mt] -= e;
+            lsum[mt] -= e;
         }
     }
     const int pmin = i0 + q0, pmax = min(p.Lq, i0 + MT * 16) - 1 + q0;
@@ -1010,7 +1018,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float wgt;
-                        const float x = s[mt][n][r] = dscore<KIND, Ty<T>::scaled>(s[mt][n][r], dp[mt][n][r], lse[mt], del[mt], Ty<T>::scaled ? 2.f * up[mt] : 2.f, wgt);
+                        const float x = s[mt][n][r] = dscore<KIND, Ty<T>::scaled>(s[mt][n][r], dp[mt][n][r], top[mt], lsum[mt], del[mt], Ty<T>::scaled ? 2.f * up[mt] : 2.f, wgt);
                         all += x;
                         if constexpr (decltype(near)::value) {
                             tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = x;
@@ -1110,7 +1118,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
 #pragma unroll
                     for (int n = 0; n < NS; ++n)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = -eta[mt] * pow2_(s[mt][n][r] - lse[mt]);
+                        for (int r = 0; r < 4; ++r) tile[(n * 16 + g * 4 + r) * LT + mt * 16 + l] = -eta[mt] * pow2_(s[mt][n][r] - top[mt] - lsum[mt]);
                 diagonals(j0);
             };
             if constexpr (ONE) {
@@ -1142,7 +1150,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
 }
 
 // dK and dV: W waves, MT x 16 keys each; walks the queries of every head that shares the keys.  S has a key in the column: W and dS in registers
-// are the B operands of dV^T = dO^T W and dK^T = Q^T dS.  Bound as dq, with four products and twice the accumulators: 254 and 106 us at its two sizes.
+// are the B operands of dV^T = dO^T W and dK^T = Q^T dS.  Bound as dq, with four products and twice the accumulators: 254 and 112 us at its two sizes.
 template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
 __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK + DVC == 256) ? 1 : 2) dkv_kernel(const Args p)
 {
@@ -1157,7 +1165,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
     using TO = Tile<T, QT, DVC, W>;
     constexpr int BUF = TQ::BYTES + TO::BYTES;
     __shared__ __attribute__((aligned(1024))) char buf0[BUF], buf1[ONE ? 16 : BUF];     // (two objects: see fwd_kernel)
-    __shared__ __attribute__((aligned(16))) float stats0[2 * QT + 4], stats1[2 * QT + 4];       // the tiles' log-sum-exp, delta (float16 relu^2: 2 * 2^e), power of two (SOFT16)
+    __shared__ __attribute__((aligned(16))) float stats0[3 * QT + 4], stats1[3 * QT + 4];       // the tiles' delta (float16 relu^2: 2 * 2^e), maximum, log2 of the sum, power of two (SOFT16)
     extern __shared__ __attribute__((aligned(16))) float tab[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15, G = p.H / p.Hk, TW = table_width(p.D);
     int id = blockIdx.x;
@@ -1206,7 +1214,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         const long long qstep = QT * p.qs[1], ostep = (long long)QT * p.H * p.dv;
         const T *Q = reinterpret_cast<const T *>(p.q) + b * p.qs[0] + h * p.qs[2] + ib * p.qs[1];              // (the tiles in turn: Q and dO move along)
         const T *dO = reinterpret_cast<const T *>(p.dO) + (((long long)b * p.Lq + ib) * p.H + h) * p.dv + c0;
-        float ls0 = INFINITY, dl0 = 0.f, e0 = 0.f;
+        float tp0 = 0.f, ls0 = INFINITY, dl0 = 0.f, e0 = 0.f;
         const auto issue = [&](int i, char *buf) __attribute__((always_inline)) {
             if (buf) {
                 tq.issue(Q, p.Lq - i, p.qs[1], buf);
@@ -1217,7 +1225,8 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
                 const bool ok = i + tid < p.Lq;
                 if (Ty<T>::scaled) e0 = !p.dO_exp ? 0.f : (ok ? p.dO_exp[row] : (float)NO_ROW);
                 if (KIND == SOFTMAX) {
-                    ls0 = ok ? p.lse[row] - e0 : INFINITY;
+                    tp0 = ok ? p.lse[2 * row] : 0.f;
+                    ls0 = ok ? p.lse[2 * row + 1] - e0 : INFINITY;
                     dl0 = ok && ch == 0 ? p.delta[row] : 0.f;
                 }
             }
@@ -1225,10 +1234,10 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         const auto keep = [&](float *st) __attribute__((always_inline)) {
             if (SOFT16 && p.dO_exp && w == 0) {
                 walked = fmaxf(walked, lanes_all<LaneMax, 32>(e0));
-                if (tid == 0) st[2 * QT] = walked;
+                if (tid == 0) st[3 * QT] = walked;
             }
-            if (KIND == SOFTMAX && tid < QT) { st[tid] = SOFT16 ? ls0 + (walked - HIGH) : ls0; st[QT + tid] = dl0; }
-            if (KIND == RELU2 && Ty<T>::scaled && tid < QT) st[QT + tid] = ldexpf(2.f, (int)e0);
+            if (KIND == SOFTMAX && tid < QT) { st[tid] = dl0; st[QT + tid] = tp0; st[2 * QT + tid] = SOFT16 ? ls0 + (walked - HIGH) : ls0; }
+            if (KIND == RELU2 && Ty<T>::scaled && tid < QT) st[tid] = ldexpf(2.f, (int)e0);
         };
         __syncthreads();                                                                  // the previous head's tiles and table are no longer read
         if (ib < p.Lq) {
@@ -1304,7 +1313,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
                 }
             }
             if (SOFT16 && p.dO_exp) {
-                const float e = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(st[2 * QT])));
+                const float e = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(st[3 * QT])));
                 if (e > held) {
                     const float f = ldexpf(1.f, (int)(held - e));
                     held = e;
@@ -1319,15 +1328,18 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
             }
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
-                f4 ls = {0, 0, 0, 0}, dl = {0, 0, 0, 0};
-                if (KIND == SOFTMAX) ls = *reinterpret_cast<const f4 *>(st + n * 16 + g * 4);
-                if (KIND == SOFTMAX || Ty<T>::scaled) dl = *reinterpret_cast<const f4 *>(st + QT + n * 16 + g * 4);
+                f4 tp = {0, 0, 0, 0}, ls = {0, 0, 0, 0}, dl = {0, 0, 0, 0};
+                if (KIND == SOFTMAX || Ty<T>::scaled) dl = *reinterpret_cast<const f4 *>(st + n * 16 + g * 4);
+                if (KIND == SOFTMAX) {
+                    tp = *reinterpret_cast<const f4 *>(st + QT + n * 16 + g * 4);
+                    ls = *reinterpret_cast<const f4 *>(st + 2 * QT + n * 16 + g * 4);
+                }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float wgt;
-                        s[mt][n][r] = dscore<KIND, Ty<T>::scaled>(s[mt][n][r], wt[mt][n][r], ls[r], dl[r], dl[r], wgt);
+                        s[mt][n][r] = dscore<KIND, Ty<T>::scaled>(s[mt][n][r], wt[mt][n][r], tp[r], ls[r], dl[r], dl[r], wgt);
                         wt[mt][n][r] = wgt;
                     }
             }
