@@ -40,3 +40,13 @@ def test_rows_whose_keys_all_carry_a_large_bias(dtype, value):
         low = float(torch.finfo(dtype).min)
         _close(_case(dtype, 50, 300, [0.5, low, low], table_dtype=dtype), start=-500)
         _close(_case(dtype, 50, 300, [0.5, low, low], table_dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_order_of_the_largest_finite_biases(dtype):
+    """biases next to float32's largest numbers keep their order and stay finite: the larger one takes the row, equal ones share it"""
+    for values in ([-2.5e38, -2.3e38, -2.3e38], [-2.3e38, -2.5e38, -3.3e38], [-2.3e38] * 3, [2.3e38, 2.5e38, 3.3e38], [3.3e38, 2.5e38, 1e38], [-1.1e38, -0.9e38, -3.4e38], [2.2e38] * 3):
+        t = _case(dtype, 50, 300, values)
+        _close(t)
+        _close(t, start=-500)
+        _close(_case(dtype, 3, 1500, values), start=700)

@@ -34,7 +34,7 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float NEG = -3.0e38f;                 // running maximum before the first key: finite, below every score
+constexpr float NEG = -3.402823466e38f;         // running maximum before the first key: the lowest finite number, so no score lies below it
 
 struct Args {
     const void *q, *k, *v, *gate;
@@ -264,7 +264,7 @@ template <int N, int B, class V8, class Load, class Use> __device__ __forceinlin
 }
 // The learned table over distances of head h, in LDS: -D .. D with MARGIN more entries of the end values on both sides, so that a tile that reaches
 // across +-D is looked up without clipping (a wave's tile spans fewer than MARGIN distances).  Softmax works in powers of two, so its bias carries
-// log2 e (finite values stay finite).
+// log2 e; beyond 1e38 the factor is 0.8, so that finite values stay finite and in order (two that differ there differ by 1e31 and more).
 constexpr int MARGIN = 128;
 __host__ __device__ __forceinline__ int table_width(int D) { return 2 * D + 1 + 2 * MARGIN; }
 template <class T, int KIND> __device__ __forceinline__ void expand_bias(const Args &p, int h, float *dst, int nth)
@@ -276,8 +276,8 @@ template <class T, int KIND> __device__ __forceinline__ void expand_bias(const A
         const long long at = (long long)b * p.H + h;
         float x = p.table_f32 ? reinterpret_cast<const float *>(p.table)[at] : (float)reinterpret_cast<const T *>(p.table)[at];
         if (KIND == SOFTMAX) {
-            const float y = x * LOG2E;
-            x = (__builtin_isinf(y) && !__builtin_isinf(x)) ? (x < 0.f ? -1.0e38f : 1.0e38f) : y;
+            const float a = fabsf(x);
+            x = a > 1.0e38f && a < INFINITY ? copysignf(1.0e38f * LOG2E + (a - 1.0e38f) * 0.8f, x) : x * LOG2E;
         }
         dst[t] = x;
     }
