@@ -9,7 +9,7 @@ operators of their own, for the head's 17 tokens as for long sequences, padded b
 
 Both are asynchronous on torch's current stream of the tensors' device, allocate through torch (so they can be captured into a graph), take no
 CPU tensors (there is no CPU fallback) and raise ``TlkError`` for arguments they do not take.  Gradients come through torch's autograd; they
-are computed without atomics: equal inputs give equal bits.  To capture a backward pass into a graph, use leaves of which no eager autograd
+are computed without atomics: equal inputs give equal bits.  Forward-mode derivatives are refused.  To capture a backward pass into a graph, use leaves of which no eager autograd
 graph is alive (torch ties a leaf's accumulation to the stream of its first use).
 """
 from __future__ import annotations
@@ -20,6 +20,7 @@ import struct
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import TlkError, _dtype_code, check, lib
@@ -69,6 +70,12 @@ def _bound():
 def _need(ok, what):
     if not ok:
         raise TlkError(what)
+
+
+def _no_tangent(what, *tensors):
+    """the operators have no forward-mode derivative: a tangent would be lost without a word.  (Tangents live inside a level alone; asking every tensor takes 4 us.)"""
+    for t in tensors if getattr(forward_ad, "_current_level", 0) >= 0 else ():
+        _need(t is None or forward_ad.unpack_dual(t).tangent is None, what + ": no forward-mode derivatives")
 
 
 def _ptr(t):
@@ -242,6 +249,7 @@ def gated_attention(q, k, v, gate=None, *, kind="relu2", scale=None, bias=None, 
     if dv % vn:
         v, gate = F.pad(v, (0, -dv % vn)), F.pad(gate, (0, -dv % vn)) if gate is not None else None
     args = (q, k, v, gate, bias, buckets, lens, q_start, KINDS[kind], bool(causal), scale)
+    _no_tangent("gated_attention", q, k, v, gate, bias)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (gate is not None and gate.requires_grad) or (bias is not None and bias.requires_grad)):
         out = _GatedAttention.apply(*args)
     else:
@@ -362,6 +370,7 @@ def norm_gate_residual(h, residual=None, *, norm=None, weight=None, bias=None, e
             gate_rows = max(1, gate_rows)
     small = [t.contiguous() if t is not None else None for t in (res_scale, weight, bias, next_weight, next_bias)]
     args = (h, residual, gate, *small, n1, n2, float(eps), float(next_eps), gate_rows)
+    _no_tangent("norm_gate_residual", *args[:8])
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8]):
         return _NormGateResidual.apply(*args)
     return _joint_forward(*args)
