@@ -375,3 +375,33 @@ def test_import_from_a_hand_written_rtmlib_style_onnx_file(tmp_path):
     rep = W.load_checkpoint(dst2, str(path), (x,))
     with torch.no_grad():
         assert torch.equal(dst2(x), src(x)), rep
+
+
+def test_rtmpose_with_a_position_bias_takes_a_plain_file(tmp_path):
+    """The reference's files hold no position bias: with one of zeros the imported network is the file's, and the report names what the file did not hold; a bias that is not
+    zero, and stays, comes with a warning (strict_heads: an error).  The bias takes nothing from the seeded weights."""
+    from tracklab_amd.backbones.rtmpose import rtmpose
+    new = lambda **kw: rtmpose("t", device="cpu", dtype=torch.float32, channels_last=False, **kw)      # noqa: E731
+    plain, biased = new(seed=4), new(seed=4, rel_buckets=8)
+    assert not biased.gau.rel_bias.any()
+    for k, v in plain.state_dict().items():
+        assert torch.equal(v, biased.state_dict()[k]), k
+    with torch.no_grad():
+        g = torch.Generator().manual_seed(3)
+        for p in plain.parameters():
+            p.add_(torch.randn(p.shape, generator=g) * 0.02)
+    x = torch.randn(1, 3, 256, 192, generator=torch.Generator().manual_seed(2))
+    path = tmp_path / "pose.onnx"
+    path.write_bytes(W.export_onnx_bytes(plain, (x,)))
+    dst = new(seed=5, rel_buckets=8)
+    rep = W.load_checkpoint(dst, path, (x,))
+    assert rep["kept"] == ["gau.rel_bias"] and rep["tensors"] == len(plain.state_dict())
+    with torch.no_grad():
+        for p, q in zip(plain(x), dst(x)):
+            assert torch.equal(p, q)
+        dst.gau.rel_bias[2] = 0.5
+    with pytest.warns(RuntimeWarning, match="gau.rel_bias"):
+        assert W.load_checkpoint(dst, path, (x,))["kept"] == ["gau.rel_bias"]
+    with pytest.raises(ValueError, match="gau.rel_bias"):
+        W.load_checkpoint(dst, path, (x,), strict_heads=True)
+    assert "kept" not in W.load_checkpoint(new(seed=5), path, (x,))

@@ -235,9 +235,12 @@ class RTMPoseNet(nn.Module):
 
 
 def rtmpose(size="m", device="cuda", dtype=torch.float16, channels_last=True, seed=0, rel_buckets=0):
-    """rel_buckets > 0: the head's attention unit learns a position bias over the keypoint tokens (GAU)"""
+    """rel_buckets > 0: the head's attention unit has a position bias over the keypoint tokens (GAU), zero until it is learned or loaded"""
     widen, deepen = {"t": (0.375, 0.167), "s": (0.5, 0.33), "m": (0.75, 0.67), "l": (1.0, 1.0)}[size]
-    net = random_init_(RTMPoseNet(widen, deepen, rel_buckets=rel_buckets), seed)
+    net = RTMPoseNet(widen, deepen, rel_buckets=rel_buckets)
+    rel_bias, net.gau.rel_bias = net.gau.rel_bias, None       # zero until it is learned or loaded, and no part of the seeded weights
+    random_init_(net, seed)
+    net.gau.rel_bias = rel_bias
     with torch.no_grad():                      # random_init_ zeroes every 1-D parameter (biases); the norm gains are 1-D too
         for m in net.modules():
             if isinstance(m, ScaleNorm):

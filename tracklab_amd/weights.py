@@ -492,7 +492,8 @@ def export_onnx_bytes(module, example_inputs) -> bytes:
 
 def import_onnx_weights(module, example_inputs, ref, strict: bool = True):
     """Copy the weights of the ONNX model `ref` (path / bytes / OnnxGraph) into `module` (same architecture, e.g. backbones.yolox.YOLOX for the
-    rtmlib YOLOX file). `module` must be on the CPU in float32 for the export; returns the number of tensors written."""
+    rtmlib YOLOX file). `module` must be on the CPU in float32 for the export; returns the number of tensors written (the
+    module's entries that `ref` does not hold stay as they are: `import_onnx_weights.kept`)."""
     import torch
     ref_g = ref if isinstance(ref, OnnxGraph) else read_onnx(ref)
     sd = module.state_dict()
@@ -513,7 +514,7 @@ def import_onnx_weights(module, example_inputs, ref, strict: bool = True):
     pairs, unmatched = match_convolutions(ref_g, own_g, set(sd))
     if strict and unmatched:
         raise ValueError(f"weight import: elementwise parameters without a structural partner in the reference graph: {unmatched}")
-    written = 0
+    written, done = 0, set()
     with torch.no_grad():
         for ow, ob, rw, rb in pairs:
             for key, arr in ((ow, rw), (ob, rb)):
@@ -530,7 +531,9 @@ def import_onnx_weights(module, example_inputs, ref, strict: bool = True):
                     raise ValueError(f"{key}: reference tensor {tuple(t.shape)} does not fit {tuple(sd[key].shape)}")
                 sd[key].copy_(t.reshape(sd[key].shape))
                 written += 1
+                done.add(key)
     import_onnx_weights.unmatched = unmatched
+    import_onnx_weights.kept = sorted(set(sd) - done)
     return written
 
 
@@ -574,7 +577,8 @@ def load_checkpoint(module, path, example_inputs=None, backbone_attr="backbone",
 
     * ``*.onnx`` -- the artefact the reference itself loads for its detector / pose estimator (rtmlib model zoo,
       configs/modules/bbox_detector/yolox_rtmlib.yaml:1-7): imported structurally (`import_onnx_weights`) through a CPU fp32 twin of `module`;
-      `example_inputs` = a tuple with one input of the network's shape.
+      `example_inputs` = a tuple with one input of the network's shape.  Entries of `module` that the file does not hold (a position bias, say) stay, and are
+      reported as ``kept``; with a WARNING where one is not zero (``strict_heads=True``: an error).
     * a torch checkpoint whose keys are `module`'s own -> `load_state_dict`.
     * a torch checkpoint of a ResNet-50 WITH BatchNorm layers in torchvision / torchreid naming (optionally under a prefix, optionally wrapped in
       {"state_dict": ...}; tracklab/wrappers/reid/kpreid_api.py:133-161 loads such files through torchreid): the backbone is folded
@@ -594,8 +598,18 @@ def load_checkpoint(module, path, example_inputs=None, backbone_attr="backbone",
             raise ValueError("load_checkpoint: an ONNX file needs example_inputs (one input tensor of the network's shape)")
         twin = copy.deepcopy(module).to(device="cpu", dtype=torch.float32).to(memory_format=torch.contiguous_format)
         n = import_onnx_weights(twin, tuple(t.detach().to("cpu", torch.float32) for t in example_inputs), path)
+        kept = import_onnx_weights.kept
+        left = [k for k in kept if bool(twin.state_dict()[k].any())]
+        if left:
+            msg = f"checkpoint {path!r}: it does not hold {left[:6]}{' ...' if len(left) > 6 else ''} of {type(module).__name__}, which are not zero and stay as they are"
+            if strict_heads:
+                raise ValueError(msg)
+            import logging
+            import warnings
+            logging.getLogger("tracklab_amd.weights").warning(msg)
+            warnings.warn(msg, RuntimeWarning, stacklevel=2)
         module.load_state_dict(twin.state_dict())
-        return {"format": "onnx", "tensors": n}
+        return {"format": "onnx", "tensors": n, **({"kept": kept} if kept else {})}
     sd = torch.load(path, map_location="cpu", weights_only=True)
     if isinstance(sd, dict) and "state_dict" in sd and isinstance(sd["state_dict"], dict):
         sd = sd["state_dict"]
