@@ -10,14 +10,17 @@ HALF = 2.0 ** -25                              # half of float16's smallest step
 
 
 def _close(got, want, names):
-    """the norm of the error over the entries within the type; an entry beyond its largest number (65520 and more round to infinity) is the infinity of its sign"""
+    """the norm of the error over the entries within the type; an entry beyond its largest number (65520 and more round to infinity) is the infinity of its sign.
+    An entry sum_j a_j b_jc whose factors a_j (a row's dO, weights or score gradients) were rounded is off by u / sqrt(3) of sqrt(sum_j a_j^2 b_jc^2), which is the root mean
+    square of its row whatever the entry itself came to: the small entries of a row whose large ones are infinite keep an error of the row's size.  So the bound is
+    u of the norm of all entries, those beyond the type among them."""
     u = X.U[F16]
     for n in names:
         a, b = got[n].double(), want[n]
         fits, beyond = b.abs() < 65504 * (1 - 4 * u), b.abs() > 65520 * (1 + 4 * u)
         assert torch.equal(a[beyond], b[beyond].sign() * float("inf")) and bool(a[fits].isfinite().all()), n
-        a, b = a[fits], b[fits]
         lim = 1.05 * u * float(b.norm()) + HALF * b.numel() ** 0.5
+        a, b = a[fits], b[fits]
         assert float((a - b).norm()) <= lim, (n, X.off(a, b), lim / float(b.norm()))
 
 
@@ -83,3 +86,16 @@ def test_values_before_the_gate_beyond_the_largest_number():
         got, want = X.run(t, "relu2"), X.attention(t, "relu2")
         assert float((want["dgate"].abs() / t["dout"].double().abs().clamp(min=1e-30)).max()) > 65504
         _close(got, want, ("out", "dgate", "dv"))
+
+
+@pytest.mark.parametrize("first", [320, 333])
+@pytest.mark.parametrize("kind", ["relu2", "softmax"])
+def test_keys_that_only_small_rows_see(kind, first):
+    """causal: from row ``first`` on dout * gate lies 2^-24 behind the rows before it, so the keys from there on have nothing but small rows; their gradients are as
+    exact as the others', whatever larger rows are worked on beside them"""
+    t = X.inputs(7, F16, 1, 640, 640, 1, 1, 64, 64, True, 0, std={"dout": 2.0 ** 9, "gate": 2.0 ** 8, "v": 2.0 ** -2, "q": 0.5, "k": 0.5})
+    t["gate"][:, first:] *= 2.0 ** -12
+    t["dout"][:, first:] *= 2.0 ** -12
+    got, want = X.run(t, kind, True), X.attention(t, kind, True)
+    _close({n: got[n][:, first:] for n in got}, {n: want[n][:, first:] for n in want}, ("dq", "dk", "dv", "dgate"))
+    _close(got, want, ("dq", "dk", "dv", "dgate"))

@@ -726,7 +726,6 @@ template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(c
 // behind the gate: dO = dout * gate, dgate = dout * O, delta = sum_d dO * O.  LANES lanes a row; bound by HBM (4 x 4096 rows of 1024 bf16: 28 us, 5 tensors of 34 MB, which the caches hold in part).
 // float16: dO stands at a power of two of its row, which puts the largest magnitude at 2^14 .. 2^15 -- the product of two float16 values reaches from 2^-48 to 2^32.
 // low: what rounding dO left; the product of two 16-bit values is dO + low exactly (16 bits of bfloat16, 22 of float16), and delta is formed from it.
-constexpr int NO_ROW = -100;                      // dO_exp of a row of zeros: below every other
 template <class T> struct GateArgs {
     const T *dout, *gate;
     const void *o;
@@ -756,7 +755,6 @@ template <class T, class O, int LANES> __global__ void __launch_bounds__(256) ga
             top = lanes_all<LaneMax, LANES>(top);
             int e = 0;                                            // (infinite: as it is)
             if (top < INFINITY) (void)frexpf(top, &e), e -= 15;
-            if (top == 0.f) e = NO_ROW;
             scale = ldexpf(1.f, -e);
             if (lane == 0) p.dO_exp[row] = (float)e;
         }
@@ -1155,9 +1153,9 @@ template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
 __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK + DVC == 256) ? 1 : 2) dkv_kernel(const Args p)
 {
     using V8 = typename Ty<T>::V8;
-    // float16 softmax: weights are at most 1, and 2^14 higher none above 2^-28 is subnormal.  Behind a gate a weight takes 2^e of its row's dO, and the largest e
-    // of the rows walked so far goes off all of them: one power of two, raised with the walk, that comes with the log-sum-exp; the score gradients carry it too.
-    // (An exponent for every key, as the squares have: 6 x 1021 tokens, 8 heads, 72 and 104 columns 124 us; factors of the weights 132; so 119.)
+    // float16 softmax: weights are at most 1, so one fixed power of two does for them: 2^14 higher none above 2^-28 is subnormal.  It comes with the row's sum, for
+    // nothing; the score gradients carry it too.  Behind a gate a weight takes 2^e of its row's dO, and rows that differ in it meet in a key: an exponent for every
+    // key, as the squares have (6 x 1021 tokens, 8 heads, 72 and 104 columns: 133 us, one power of two a workgroup 118, which lost keys that small rows alone see).
     constexpr bool SOFT16 = KIND == SOFTMAX && Ty<T>::scaled;
     constexpr float HIGH = 14.f;
     constexpr int QT = 32, NTH = 64 * W, BN = W * MT * 16, NS = 2;
@@ -1165,7 +1163,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
     using TO = Tile<T, QT, DVC, W>;
     constexpr int BUF = TQ::BYTES + TO::BYTES;
     __shared__ __attribute__((aligned(1024))) char buf0[BUF], buf1[ONE ? 16 : BUF];     // (two objects: see fwd_kernel)
-    __shared__ __attribute__((aligned(16))) float stats0[3 * QT + 4], stats1[3 * QT + 4];       // the tiles' delta (float16 relu^2: 2 * 2^e), maximum, log2 of the sum, power of two (SOFT16)
+    __shared__ __attribute__((aligned(16))) float stats0[3 * QT], stats1[3 * QT];       // the tiles' delta (float16 relu^2: 2 * 2^e), maximum, log2 of the sum
     extern __shared__ __attribute__((aligned(16))) float tab[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, l = lane & 15, G = p.H / p.Hk, TW = table_width(p.D);
     int id = blockIdx.x;
@@ -1196,7 +1194,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         for (int n = 0; n < DK / 16; ++n) ak[n][mt] = f4{0, 0, 0, 0};
     }
     int ev[MT], ek[MT];
-    float walked = p.dO_exp ? (float)NO_ROW : 0.f, held = walked;                       // SOFT16: the rows' largest e so far (the first wave's), and what the sums stand at
+    const float high = SOFT16 && !p.dO_exp ? HIGH : 0.f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) ev[mt] = ek[mt] = E_NONE;
     const float sc = KIND == SOFTMAX ? p.scale * LOG2E : p.scale;
@@ -1223,7 +1221,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
             if ((KIND == SOFTMAX || Ty<T>::scaled) && tid < QT) {
                 const long long row = ((long long)b * p.Lq + i + tid) * p.H + h;
                 const bool ok = i + tid < p.Lq;
-                if (Ty<T>::scaled) e0 = !p.dO_exp ? 0.f : (ok ? p.dO_exp[row] : (float)NO_ROW);
+                if (Ty<T>::scaled) e0 = p.dO_exp && ok ? p.dO_exp[row] : 0.f;
                 if (KIND == SOFTMAX) {
                     tp0 = ok ? p.lse[2 * row] : 0.f;
                     ls0 = ok ? p.lse[2 * row + 1] - e0 : INFINITY;
@@ -1232,11 +1230,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
             }
         };
         const auto keep = [&](float *st) __attribute__((always_inline)) {
-            if (SOFT16 && p.dO_exp && w == 0) {
-                walked = fmaxf(walked, lanes_all<LaneMax, 32>(e0));
-                if (tid == 0) st[3 * QT] = walked;
-            }
-            if (KIND == SOFTMAX && tid < QT) { st[tid] = dl0; st[QT + tid] = tp0; st[2 * QT + tid] = SOFT16 ? ls0 + (walked - HIGH) : ls0; }
+            if (KIND == SOFTMAX && tid < QT) { st[tid] = dl0; st[QT + tid] = tp0; st[2 * QT + tid] = ls0 - high; }
             if (KIND == RELU2 && Ty<T>::scaled && tid < QT) st[tid] = ldexpf(2.f, (int)e0);
         };
         __syncthreads();                                                                  // the previous head's tiles and table are no longer read
@@ -1312,20 +1306,6 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
                     }
                 }
             }
-            if (SOFT16 && p.dO_exp) {
-                const float e = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(st[3 * QT])));
-                if (e > held) {
-                    const float f = ldexpf(1.f, (int)(held - e));
-                    held = e;
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                        for (int n = 0; n < DVC / 16; ++n) av[n][mt] *= f;
-#pragma unroll
-                        for (int n = 0; n < DK / 16; ++n) ak[n][mt] *= f;
-                    }
-                }
-            }
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
                 f4 tp = {0, 0, 0, 0}, ls = {0, 0, 0, 0}, dl = {0, 0, 0, 0};
@@ -1346,7 +1326,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
             V8 wb[MT], db[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const float fv = SOFT16 ? 1.f : hold<T, NS>(wt[mt], ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
+                const float fv = high != 0.f ? 1.f : hold<T, NS>(wt[mt], ev[mt]), fk = hold<T, NS>(s[mt], ek[mt]);
                 if (Ty<T>::scaled && __any(fv != 1.f))
 #pragma unroll
                     for (int n = 0; n < DVC / 16; ++n) av[n][mt] *= fv;
@@ -1382,7 +1362,7 @@ __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK
         const int j = j0 + mt * 16 + l;
         if (j >= p.Lk) continue;
         const long long row = ((long long)b * p.Lk + j) * p.Hk + hk;
-        const float down = SOFT16 ? ldexpf(1.f, (int)(held - HIGH)) : 1.f, finv = SOFT16 ? down : unhold<T>(ev[mt]) * (Ty<T>::scaled ? 0.5f : 1.f),
+        const float down = ldexpf(1.f, -(int)high), finv = high != 0.f ? down : unhold<T>(ev[mt]) * (Ty<T>::scaled && KIND == RELU2 ? 0.5f : 1.f),
                     fink = p.scale * unhold<T>(ek[mt]) * down;
         typename Ty<T>::V4 y;
 #pragma unroll

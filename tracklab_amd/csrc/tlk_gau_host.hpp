@@ -225,8 +225,8 @@ template <class T, int KIND, int DK, int DVC, int W> int launch_dkv(const Args &
     const size_t fixed = sizeof(T) * 32 * (tile_width(DK) + DVC), smem = a.table ? sizeof(float) * table_width(a.D) : 0;
     const long long blocks = (long long)a.B * a.Hk * f.nchunk * f.nparts * f.nrow_k;
     if constexpr (W < 4)
-        if (a.Lq <= 32) return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, true>, blocks, 64 * W, fixed + 800, smem, a, st);
-    return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, false>, blocks, 64 * W, 2 * fixed + 800, smem, a, st);
+        if (a.Lq <= 32) return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, true>, blocks, 64 * W, fixed + 768, smem, a, st);
+    return launch(dkv_kernel<T, KIND, DK, DVC, MT, W, false>, blocks, 64 * W, 2 * fixed + 768, smem, a, st);
 }
 template <class T, int KIND, int DK, int DVC> int pick_bwd(Args a, const BwdPlan &f, hipStream_t st)
 {
