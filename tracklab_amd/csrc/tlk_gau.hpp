@@ -723,7 +723,7 @@ template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(c
 }
 
 // ----------------------------------------------------------------------------------------------------------------------------------- backward
-// behind the gate: dO = dout * gate, dgate = dout * O, delta = sum_d dO * O.  LANES lanes a row; bound by HBM (4 x 4096 rows of 1024 bf16: 28 us, 5 tensors of 34 MB, which the caches hold in part).
+// behind the gate: dO = dout * gate, dgate = dout * O, delta = sum_d dO * O.  LANES lanes a row; bound by HBM (4 x 4096 rows of 1024 bf16: 34 us, 6 tensors of 34 MB, which the caches hold in part).
 // float16: dO stands at a power of two of its row, which puts the largest magnitude at 2^14 .. 2^15 -- the product of two float16 values reaches from 2^-48 to 2^32.
 // low: what rounding dO left; the product of two 16-bit values is dO + low exactly (16 bits of bfloat16, 22 of float16), and delta is formed from it.
 template <class T> struct GateArgs {
@@ -1148,7 +1148,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
 }
 
 // dK and dV: W waves, MT x 16 keys each; walks the queries of every head that shares the keys.  S has a key in the column: W and dS in registers
-// are the B operands of dV^T = dO^T W and dK^T = Q^T dS.  Bound as dq, with four products and twice the accumulators: 254 and 112 us at its two sizes.
+// are the B operands of dV^T = dO^T W and dK^T = Q^T dS.  Bound as dq, with four products and twice the accumulators: 251 and 111 us at its two sizes.
 template <class T, int KIND, int DK, int DVC, int MT, int W, bool ONE>
 __global__ void __launch_bounds__(64 * W, DK + DVC > 256 || (Ty<T>::scaled && DK + DVC == 256) ? 1 : 2) dkv_kernel(const Args p)
 {

@@ -254,11 +254,12 @@ template <class T, int LPR, int NV, int V> __global__ void __launch_bounds__(256
 }
 
 // One backward workgroup of 512 threads per CU walks rows in turn, 512 / LPR of them at a time.  The next rows' five tensors are fetched while the present
-// ones pass their four reductions: a lane holds 8 values of a row (16 of the widest), so that its sums and two rows' data fit the registers.
+// ones pass their four reductions: a lane holds 8 values of a row, so that its sums and two rows' data fit the registers.  Rows of more than 4096 columns put 16 in a lane, and
+// what does not fit goes to memory: 8192 x 8192 bf16 500 us lean and 1218 with all six arrays (192 and 384 bytes of scratch a lane), float32 1323 and 1661 (452 and 644).
 constexpr int BT = 512;
 
 // LEAN: no layer norm and no shared gate, so only res_scale and the two weights have column sums -- half the registers of a lane's sums, which is what
-// lets the rows' loads stay in flight (4096 columns bf16: with all six arrays the sums spilled, 674 us; lean 0 bytes spilled)
+// lets the rows' loads stay in flight (16384 rows of 4096 bf16: 240 us, with all six arrays 320)
 template <class T, int LPR, int NV, int V, bool LEAN> __global__ void __attribute__((amdgpu_flat_work_group_size(BT, BT), amdgpu_waves_per_eu(2, 2))) joint_bwd_kernel(const NormArgs p)
 {
     using R = Row<T, LPR, NV, V>;
@@ -454,16 +455,16 @@ template <class T, int LPR, int NV, int V> int fwd_launch(const NormArgs &a, hip
 }
 template <class T, int LPR, int NV, int V> int bwd_launch(const NormArgs &a, hipStream_t st)
 {
+    static_assert(BT * NV * V * sizeof(float) <= 48 * 1024, "dynamic LDS that needs no attribute");
     const size_t smem = (size_t)BT * NV * V * sizeof(float);
     const bool lean = a.slot[A_GATE] < 0 && a.slot[A_B1] < 0 && a.slot[A_B2] < 0;
     const auto kernel = lean ? joint_bwd_kernel<T, LPR, NV, V, true> : joint_bwd_kernel<T, LPR, NV, V, false>;
-    if (smem > 48 * 1024) TLK_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
     hipLaunchKernelGGL(kernel, dim3((unsigned)(a.groups * a.per_group)), dim3(BT), smem, st, a);
     TLK_HIP(hipGetLastError());
     return TLK_OK;
 }
 
-// lanes a row: forward at most 16 values a lane (8192 columns of float32: 32), backward 8 (16)
+// lanes a row: forward at most 16 values a lane (beyond 4096 columns: 32), backward 8 (16)
 template <class T> int pick_fwd(const NormArgs &a, bool vec, hipStream_t st)
 {
     constexpr int V = 16 / sizeof(T);
