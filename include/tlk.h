@@ -848,7 +848,8 @@ int tlk_reid_part_head(const void *feat_dev, int feat_pix_stride, int dtype, int
  *   a row's largest x = S log2 e and log2 sum_j 2^(x_j - largest), the latter +inf for a row without keys: what the backward call takes.  Products run on the matrix cores in `dtype` and are summed in float32; weights are rounded to `dtype` for the second product
  *   (float16: with a power of two per row, so weights beyond its range survive), o and out once.
  * tlk_gau_attention_bwd:  dout, o_raw (needed with a gate or softmax), lse (softmax) -> dq, dk, dv, dgate (with a gate), dtable (with a table); weights
- *   are formed again from q and k.  With shared key heads the gradients of the sharing heads are summed in float32.  No atomics: equal bits on every run.
+ *   are formed again from q and k.  With shared key heads the gradients of the sharing heads are summed in float32.  dtable takes up no rounding of dout * gate, of
+ *   the weights or of o.  No atomics: equal bits on every run.
  * Workspace: device memory of at least tlk_gau_attention_workspace(args, backward) bytes (-1..: an error code; forward: 0 up to 512 keys), 16-byte aligned, not shared by
  *   calls that may overlap. */
 enum { TLK_GAU_RELU2 = 0, TLK_GAU_SOFTMAX = 1 };
