@@ -52,7 +52,7 @@ struct Args {
     const void *dO;                             // (B, Lq, H, dv) contiguous: the gradient behind the gate
     const void *dO_low;                         // the same shape: what dO's rounding left (16-bit types with a gate and a table)
     const float *dO_exp;                        // (B, Lq, H): dO stands at 2^-dO_exp of its row (float16 with a gate; null: as it is)
-    const float *delta;                         // (B, Lq, H): sum_d dO o (softmax), at dO's scale
+    const float *delta, *delta_q;               // (B, Lq, H): sum_d dO o (softmax), at dO's scale; dq's with both parts of dO
     void *dq, *dk_, *dv_;
     float *dq_part, *dk_part, *dv_part;         // (chunk, B, Lq, H, dk); (chunk x part, B, Lk, Hk, dk), (part, B, Lk, Hk, dv): sums of several blocks, joined afterwards
     float *db_part;                             // (heads, B * chunk * nrow * waves, 2 D + 1)
@@ -725,13 +725,14 @@ template <class T, int KIND> __global__ void __launch_bounds__(64) join_kernel(c
 // ----------------------------------------------------------------------------------------------------------------------------------- backward
 // behind the gate: dO = dout * gate, dgate = dout * O, delta = sum_d dO * O.  LANES lanes a row; bound by HBM (4 x 4096 rows of 1024 bf16: 34 us, 6 tensors of 34 MB, which the caches hold in part).
 // float16: dO stands at a power of two of its row, which puts the largest magnitude at 2^14 .. 2^15 -- the product of two float16 values reaches from 2^-48 to 2^32.
-// low: what rounding dO left; the product of two 16-bit values is dO + low exactly (16 bits of bfloat16, 22 of float16), and delta is formed from it.
+// low: what rounding dO left; the product of two 16-bit values is dO + low exactly (16 bits of bfloat16, 22 of float16).  Each kernel is given the delta of the dO that it multiplies: where
+// a row sees one key, dW - delta is nothing, and one with low and one without would leave low . o of it.
 template <class T> struct GateArgs {
     const T *dout, *gate;
     const void *o;
     long long gs[3];
     T *dO, *low, *dgate;
-    float *delta, *dO_exp;
+    float *delta, *delta_q, *dO_exp;
     long long rows;
     int Lq, H, dv;
 };
@@ -743,7 +744,7 @@ template <class T, class O, int LANES> __global__ void __launch_bounds__(256) ga
     if (row >= p.rows) return;
     const long long bi = row / p.H;
     const T *gp = p.gate ? p.gate + (bi / p.Lq) * p.gs[0] + (bi % p.Lq) * p.gs[1] + (row % p.H) * p.gs[2] : nullptr;
-    float d = 0.f, scale = 1.f;
+    float d = 0.f, d_low = 0.f, scale = 1.f;
     if constexpr (Ty<T>::scaled)
         if (gp) {
             float top = 0.f;
@@ -770,7 +771,8 @@ template <class T, class O, int LANES> __global__ void __launch_bounds__(256) ga
                 a[r] = (T)x;
                 rest[r] = (T)(x - (float)a[r]);
                 b[r] = (T)((float)du[r] * (float)o[r]);
-                d += (p.low ? x : (float)a[r]) * (float)o[r];
+                d += (float)a[r] * (float)o[r];
+                d_low += (float)rest[r] * (float)o[r];
             }
             *reinterpret_cast<V4 *>(p.dO + row * p.dv + c) = a;
             if (p.low) *reinterpret_cast<V4 *>(p.low + row * p.dv + c) = rest;
@@ -782,6 +784,9 @@ template <class T, class O, int LANES> __global__ void __launch_bounds__(256) ga
     }
     d = lanes_all<LaneAdd, LANES>(d);
     if (p.delta && lane == 0) p.delta[row] = d;
+    if (!p.low || !p.delta) return;                               // (uniform over the launch)
+    d_low = lanes_all<LaneAdd, LANES>(d_low);
+    if (lane == 0) p.delta_q[row] = d + d_low;
 }
 
 // dS of one pair from its score x (scaled, biased, masked: -inf; softmax in powers of two), dW and the row's statistics; w returns the weight.  Where dO, and dW
@@ -889,7 +894,7 @@ __global__ void __launch_bounds__(64 * W, LOW && DVC == 256 ? 1 : 2) dq_kernel(c
         }
         top[mt] = KIND == SOFTMAX && ok ? p.lse[2 * row] : 0.f;
         lsum[mt] = KIND == SOFTMAX ? (ok ? p.lse[2 * row + 1] : INFINITY) : 0.f;
-        del[mt] = KIND == SOFTMAX && ok && ch == 0 ? p.delta[row] : 0.f;              // (dW comes in chunks of dv: the subtraction belongs to one of them)
+        del[mt] = KIND == SOFTMAX && ok && ch == 0 ? p.delta_q[row] : 0.f;              // (dW comes in chunks of dv: the subtraction belongs to one of them)
         if constexpr (Ty<T>::scaled) {
             const float e = p.dO_exp && ok ? p.dO_exp[row] : 0.f;
             up[mt] = ldexpf(1.f, (int)e);

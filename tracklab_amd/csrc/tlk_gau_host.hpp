@@ -74,7 +74,7 @@ inline BwdPlan plan_backward(const Args &a, int elem)
 constexpr int DB_SPLITS = 64;
 
 struct BwdWs {
-    long long dO, low, exp, delta, dq, dk, dv, db, db2, total;
+    long long dO, low, exp, delta, delta_q, dq, dk, dv, db, db2, total;
 };
 inline BwdWs layout_backward(const Args &a, int kind, int elem, const BwdPlan &f)
 {
@@ -86,6 +86,7 @@ inline BwdWs layout_backward(const Args &a, int kind, int elem, const BwdPlan &f
     w.low = take(a.gate && a.table && elem == 2 ? rows * a.dv * elem : 0);
     w.exp = take(a.gate && elem == 2 ? rows * 4 : 0);
     w.delta = take(kind == SOFTMAX ? rows * 4 : 0);
+    w.delta_q = take(kind == SOFTMAX && a.gate && a.table && elem == 2 ? rows * 4 : 0);
     w.dq = take(f.nchunk > 1 ? rows * a.dk * f.nchunk * 4 : 0);
     w.dk = take(f.nchunk * f.nparts > 1 ? keys * a.dk * f.nchunk * f.nparts * 4 : 0);
     w.dv = take(f.nparts > 1 ? keys * a.dv * f.nparts * 4 : 0);
@@ -269,6 +270,7 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
         ga.dO_exp = a.gate && Ty<T>::scaled ? reinterpret_cast<float *>(ws + w.exp) : nullptr;
         ga.dgate = reinterpret_cast<T *>(io.dgate);
         ga.delta = kind == SOFTMAX ? reinterpret_cast<float *>(ws + w.delta) : nullptr;
+        ga.delta_q = kind == SOFTMAX && ga.low ? reinterpret_cast<float *>(ws + w.delta_q) : ga.delta;
         ga.rows = rows; ga.Lq = a.Lq; ga.H = a.H; ga.dv = a.dv;
         const int lanes = a.dv <= 64 ? 16 : (a.dv <= 128 ? 32 : 64);
         const long long blocks = (rows + 256 / lanes - 1) / (256 / lanes);
@@ -279,6 +281,7 @@ template <class T> int backward(Args a, const BwdIo &io, int kind, hipStream_t s
         TLK_HIP(hipGetLastError());
         if (a.gate) a.dO = ws + w.dO;
         a.delta = ga.delta;
+        a.delta_q = ga.delta_q;
         a.dO_low = ga.low;
         a.dO_exp = ga.dO_exp;
     }
